@@ -246,6 +246,122 @@ int kr_op_transpose(const void *src, void *dst, int R, int C, void *stream);
 void *kr_op_stream_create(void);
 int kr_op_stream_destroy(void *stream);
 
+/* ------------------------------------------------------------------------
+ * Paged key/value cache: what a program that goes on after the prompt needs
+ * (no counterpart in the reference, which stops at the prefill). Plain host
+ * structs; the pointers in them are device memory and outlive the calls.
+ */
+
+/* The cache of a model: k and v are [layers, pages, page_size, heads,
+ * head_dim] 16-bit tensors with the same strides (elements; rows of head_dim
+ * contiguous; strides positive, multiples of 8, below 2^31 but for the
+ * layers'). Token t of a sequence is row t % page_size of the page that its
+ * table names at t / page_size. page_size >= 1, head_dim 64 or 128. */
+typedef struct kr_cache {
+    void *k;
+    void *v;
+    int64_t layer_stride;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t layers;
+    int32_t pages;
+    int32_t page_size;
+    int32_t heads;
+    int32_t head_dim;
+    int32_t dtype; /* KR_BF16 or KR_F16 */
+} kr_cache;
+
+/* A launch's sequences. Sequence b has lens[b] tokens in the cache before the
+ * launch's own, and rows starts[b] .. starts[b+1]-1 of the launch are its new
+ * tokens (none is allowed), whose keys and values stand in the cache behind
+ * them, at positions lens[b], lens[b]+1, ..; table[b] names its pages.
+ * tree == NULL: a new token sees the cached ones, the new ones before it and
+ * itself. Otherwise row r's words tree[r * ld_tree ..] say which new tokens
+ * of its sequence it sees: bit j % 64 of word j / 64 for new token j (its own
+ * bit too); every cached one is seen.
+ * The arrays are read on the device when the launch runs, so a captured graph
+ * follows their contents. Nothing in them can lead outside the tensors: rows
+ * outside the launch's and new tokens past max_new are not worked, tokens past the
+ * table's end are not there, and the keys of a page id outside 0..pages-1 are
+ * seen by nobody. */
+typedef struct kr_seqs {
+    const int32_t *table;  /* [seqs, table_pages], row stride ld_table */
+    int64_t ld_table;
+    const int32_t *lens;   /* [seqs] */
+    const int32_t *starts; /* [seqs + 1], ascending */
+    const uint64_t *tree;  /* [rows of the launch, tree_words], row stride ld_tree; or NULL */
+    int64_t ld_tree;
+    int32_t table_pages;
+    int32_t seqs;
+    int32_t max_new;    /* no sequence has more new tokens; <= 64 * tree_words with a tree */
+    int32_t tree_words;
+} kr_seqs;
+
+/* Rotation tables [positions, head_dim] and, optionally, the gains of the
+ * per-head norms of q and k (both or none; of the activations' type).
+ * table_dtype: KR_F32 or the activations' type. chain != 0 rounds as the
+ * separate calls do (x * rstd, then the gain's product to 16 bits before the
+ * rotation: the bits of kr_op_rowop and kr_op_rope); 0 rounds once. */
+typedef struct kr_rope {
+    const void *cos_t;
+    const void *sin_t;
+    const void *q_gamma;
+    const void *k_gamma;
+    int64_t positions;
+    int32_t head_dim;
+    int32_t table_dtype;
+    int32_t chain;
+    float eps;
+} kr_rope;
+
+/* Per-head RMSNorm (with gammas) and rotate-half RoPE of q [rows, HQ, D] and
+ * k [rows, HKV, D] in one pass (D 64, 128 or 256; ld* = row strides, 0 =
+ * packed). Row r stands at positions[r] (NULL: r); a position outside the
+ * tables gives zero rows. An output may be its own input. Same role as
+ * kr_op_rowop's rmsnorm and kr_op_rope in sequence (reference EmitQkNorm,
+ * exec/qwen_main.cpp:1346-1357, and Rope, :567-582). */
+int kr_op_qk_norm_rope(int dtype, const kr_rope *rope, const void *q, int64_t ldq, const void *k, int64_t ldk,
+                       void *q_out, int64_t ldqo, void *k_out, int64_t ldko, const int64_t *positions, int rows,
+                       int HQ, int HKV, void *stream);
+
+/* The same with k and v [rows, heads, D] written to their cache slots
+ * (slots[r] = page * page_size + row in the page; outside the cache, -1 say:
+ * not written). No two rows may share a slot: it would hold a mixture. */
+int kr_op_qk_norm_rope_cache(const kr_rope *rope, const kr_cache *cache, int layer, const void *q, int64_t ldq,
+                             const void *k, int64_t ldk, const void *v, int64_t ldv, void *q_out, int64_t ldqo,
+                             const int64_t *positions, const int64_t *slots, int rows, int HQ, void *stream);
+
+/* Attention of a launch's new tokens over the pages: out [rows, HQ, D] (rows
+ * of no sequence are left alone), query head h reads key head h / (HQ /
+ * heads), scores scaled by `scale` (> 0). A row that sees no key gives zeros.
+ * What a row does not see has no part in its result, NaN and infinities
+ * included. ws / counters: caller-owned device memory of at least the sizes
+ * kr_op_attention_paged_workspace reports (functions of the handles' host
+ * fields alone), with which long sequences are cut into pieces that run side
+ * by side and are summed in order; the counters must be zero before the first
+ * call and are left zero; calls sharing them must be ordered. NULL: uncut.
+ * The bits depend on the sequences' lengths, not on when which piece ends. */
+int kr_op_attention_paged_workspace(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_bytes,
+                                    int *counters);
+int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                          void *out, int64_t ldo, int rows, int HQ, float scale, void *ws, size_t ws_bytes,
+                          int32_t *counters, int n_counters, void *stream);
+
+/* Page dst[i] becomes a copy of page src[i], keys and values of every layer.
+ * src and dst are HOST arrays, read during the call. Refused: ids outside the
+ * cache, a page named twice in dst, a page in both src and dst. */
+int kr_op_cache_copy_pages(const kr_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* After drafts have been accepted: for every layer's keys and values and each
+ * sequence b, the rows at positions lens[b] + path[b][i], i < path_lens[b],
+ * move to lens[b] + i, as if all were read before any is written. path:
+ * device [seqs, width], row stride ld_path, width <= 256; entries below 0 and
+ * rows off the table or the cache stay. Uses the handle's table and lens.
+ * Sequences must not share the pages of these rows. */
+int kr_op_cache_compact(const kr_cache *cache, const kr_seqs *seqs, const int32_t *path, int64_t ld_path, int width,
+                        const int32_t *path_lens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@
 
 #include "kr_gemm.h"
 #include "kr_misc.h"
+#include "kr_paged.h"
 #include "kr_rowops.h"
 
 static_assert(sizeof(kr_wait) == sizeof(kr::RelayWait), "kr_wait layout");
@@ -395,6 +396,108 @@ int kr_op_attention_split(int dtype, const void *q, int64_t ldq, const void *k, 
         sp.cnt_len = n_counters;
         kr::AttnLaunch(dtype, q, ldq, k, ldk, v, ldv, out, ldo, S_, HQ, HKV, D, scale, S(stream), &sp);
     });
+}
+
+int kr_op_qk_norm_rope(int dtype, const kr_rope *rope, const void *q, int64_t ldq, const void *k, int64_t ldk,
+                       void *q_out, int64_t ldqo, void *k_out, int64_t ldko, const int64_t *positions, int rows,
+                       int HQ, int HKV, void *stream)
+{
+    return Guard([&] {
+        if (rope == nullptr) throw std::runtime_error("qk_norm_rope: needs rotation tables");
+        kr::QkRopeDesc d;
+        d.rope = *rope;
+        d.dtype = dtype;
+        d.q = q;
+        d.k = k;
+        d.ldq = ldq;
+        d.ldk = ldk;
+        d.q_out = q_out;
+        d.k_out = k_out;
+        d.ldqo = ldqo;
+        d.ldko = ldko;
+        d.positions = positions;
+        d.rows = rows;
+        d.HQ = HQ;
+        d.HKV = HKV;
+        d.D = rope->head_dim;
+        kr::QkRopeLaunch(d, S(stream));
+    });
+}
+
+int kr_op_qk_norm_rope_cache(const kr_rope *rope, const kr_cache *cache, int layer, const void *q, int64_t ldq,
+                             const void *k, int64_t ldk, const void *v, int64_t ldv, void *q_out, int64_t ldqo,
+                             const int64_t *positions, const int64_t *slots, int rows, int HQ, void *stream)
+{
+    return Guard([&] {
+        if (rope == nullptr) throw std::runtime_error("qk_norm_rope_cache: needs rotation tables");
+        if (cache == nullptr) throw std::runtime_error("qk_norm_rope_cache: needs a cache");
+        if (rope->head_dim != cache->head_dim)
+            throw std::runtime_error("qk_norm_rope_cache: the tables and the cache differ in head_dim");
+        kr::QkRopeDesc d;
+        d.rope = *rope;
+        d.dtype = cache->dtype;
+        d.cache = cache;
+        d.layer = layer;
+        d.q = q;
+        d.k = k;
+        d.v = v;
+        d.ldq = ldq;
+        d.ldk = ldk;
+        d.ldv = ldv;
+        d.q_out = q_out;
+        d.ldqo = ldqo;
+        d.positions = positions;
+        d.slots = slots;
+        d.rows = rows;
+        d.HQ = HQ;
+        d.HKV = cache->heads;
+        d.D = cache->head_dim;
+        kr::QkRopeLaunch(d, S(stream));
+    });
+}
+
+int kr_op_attention_paged_workspace(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_bytes,
+                                    int *counters)
+{
+    return Guard([&] {
+        if (ws_bytes == nullptr || counters == nullptr) throw std::runtime_error("null output pointer");
+        kr::PagedAttnNeeds(cache, seqs, HQ, ws_bytes, counters);
+    });
+}
+
+int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                          void *out, int64_t ldo, int rows, int HQ, float scale, void *ws, size_t ws_bytes,
+                          int32_t *counters, int n_counters, void *stream)
+{
+    return Guard([&] {
+        kr::PagedAttnDesc d;
+        d.cache = cache;
+        d.seqs = seqs;
+        d.layer = layer;
+        d.q = q;
+        d.out = out;
+        d.ldq = ldq;
+        d.ldo = ldo;
+        d.rows = rows;
+        d.HQ = HQ;
+        d.scale = scale;
+        d.ws = ws;
+        d.ws_bytes = ws_bytes;
+        d.cnt = counters;
+        d.cnt_len = n_counters;
+        kr::PagedAttnLaunch(d, S(stream));
+    });
+}
+
+int kr_op_cache_copy_pages(const kr_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream)
+{
+    return Guard([&] { kr::CopyPagesLaunch(cache, src, dst, n, S(stream)); });
+}
+
+int kr_op_cache_compact(const kr_cache *cache, const kr_seqs *seqs, const int32_t *path, int64_t ld_path, int width,
+                        const int32_t *path_lens, void *stream)
+{
+    return Guard([&] { kr::CompactLaunch(cache, seqs, path, ld_path, width, path_lens, S(stream)); });
 }
 
 int kr_op_transpose(const void *src, void *dst, int R, int C, void *stream)

@@ -27,6 +27,29 @@ class KrPub(ctypes.Structure):
                 ("rows_per_tile", ctypes.c_int32), ("arrivals", ctypes.c_int32)]
 
 
+class KrCache(ctypes.Structure):
+    """A paged key/value cache (kr_cache); make_cache fills it."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("layer_stride", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class KrSeqs(ctypes.Structure):
+    """A launch's sequences (kr_seqs); make_seqs fills it."""
+    _fields_ = [("table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("lens", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("tree", ctypes.c_void_p), ("ld_tree", ctypes.c_int64),
+                ("table_pages", ctypes.c_int32), ("seqs", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("tree_words", ctypes.c_int32)]
+
+
+class KrRope(ctypes.Structure):
+    """Rotation tables and the gains of the per-head norms (kr_rope); make_rope fills it."""
+    _fields_ = [("cos_t", ctypes.c_void_p), ("sin_t", ctypes.c_void_p), ("q_gamma", ctypes.c_void_p),
+                ("k_gamma", ctypes.c_void_p), ("positions", ctypes.c_int64), ("head_dim", ctypes.c_int32),
+                ("table_dtype", ctypes.c_int32), ("chain", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
 _BOUND = False
 
 
@@ -63,6 +86,15 @@ def _lib():
         L.kr_op_gemm_add_rmsnorm.argtypes = [i32, vp, i64, vp, i64, vp, i32, i32, i32, vp, vp, vp, vp, vp, f32,
                                              ctypes.POINTER(KrPub), ctypes.c_uint32, vp, ctypes.c_size_t, vp, i32, vp]
         L.kr_op_gemm_streamk_noalloc.argtypes = [i32, vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp]
+        sz, p = ctypes.c_size_t, ctypes.POINTER
+        L.kr_op_qk_norm_rope.argtypes = [i32, p(KrRope), vp, i64, vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp]
+        L.kr_op_qk_norm_rope_cache.argtypes = [p(KrRope), p(KrCache), i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp,
+                                               i32, i32, vp]
+        L.kr_op_attention_paged_workspace.argtypes = [p(KrCache), p(KrSeqs), i32, p(sz), p(ctypes.c_int)]
+        L.kr_op_attention_paged.argtypes = [p(KrCache), i32, p(KrSeqs), vp, i64, vp, i64, i32, i32, f32, vp, sz, vp,
+                                            i32, vp]
+        L.kr_op_cache_copy_pages.argtypes = [p(KrCache), vp, vp, i32, vp]
+        L.kr_op_cache_compact.argtypes = [p(KrCache), p(KrSeqs), vp, i64, i32, vp, vp]
         L.kr_op_stream_create.argtypes = []
         L.kr_op_stream_create.restype = vp
         L.kr_op_stream_destroy.argtypes = [vp]
@@ -71,7 +103,9 @@ def _lib():
                      "kr_op_gemm_add_rmsnorm", "kr_op_gemm_streamk_noalloc",
                      "kr_op_gemm_streamk_workspace", "kr_op_elementwise", "kr_op_rowop", "kr_op_wait", "kr_op_publish",
                      "kr_op_embedding", "kr_op_rope", "kr_op_attention", "kr_op_attention_workspace",
-                     "kr_op_attention_split", "kr_op_transpose"):
+                     "kr_op_attention_split", "kr_op_transpose", "kr_op_qk_norm_rope", "kr_op_qk_norm_rope_cache",
+                     "kr_op_attention_paged_workspace", "kr_op_attention_paged", "kr_op_cache_copy_pages",
+                     "kr_op_cache_compact"):
             getattr(L, name).restype = ctypes.c_int
         _BOUND = True
     return L
@@ -300,3 +334,207 @@ def transpose(src, dst, stream=None):
     R, C = src.shape
     assert dst.shape[0] == C and dst.shape[1] == R
     _check(_lib().kr_op_transpose(_ptr(src), _ptr(dst), R, C, _stream(stream)))
+
+
+# ------------------------------------------------------------- paged cache
+# Handles are made once and passed to every call (their tensors are kept
+# alive with them); the calls check what the C entry cannot see: shapes,
+# strides and devices of the tensors.
+def _need(ok, who, what):
+    if not ok:
+        raise ValueError("%s: %s" % (who, what))
+
+
+def _vector(t, dtype, n, who, name):
+    """A contiguous [n] (or longer, n None) tensor of a torch dtype given by name."""
+    import torch
+    _need(t.dtype == getattr(torch, dtype) and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
+          who, "%s must be a contiguous %s vector%s" % (name, dtype, "" if n is None else " of %d" % n))
+
+
+def _heads(t, shape, dtype, who, name):
+    """A [rows, heads, D] tensor with packed heads; returns its row stride."""
+    _need(tuple(t.shape) == shape and t.dtype == dtype, who, "%s must be %s %s" % (name, shape, dtype))
+    s = t.stride()
+    _need(s[2] == 1 and (s[1] == shape[2] or shape[1] == 1), who, "%s: the heads of a row must be packed" % name)
+    if shape[0] <= 1:
+        return 0
+    _need(s[0] >= shape[1] * shape[2], who, "%s: rows overlap" % name)
+    return s[0]
+
+
+def _here(who, handle_device, *tensors):
+    """Kernels go to the current device's stream: everything must be on it."""
+    if _RAW is None:
+        _stream(None)
+    dev = _RAW[0]()
+    if handle_device != dev:
+        raise ValueError("%s: a handle's tensors are on device %d, the current device is %d" % (
+            who, handle_device, dev))
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("%s: a tensor is on %s, the current device is %d" % (who, t.device, dev))
+
+
+def make_cache(k, v):
+    """Handle of a paged cache: k and v [layers, pages, page_size, heads,
+    head_dim] (or without layers), bf16 or f16, the same strides, rows of
+    head_dim contiguous."""
+    who = "make_cache"
+    _need(k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride(), who,
+          "k and v must agree in shape, type and strides")
+    _need(k.dim() in (4, 5), who, "k and v are [layers, pages, page_size, heads, head_dim]")
+    _need(k.stride(-1) == 1, who, "rows must be contiguous")
+    _need(k.device == v.device, who, "k and v must be on one device")
+    shape, stride = list(k.shape), list(k.stride())
+    if len(shape) == 4:
+        shape, stride = [1] + shape, [0] + stride
+    c = KrCache(_ptr(k), _ptr(v), *stride[:4], *shape, _dt(k))
+    c.keep, c.device, c.torch_dtype = (k, v), k.get_device(), k.dtype
+    return c
+
+
+def make_seqs(table, lens, starts, max_new, tree=None):
+    """Handle of a launch's sequences: table [seqs, pages] and lens [seqs]
+    int32, starts [seqs + 1] int32 (rows starts[b] .. starts[b + 1] - 1 are
+    sequence b's new tokens), all read on the device at each call. max_new: no
+    sequence has more new tokens. tree [rows, words] int64: bit j % 64 of word
+    j // 64 says whether the row sees new token j of its sequence (None:
+    causal)."""
+    import torch
+    who = "make_seqs"
+    _need(table.dtype == torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1), who,
+          "table must be int32 [seqs, pages] with contiguous rows")
+    n = table.shape[0]
+    _vector(lens, "int32", n, who, "lens")
+    _vector(starts, "int32", n + 1, who, "starts")
+    _need(max_new >= 0, who, "max_new must not be negative")
+    words = ld = 0
+    if tree is not None:
+        _need(tree.dtype == torch.int64 and tree.dim() == 2 and (tree.shape[1] <= 1 or tree.stride(1) == 1), who,
+              "tree must be int64 [rows, words] with contiguous rows")
+        words, ld = tree.shape[1], max(tree.stride(0), tree.shape[1])
+        _need(max_new <= 64 * words, who, "the tree has too few words for max_new")
+    tensors = [t for t in (table, lens, starts, tree) if t is not None]
+    _need(len({t.device for t in tensors}) == 1, who, "the tensors must be on one device")
+    s = KrSeqs(_ptr(table), max(table.stride(0), table.shape[1]), _ptr(lens), _ptr(starts), _ptr(tree), ld,
+               table.shape[1], n, max_new, words)
+    s.keep, s.device, s.rows = tensors, table.get_device(), None if tree is None else tree.shape[0]
+    return s
+
+
+def make_rope(cos_t, sin_t, q_gamma=None, k_gamma=None, eps=1e-6, chain=False):
+    """Handle of rotation tables [positions, head_dim] (fp32 or the
+    activations' type) and, optionally, the gains [head_dim] of the per-head
+    norms of q and k. chain: round after each step, the bits of rowop
+    ("rmsnorm") and rope in sequence; otherwise once, at the store."""
+    who = "make_rope"
+    _need(cos_t.dim() == 2 and cos_t.shape == sin_t.shape and cos_t.dtype == sin_t.dtype and cos_t.is_contiguous()
+          and sin_t.is_contiguous(), who, "cos and sin must be contiguous [positions, head_dim] of one type")
+    _need((q_gamma is None) == (k_gamma is None), who, "one of the two gains is missing")
+    for g in (q_gamma, k_gamma):
+        _need(g is None or (g.shape == cos_t.shape[1:] and g.is_contiguous() and g.dtype == q_gamma.dtype), who,
+              "gains must be [head_dim] of one type")
+    tensors = [t for t in (cos_t, sin_t, q_gamma, k_gamma) if t is not None]
+    _need(len({t.device for t in tensors}) == 1, who, "the tensors must be on one device")
+    r = KrRope(_ptr(cos_t), _ptr(sin_t), _ptr(q_gamma), _ptr(k_gamma), cos_t.shape[0], cos_t.shape[1], _dt(cos_t),
+               int(bool(chain)), float(eps))
+    r.keep, r.device = tensors, cos_t.get_device()
+    r.torch_dtype = None if q_gamma is None else q_gamma.dtype
+    return r
+
+
+def qk_norm_rope(rope, q, k, q_out, k_out, positions=None, stream=None):
+    """q_out, k_out = per-head RMSNorm (if the handle has gains) and rotation
+    of q [rows, HQ, D] and k [rows, HKV, D] in one pass. Row r stands at
+    positions[r] (int64; None: r); outside the tables: zeros. Outputs may be
+    the inputs themselves."""
+    who = "qk_norm_rope"
+    _need(q.dim() == 3 and k.dim() == 3, who, "q and k are [rows, heads, head_dim]")
+    rows, HQ, D = q.shape
+    HKV, dt = k.shape[1], q.dtype
+    _need(D == rope.head_dim, who, "the tables have another head_dim")
+    _need(rope.torch_dtype in (None, dt), who, "the gains must be of q's type")
+    lds = [_heads(t, s, dt, who, n) for t, s, n in ((q, (rows, HQ, D), "q"), (k, (rows, HKV, D), "k"),
+                                                    (q_out, (rows, HQ, D), "q_out"), (k_out, (rows, HKV, D), "k_out"))]
+    if positions is not None:
+        _vector(positions, "int64", rows, who, "positions")
+    _here(who, rope.device, q, k, q_out, k_out, positions)
+    _check(_lib().kr_op_qk_norm_rope(_dt(q), rope, _ptr(q), lds[0], _ptr(k), lds[1], _ptr(q_out), lds[2], _ptr(k_out),
+                                     lds[3], _ptr(positions), rows, HQ, HKV, _stream(stream)))
+
+
+def qk_norm_rope_cache(rope, cache, layer, q, k, v, q_out, positions, slots, stream=None):
+    """qk_norm_rope with row r's k and v written to slot slots[r] (int64: page *
+    page_size + row in the page; outside the cache, say -1: not written) of a
+    layer of the cache."""
+    who = "qk_norm_rope_cache"
+    _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
+    rows, HQ, D = q.shape
+    dt, kv = cache.torch_dtype, (rows, cache.heads, cache.head_dim)
+    _need(D == cache.head_dim, who, "q has another head_dim than the cache")
+    _need(rope.torch_dtype in (None, dt), who, "the gains must be of the cache's type")
+    lds = [_heads(t, s, dt, who, n) for t, s, n in ((q, (rows, HQ, D), "q"), (k, kv, "k"), (v, kv, "v"),
+                                                    (q_out, (rows, HQ, D), "q_out"))]
+    if positions is not None:
+        _vector(positions, "int64", rows, who, "positions")
+    _vector(slots, "int64", rows, who, "slots")
+    _here(who, rope.device, cache.keep[0], q, k, v, q_out, positions, slots)
+    _check(_lib().kr_op_qk_norm_rope_cache(rope, cache, layer, _ptr(q), lds[0], _ptr(k), lds[1], _ptr(v), lds[2],
+                                           _ptr(q_out), lds[3], _ptr(positions), _ptr(slots), rows, HQ,
+                                           _stream(stream)))
+
+
+def attention_paged_workspace(cache, seqs, HQ):
+    """(workspace bytes, counters) with which attention_paged cuts long
+    sequences into pieces; (0, 0) when it never would."""
+    b, c = ctypes.c_size_t(0), ctypes.c_int(0)
+    _check(_lib().kr_op_attention_paged_workspace(cache, seqs, HQ, ctypes.byref(b), ctypes.byref(c)))
+    return b.value, c.value
+
+
+def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
+    """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
+    cache; their own keys and values are in the cache already. ws (uint8) and
+    counters (int32, zero before the first call): of attention_paged_workspace's
+    sizes, for one stream at a time; None: no sequence is cut into pieces."""
+    who = "attention_paged"
+    _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
+    shape = (q.shape[0], q.shape[1], cache.head_dim)
+    _need(seqs.rows is None or seqs.rows >= shape[0], who, "the tree has too few rows")
+    ldq = _heads(q, shape, cache.torch_dtype, who, "q")
+    ldo = _heads(out, shape, cache.torch_dtype, who, "out")
+    _here(who, cache.device, seqs.keep[0], q, out, ws, counters)
+    if ws is not None:
+        _need(ws.is_contiguous() and counters is not None and counters.is_contiguous() and counters.element_size() == 4,
+              who, "ws and counters must be contiguous, counters of 32 bits")
+    _check(_lib().kr_op_attention_paged(cache, layer, seqs, _ptr(q), ldq, _ptr(out), ldo, shape[0],
+                                        shape[1], cache.head_dim ** -0.5 if scale is None else float(scale), _ptr(ws),
+                                        0 if ws is None else ws.numel() * ws.element_size(),
+                                        None if ws is None else _ptr(counters),
+                                        0 if ws is None else counters.numel(), _stream(stream)))
+
+
+def cache_copy_pages(cache, src, dst, stream=None):
+    """Page dst[i] becomes a copy of page src[i] in every layer (lists of page
+    ids, no page twice in dst and none in both)."""
+    n = len(src)
+    _need(len(dst) == n, "cache_copy_pages", "src and dst differ in length")
+    _here("cache_copy_pages", cache.device)
+    ids = ctypes.c_int32 * n
+    _check(_lib().kr_op_cache_copy_pages(cache, ids(*src), ids(*dst), n, _stream(stream)))
+
+
+def cache_compact(cache, seqs, path, path_lens, stream=None):
+    """Accepted drafts move to the front: in every layer and for each sequence
+    the rows at lens[b] + path[b, i], i < path_lens[b], go to lens[b] + i, as if
+    all were read before any is written. path [seqs, width <= 256] and
+    path_lens [seqs] int32; entries below 0 move nothing."""
+    import torch
+    who = "cache_compact"
+    _need(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == seqs.seqs
+          and (path.shape[1] <= 1 or path.stride(1) == 1), who, "path must be int32 [seqs, width] with contiguous rows")
+    _vector(path_lens, "int32", seqs.seqs, who, "path_lens")
+    _here(who, cache.device, seqs.keep[0], path, path_lens)
+    _check(_lib().kr_op_cache_compact(cache, seqs, _ptr(path), max(path.stride(0), path.shape[1]), path.shape[1],
+                                      _ptr(path_lens), _stream(stream)))
