@@ -53,6 +53,7 @@
 #include "kr_gemm.h"
 #include "kr_json.h"
 #include "kr_misc.h"
+#include "kr_paged.h"
 #include "kr_rowops.h"
 #include "kr_runtime.h"
 
@@ -915,17 +916,43 @@ private:
         Timed(P, "qkv", [&] { Emit(P, [gd](hipStream_t st) { GemmLaunch(gd, st); }); });
         uint16_t *q = qkv, *kk = qkv + size_t(HQ_) * D_, *v = qkv + size_t(HQ_ + HKV_) * D_;
         int64_t ldq = ld, ldk = ld;
+        const int HQ = HQ_, HKV = HKV_, D = D_;
+        const uint16_t *cs = cos_, *sn = sin_;
+        // with q/k norms both norms and rotations are one pass, rounded as the
+        // separate launches round (KR_QWEN_QK_FUSED=0: those four)
+        const bool fused = qk_norm_ && EnvInt("KR_QWEN_QK_FUSED", 1) != 0;
         if (qk_norm_) {
-            RmsNorm(P, q, w.qn, qn_.get(), S * HQ_, D_, HQ_, ld);
-            RmsNorm(P, kk, w.kn, kn_.get(), S * HKV_, D_, HKV_, ld);
+            if (fused) {
+                QkRopeDesc d;
+                d.rope.cos_t = cs;
+                d.rope.sin_t = sn;
+                d.rope.q_gamma = w.qn;
+                d.rope.k_gamma = w.kn;
+                d.rope.positions = S;
+                d.rope.head_dim = D;
+                d.rope.table_dtype = kBF16;
+                d.rope.chain = 1;
+                d.rope.eps = float(eps_);
+                d.q = q;
+                d.k = kk;
+                d.ldq = d.ldk = ld;
+                d.q_out = qn_.get();
+                d.k_out = kn_.get();
+                d.rows = S;
+                d.HQ = HQ;
+                d.HKV = HKV;
+                d.D = D;
+                Emit(P, [d](hipStream_t st) { QkRopeLaunch(d, st); });
+            } else {
+                RmsNorm(P, q, w.qn, qn_.get(), S * HQ_, D_, HQ_, ld);
+                RmsNorm(P, kk, w.kn, kn_.get(), S * HKV_, D_, HKV_, ld);
+            }
             q = qn_.as<uint16_t>();
             kk = kn_.as<uint16_t>();
             ldq = int64_t(HQ_) * D_;
             ldk = int64_t(HKV_) * D_;
         }
-        const int HQ = HQ_, HKV = HKV_, D = D_;
-        const uint16_t *cs = cos_, *sn = sin_;
-        if (!rope_epi) {
+        if (!rope_epi && !fused) {
             Emit(P, [=](hipStream_t st) {
                 RopeLaunch(kBF16, q, ldq, S, HQ, D, cs, sn, st);
                 RopeLaunch(kBF16, kk, ldk, S, HKV, D, cs, sn, st);
