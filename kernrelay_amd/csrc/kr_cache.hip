@@ -322,13 +322,18 @@ __global__ void __launch_bounds__(256) CopyPagesKernel(CopyParams p)
     const uint16_t *src = base + int64_t(p.src[pair]) * p.page_stride;
     uint16_t *dst = base + int64_t(p.dst[pair]) * p.page_stride;
     const int c0 = seg * 256 * kCopyUnroll + int(threadIdx.x);
-    uint4 x[kCopyUnroll];
+    // chunks past the page's end repeat its last one: every load goes out
+    // before the first store, with no branch between them
+    typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+    int64_t at[kCopyUnroll];
+    U32x4 x[kCopyUnroll];
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) at[u] = PageChunk(p, min(c0 + u * 256, p.chunks - 1));
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) x[u] = *reinterpret_cast<const U32x4 *>(src + at[u]);
 #pragma unroll
     for (int u = 0; u < kCopyUnroll; ++u)
-        if (c0 + u * 256 < p.chunks) x[u] = *reinterpret_cast<const uint4 *>(src + PageChunk(p, c0 + u * 256));
-#pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
-        if (c0 + u * 256 < p.chunks) *reinterpret_cast<uint4 *>(dst + PageChunk(p, c0 + u * 256)) = x[u];
+        if (c0 + u * 256 < p.chunks) *reinterpret_cast<U32x4 *>(dst + at[u]) = x[u];
 }
 
 }  // namespace
@@ -429,13 +434,12 @@ __global__ void __launch_bounds__(256) CompactKernel(CompactParams p)
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
         const int i = int(threadIdx.x) / LPR + u * RPS;
-        to[u] = -1;
-        if (i >= n || head >= p.heads) continue;
-        const int from = p.path[b * p.ld_path + i];
-        if (from < 0 || from == i) continue;
-        const int64_t src = row(int64_t(len) + from);
-        if (src < 0) continue;
-        to[u] = row(int64_t(len) + i);
+        const bool in = i < n && head < p.heads;
+        const int from = in ? p.path[b * p.ld_path + i] : -1;
+        const bool moves = from >= 0 && from != i;
+        const int64_t src = moves ? row(int64_t(len) + from) : -1;
+        to[u] = src >= 0 ? row(int64_t(len) + i) : -1;
+        x[u] = make_uint4(0, 0, 0, 0);
         if (to[u] >= 0) x[u] = *reinterpret_cast<const uint4 *>(base + src);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers

@@ -6,6 +6,7 @@ without the built library raises: there is no CPU fallback.
 """
 
 import ctypes
+from array import array
 
 from . import libapi
 
@@ -339,41 +340,59 @@ def transpose(src, dst, stream=None):
 # ------------------------------------------------------------- paged cache
 # Handles are made once and passed to every call (their tensors are kept
 # alive with them); the calls check what the C entry cannot see: shapes,
-# strides and devices of the tensors.
+# strides and devices of the tensors. The checks are one expression per tensor
+# and the reason is looked for only after a refusal: the step kernels run in
+# 3 to 7 us, and the wrappers' own time is what a caller of them waits for.
 def _need(ok, who, what):
     if not ok:
         raise ValueError("%s: %s" % (who, what))
 
 
-def _vector(t, dtype, n, who, name):
-    """A contiguous [n] (or longer, n None) tensor of a torch dtype given by name."""
-    import torch
-    _need(t.dtype == getattr(torch, dtype) and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
-          who, "%s must be a contiguous %s vector%s" % (name, dtype, "" if n is None else " of %d" % n))
+_INTS = None  # (torch.int32, torch.int64)
+
+
+def _ints():
+    global _INTS
+    if _INTS is None:
+        import torch
+        _INTS = (torch.int32, torch.int64)
+    return _INTS
 
 
 def _heads(t, shape, dtype, who, name):
-    """A [rows, heads, D] tensor with packed heads; returns its row stride."""
-    _need(tuple(t.shape) == shape and t.dtype == dtype, who, "%s must be %s %s" % (name, shape, dtype))
+    """Address and row stride of a [rows, heads, D] tensor with packed heads."""
     s = t.stride()
-    _need(s[2] == 1 and (s[1] == shape[2] or shape[1] == 1), who, "%s: the heads of a row must be packed" % name)
-    if shape[0] <= 1:
-        return 0
-    _need(s[0] >= shape[1] * shape[2], who, "%s: rows overlap" % name)
-    return s[0]
+    if t.dtype == dtype and t.shape == shape and s[2] == 1 and (s[1] == shape[2] or shape[1] == 1):
+        if shape[0] <= 1:
+            return t.data_ptr(), 0
+        if s[0] >= shape[1] * shape[2]:
+            return t.data_ptr(), s[0]
+        raise ValueError("%s: %s: rows overlap" % (who, name))
+    _need(t.shape == shape and t.dtype == dtype, who, "%s must be %s %s" % (name, tuple(shape), dtype))
+    raise ValueError("%s: %s: the heads of a row must be packed" % (who, name))
 
 
-def _here(who, handle_device, *tensors):
-    """Kernels go to the current device's stream: everything must be on it."""
-    if _RAW is None:
-        _stream(None)
-    dev = _RAW[0]()
-    if handle_device != dev:
-        raise ValueError("%s: a handle's tensors are on device %d, the current device is %d" % (
-            who, handle_device, dev))
+def _vector(t, dtype, n, who, name):
+    """Address of a contiguous [n] tensor."""
+    if t.dtype == dtype and t.shape == (n,) and (n <= 1 or t.stride(0) == 1):
+        return t.data_ptr()
+    raise ValueError("%s: %s must be a contiguous %s vector of %d" % (who, name, dtype, n))
+
+
+def _launch_stream(stream, who, dev, other, *tensors):
+    """The stream's handle. Kernels go to the current device's streams: the
+    handles' tensors and the call's must be on it."""
     for t in tensors:
         if t is not None and t.get_device() != dev:
-            raise ValueError("%s: a tensor is on %s, the current device is %d" % (who, t.device, dev))
+            if not t.is_cuda:
+                raise RuntimeError("kernrelay ops need device tensors (got a CPU tensor)")
+            raise ValueError("%s: a tensor is on %s, the handle's are on device %d" % (who, t.device, dev))
+    if _RAW is None:
+        _stream(None)
+    if dev != other or _RAW[0]() != dev:
+        raise ValueError("%s: the handles' tensors are on devices %d and %d, the current device is %d" % (
+            who, dev, other, _RAW[0]()))
+    return _stream(stream)
 
 
 def make_cache(k, v):
@@ -406,8 +425,9 @@ def make_seqs(table, lens, starts, max_new, tree=None):
     _need(table.dtype == torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1), who,
           "table must be int32 [seqs, pages] with contiguous rows")
     n = table.shape[0]
-    _vector(lens, "int32", n, who, "lens")
-    _vector(starts, "int32", n + 1, who, "starts")
+    for v, size, name in ((lens, n, "lens"), (starts, n + 1, "starts")):
+        _need(v.dtype == torch.int32 and v.shape == (size,) and v.is_contiguous(), who,
+              "%s must be a contiguous int32 vector of %d" % (name, size))
     _need(max_new >= 0, who, "max_new must not be negative")
     words = ld = 0
     if tree is not None:
@@ -451,38 +471,40 @@ def qk_norm_rope(rope, q, k, q_out, k_out, positions=None, stream=None):
     the inputs themselves."""
     who = "qk_norm_rope"
     _need(q.dim() == 3 and k.dim() == 3, who, "q and k are [rows, heads, head_dim]")
-    rows, HQ, D = q.shape
-    HKV, dt = k.shape[1], q.dtype
-    _need(D == rope.head_dim, who, "the tables have another head_dim")
+    qs, ks, dt, dev = q.shape, k.shape, q.dtype, rope.device
+    rows = qs[0]
+    _need(qs[2] == rope.head_dim, who, "the tables have another head_dim")
     _need(rope.torch_dtype in (None, dt), who, "the gains must be of q's type")
-    lds = [_heads(t, s, dt, who, n) for t, s, n in ((q, (rows, HQ, D), "q"), (k, (rows, HKV, D), "k"),
-                                                    (q_out, (rows, HQ, D), "q_out"), (k_out, (rows, HKV, D), "k_out"))]
-    if positions is not None:
-        _vector(positions, "int64", rows, who, "positions")
-    _here(who, rope.device, q, k, q_out, k_out, positions)
-    _check(_lib().kr_op_qk_norm_rope(_dt(q), rope, _ptr(q), lds[0], _ptr(k), lds[1], _ptr(q_out), lds[2], _ptr(k_out),
-                                     lds[3], _ptr(positions), rows, HQ, HKV, _stream(stream)))
+    _need(ks[0] == rows and ks[2] == qs[2], who, "k must be [%d, heads, %d]" % (rows, qs[2]))
+    qp, ldq = _heads(q, qs, dt, who, "q")
+    kp, ldk = _heads(k, ks, dt, who, "k")
+    qo, ldqo = _heads(q_out, qs, dt, who, "q_out")
+    ko, ldko = _heads(k_out, ks, dt, who, "k_out")
+    pos = None if positions is None else _vector(positions, _ints()[1], rows, who, "positions")
+    _check(_lib().kr_op_qk_norm_rope(_dt(q), rope, qp, ldq, kp, ldk, qo, ldqo, ko, ldko, pos, rows, qs[1], ks[1],
+                                     _launch_stream(stream, who, dev, dev, q, k, q_out, k_out, positions)))
 
 
 def qk_norm_rope_cache(rope, cache, layer, q, k, v, q_out, positions, slots, stream=None):
     """qk_norm_rope with row r's k and v written to slot slots[r] (int64: page *
     page_size + row in the page; outside the cache, say -1: not written) of a
-    layer of the cache."""
+    layer of the cache. No two rows may share a slot."""
     who = "qk_norm_rope_cache"
     _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
-    rows, HQ, D = q.shape
-    dt, kv = cache.torch_dtype, (rows, cache.heads, cache.head_dim)
-    _need(D == cache.head_dim, who, "q has another head_dim than the cache")
+    qs, dt, dev, i64 = q.shape, cache.torch_dtype, cache.device, _ints()[1]
+    rows = qs[0]
+    kv = (rows, cache.heads, cache.head_dim)
+    _need(qs[2] == kv[2], who, "q has another head_dim than the cache")
     _need(rope.torch_dtype in (None, dt), who, "the gains must be of the cache's type")
-    lds = [_heads(t, s, dt, who, n) for t, s, n in ((q, (rows, HQ, D), "q"), (k, kv, "k"), (v, kv, "v"),
-                                                    (q_out, (rows, HQ, D), "q_out"))]
-    if positions is not None:
-        _vector(positions, "int64", rows, who, "positions")
-    _vector(slots, "int64", rows, who, "slots")
-    _here(who, rope.device, cache.keep[0], q, k, v, q_out, positions, slots)
-    _check(_lib().kr_op_qk_norm_rope_cache(rope, cache, layer, _ptr(q), lds[0], _ptr(k), lds[1], _ptr(v), lds[2],
-                                           _ptr(q_out), lds[3], _ptr(positions), _ptr(slots), rows, HQ,
-                                           _stream(stream)))
+    qp, ldq = _heads(q, qs, dt, who, "q")
+    kp, ldk = _heads(k, kv, dt, who, "k")
+    vp, ldv = _heads(v, kv, dt, who, "v")
+    qo, ldqo = _heads(q_out, qs, dt, who, "q_out")
+    pos = None if positions is None else _vector(positions, i64, rows, who, "positions")
+    _check(_lib().kr_op_qk_norm_rope_cache(rope, cache, layer, qp, ldq, kp, ldk, vp, ldv, qo, ldqo, pos,
+                                           _vector(slots, i64, rows, who, "slots"), rows, qs[1],
+                                           _launch_stream(stream, who, dev, rope.device, q, k, v, q_out, positions,
+                                                          slots)))
 
 
 def attention_paged_workspace(cache, seqs, HQ):
@@ -500,29 +522,29 @@ def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=No
     sizes, for one stream at a time; None: no sequence is cut into pieces."""
     who = "attention_paged"
     _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
-    shape = (q.shape[0], q.shape[1], cache.head_dim)
+    shape, dt, dev = q.shape, cache.torch_dtype, cache.device
+    _need(shape[2] == cache.head_dim, who, "q has another head_dim than the cache")
     _need(seqs.rows is None or seqs.rows >= shape[0], who, "the tree has too few rows")
-    ldq = _heads(q, shape, cache.torch_dtype, who, "q")
-    ldo = _heads(out, shape, cache.torch_dtype, who, "out")
-    _here(who, cache.device, seqs.keep[0], q, out, ws, counters)
+    qp, ldq = _heads(q, shape, dt, who, "q")
+    op, ldo = _heads(out, shape, dt, who, "out")
+    wp, cp, nbytes, ncnt = None, None, 0, 0
     if ws is not None:
-        _need(ws.is_contiguous() and counters is not None and counters.is_contiguous() and counters.element_size() == 4,
-              who, "ws and counters must be contiguous, counters of 32 bits")
-    _check(_lib().kr_op_attention_paged(cache, layer, seqs, _ptr(q), ldq, _ptr(out), ldo, shape[0],
-                                        shape[1], cache.head_dim ** -0.5 if scale is None else float(scale), _ptr(ws),
-                                        0 if ws is None else ws.numel() * ws.element_size(),
-                                        None if ws is None else _ptr(counters),
-                                        0 if ws is None else counters.numel(), _stream(stream)))
+        _need(counters is not None and counters.dtype == _ints()[0] and counters.dim() == 1 and counters.is_contiguous()
+              and ws.is_contiguous(), who, "ws and counters (an int32 vector) must be contiguous")
+        wp, cp, nbytes, ncnt = ws.data_ptr(), counters.data_ptr(), ws.nbytes, counters.shape[0]
+    _check(_lib().kr_op_attention_paged(cache, layer, seqs, qp, ldq, op, ldo, shape[0], shape[1],
+                                        cache.head_dim ** -0.5 if scale is None else scale, wp, nbytes, cp, ncnt,
+                                        _launch_stream(stream, who, dev, seqs.device, q, out, ws, counters)))
 
 
 def cache_copy_pages(cache, src, dst, stream=None):
     """Page dst[i] becomes a copy of page src[i] in every layer (lists of page
     ids, no page twice in dst and none in both)."""
-    n = len(src)
-    _need(len(dst) == n, "cache_copy_pages", "src and dst differ in length")
-    _here("cache_copy_pages", cache.device)
-    ids = ctypes.c_int32 * n
-    _check(_lib().kr_op_cache_copy_pages(cache, ids(*src), ids(*dst), n, _stream(stream)))
+    who = "cache_copy_pages"
+    a, b = array("i", src), array("i", dst)
+    _need(len(a) == len(b), who, "src and dst differ in length")
+    _check(_lib().kr_op_cache_copy_pages(cache, a.buffer_info()[0], b.buffer_info()[0], len(a),
+                                         _launch_stream(stream, who, cache.device, cache.device)))
 
 
 def cache_compact(cache, seqs, path, path_lens, stream=None):
@@ -530,11 +552,11 @@ def cache_compact(cache, seqs, path, path_lens, stream=None):
     the rows at lens[b] + path[b, i], i < path_lens[b], go to lens[b] + i, as if
     all were read before any is written. path [seqs, width <= 256] and
     path_lens [seqs] int32; entries below 0 move nothing."""
-    import torch
     who = "cache_compact"
-    _need(path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == seqs.seqs
-          and (path.shape[1] <= 1 or path.stride(1) == 1), who, "path must be int32 [seqs, width] with contiguous rows")
-    _vector(path_lens, "int32", seqs.seqs, who, "path_lens")
-    _here(who, cache.device, seqs.keep[0], path, path_lens)
-    _check(_lib().kr_op_cache_compact(cache, seqs, _ptr(path), max(path.stride(0), path.shape[1]), path.shape[1],
-                                      _ptr(path_lens), _stream(stream)))
+    n, dev, i32 = seqs.seqs, cache.device, _ints()[0]
+    _need(path.dim() == 2 and path.dtype == i32 and path.shape[0] == n and (path.shape[1] <= 1 or path.stride(1) == 1),
+          who, "path must be int32 [seqs, width] with contiguous rows")
+    lens = _vector(path_lens, i32, n, who, "path_lens")
+    width = path.shape[1]
+    _check(_lib().kr_op_cache_compact(cache, seqs, path.data_ptr(), max(path.stride(0), width), width, lens,
+                                      _launch_stream(stream, who, dev, seqs.device, path, path_lens)))
