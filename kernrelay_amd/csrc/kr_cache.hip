@@ -393,11 +393,13 @@ void CopyPagesLaunch(const kr_cache *cache, const int32_t *src, const int32_t *d
 }
 
 // ----------------------------------------------------------------- compaction
-// Bound by the launch: a few rows of each layer move. A workgroup takes LPR
-// 16-byte chunks of every row of one sequence in one layer's k or v and holds
-// all of them in registers before it writes the first (a row's new place may
-// be another's old one): NS sweeps of 256 / LPR rows. Columns are
-// independent, so workgroups are too.
+// Bound by latency: a few rows of each layer move, and where they are takes a
+// chain of loads (length, path, page ids). A workgroup takes LPR 16-byte
+// chunks of every row of one sequence, in PL of the layers' k and v: the chain
+// once, then PL planes in flight. It holds all of a plane in registers before
+// it writes the first row (a row's new place may be another's old one): NS
+// sweeps of 256 / LPR rows. Columns and planes are independent. 32 paths of up
+// to 9 drafts, 28 layers of 4 heads: PL 1 9.6 us, 4 6.1 us.
 namespace {
 
 struct CompactParams {
@@ -405,11 +407,11 @@ struct CompactParams {
     int64_t layer_stride, page_stride, token_stride, head_stride;
     const int32_t *table, *lens, *path, *path_lens;
     int64_t ld_table, ld_path, cap;  // cap: table_pages * page_size
-    int pages, heads, dch, width, slices, seqs;
+    int pages, heads, dch, width, slices, planes;
     PageDiv div;
 };
 
-template <int LPR, int NS>
+template <int LPR, int NS, int PL>
 __global__ void __launch_bounds__(256) CompactKernel(CompactParams p)
 {
     constexpr int RPS = 256 / LPR;
@@ -417,7 +419,6 @@ __global__ void __launch_bounds__(256) CompactKernel(CompactParams p)
     const int ch = (int(blockIdx.x) - b * p.slices) * LPR + int(threadIdx.x) % LPR;
     const int n = min(max(p.path_lens[b], 0), p.width);
     const int len = max(p.lens[b], 0);
-    uint16_t *base = ((blockIdx.y & 1) != 0 ? p.v : p.k) + int64_t(blockIdx.y >> 1) * p.layer_stride;
     const int head = ch / p.dch;
     const int64_t col = int64_t(head) * p.head_stride + (ch - head * p.dch) * 8;
     const int32_t *table = p.table + b * p.ld_table;
@@ -429,7 +430,12 @@ __global__ void __launch_bounds__(256) CompactKernel(CompactParams p)
         if (id < 0 || id >= p.pages) return -1;
         return id * p.page_stride + int64_t(int(pos) - pg * p.div.size) * p.token_stride + col;
     };
-    uint4 x[NS];
+    const int plane0 = int(blockIdx.y) * PL;  // layer plane / 2, its k or v
+    const auto base = [&](int i) {
+        const int plane = min(plane0 + i, p.planes - 1);
+        return ((plane & 1) != 0 ? p.v : p.k) + int64_t(plane >> 1) * p.layer_stride;
+    };
+    uint4 x[NS][PL];
     int64_t to[NS];
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
@@ -439,14 +445,19 @@ __global__ void __launch_bounds__(256) CompactKernel(CompactParams p)
         const bool moves = from >= 0 && from != i;
         const int64_t src = moves ? row(int64_t(len) + from) : -1;
         to[u] = src >= 0 ? row(int64_t(len) + i) : -1;
-        x[u] = make_uint4(0, 0, 0, 0);
-        if (to[u] >= 0) x[u] = *reinterpret_cast<const uint4 *>(base + src);
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            x[u][q] = make_uint4(0, 0, 0, 0);
+            if (to[u] >= 0) x[u][q] = *reinterpret_cast<const uint4 *>(base(q) + src);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < NS; ++u)
-        if (to[u] >= 0) *reinterpret_cast<uint4 *>(base + to[u]) = x[u];
+#pragma unroll
+        for (int q = 0; q < PL; ++q)
+            if (to[u] >= 0 && plane0 + q < p.planes) *reinterpret_cast<uint4 *>(base(q) + to[u]) = x[u][q];
 }
 
 }  // namespace
@@ -481,18 +492,21 @@ void CompactLaunch(const kr_cache *cache, const kr_seqs *s, const int32_t *path,
     p.heads = c.heads;
     p.dch = c.head_dim / 8;
     p.width = width;
-    p.seqs = s->seqs;
+    p.planes = 2 * c.layers;
     p.div = MakePageDiv(c.page_size);
     // lanes per row: as many as leave one sweep for a path of this width, so
     // that a short path keeps its workgroups full
     const int lpr = width <= 8 ? 32 : width <= 16 ? 16 : 8;
     p.slices = (c.heads * p.dch + lpr - 1) / lpr;
     if (int64_t(p.slices) * s->seqs >= (int64_t(1) << 31)) Refuse(who, "too many sequences");
-    const dim3 grid(unsigned(p.slices) * unsigned(s->seqs), unsigned(2 * c.layers));
-    if (lpr == 32) hipLaunchKernelGGL((CompactKernel<32, 1>), grid, dim3(256), 0, stream, p);
-    else if (lpr == 16) hipLaunchKernelGGL((CompactKernel<16, 1>), grid, dim3(256), 0, stream, p);
-    else if (width <= 64) hipLaunchKernelGGL((CompactKernel<8, 2>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((CompactKernel<8, 8>), grid, dim3(256), 0, stream, p);
+    const auto go = [&](auto kern, int pl) {
+        const dim3 grid(unsigned(p.slices) * unsigned(s->seqs), unsigned((p.planes + pl - 1) / pl));
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p);
+    };
+    if (lpr == 32) go(CompactKernel<32, 1, 4>, 4);
+    else if (lpr == 16) go(CompactKernel<16, 1, 4>, 4);
+    else if (width <= 64) go(CompactKernel<8, 2, 4>, 4);
+    else go(CompactKernel<8, 8, 1>, 1);
     Check(hipGetLastError(), "cache_compact launch");
 }
 

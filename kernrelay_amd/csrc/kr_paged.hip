@@ -17,31 +17,39 @@
 // of 32 rows each over the same keys, times KW key streams that take the
 // 32 KB-key blocks of the unit in turn and are merged at its end.
 //
-// Keys and values go HBM -> LDS by the direct-to-LDS DMA into a two-stage
-// ring, each lane fetching 16 bytes of a row wherever the page table puts it.
-// The table's entries travel the same way two stages ahead (so nothing in the
-// loop waits for a dependent load), and each wave turns the next stage's into
-// row offsets: lane l's key is l, its validity a ballot. A position past the
+// Keys and values go HBM -> LDS by the direct-to-LDS DMA into a ring of NS
+// stages, each lane fetching 16 bytes of a row wherever the page table puts it.
+// The table's entries travel the same way, further ahead (so nothing in the
+// loop waits for a dependent load), and each wave turns a stage's into row
+// offsets: lane l's key is l, its validity a ballot. A position past the
 // sequence's end or on a page that is none is fetched from the cache's first
 // row instead and seen by nobody.
 // The products are those of the prompt's kernel (kr_attn.hip): S^T = K Q^T,
 // softmax in base 2 with a lazily moved maximum, O^T += V^T P^T, fp32 state;
 // P is rounded to 16 bits for the matrix cores, its sum is of the unrounded.
 // A block in which some row does not see some key goes the careful way: the
-// scores are masked by 64 bits a row, values of unseen rows are zeroed in LDS
-// (0 x NaN would reach everybody), and where a seen draft's value is no
-// finite number the block is summed on the VALU, row by row.
+// scores are masked by 64 bits a row; value rows that are not there or hold a
+// number that is not finite are zeroed in LDS (0 x NaN would reach everybody),
+// and the latter added on the VALU to the rows that see them.
 #include <algorithm>
 #include <cmath>
 
 #include "kr_attncore.h"
 #include "kr_dma.h"
 #include "kr_paged.h"
-#include "kr_rowcore.h"
 
 namespace kr {
 
 namespace {
+
+// What the second launch needs of a unit that came in pieces: they are slot 1
+// of workgroup `part` and slot 0 of the next pieces - 1 ones.
+struct PagedJoin {
+    int32_t pieces, part;     // at most one: nothing to do
+    int32_t first, r0, nrow;  // the sequence's first row; the unit's rows of it
+    int32_t head;             // first query head
+    int32_t pad[2];
+};
 
 struct PagedParams {
     const uint16_t *q, *k, *v;
@@ -51,13 +59,17 @@ struct PagedParams {
     int64_t ldq, ldo, ld_table, ld_tree;
     int64_t head_stride;
     uint32_t page_stride, token_stride;
-    int cap, pages, table_pages, seqs, rows, max_new, tree_words, HQ, HKV, G, qt_max;
+    int cap, pages, table_pages, seqs, rows, max_new, tree_words, HQ, HKV, G;
     float scale_log2;
     PageDiv div;
-    float *ws;       // two partial slots per workgroup of the cut schedule
-    int32_t *cnt;    // [seqs][HKV][qt_max] arrival tickets, zero between launches
-    int slots;       // workgroups of the cut schedule; 0: whole units only
+    float *ws;         // two partial slots per workgroup of the cut schedule
+    PagedJoin *joins;  // [max_units], unit by unit as they come in the line
+    int max_units;
+    int min_piece;     // stages of a piece, unless the units are shorter
+    int slots;         // workgroups of the cut schedule; 0: whole units only
 };
+
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
 
 // A sequence as the launch has it, every number within its bounds whatever
 // the device arrays hold.
@@ -76,15 +88,18 @@ __device__ __forceinline__ PagedSeq LoadSeq(const PagedParams &p, int b)
     return s;
 }
 
-__device__ __forceinline__ int64_t WaveScan(int64_t v, int lane)
+__device__ __forceinline__ int WaveScan(int v, int lane)
 {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = __shfl_up(v, o, 64);
+        const int u = __shfl_up(v, o, 64);
         if (lane >= o) v += u;
     }
     return v;
 }
+
+// A value that is the same in every lane, as the scalar it is.
+__device__ __forceinline__ int Uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A wave's own LDS writes before its other lanes' reads of them.
 __device__ __forceinline__ void WaveLdsOrder()
@@ -104,17 +119,33 @@ __device__ __forceinline__ bool AnyNonFinite(const uint4 &x)
     return bad;
 }
 
-// Smallest piece of the cut schedule, in stages of a workgroup: a piece costs
-// its partial and a share of the sum at the unit's end.
-constexpr int kMinPiece = 4;
+// Workgroups of the cut schedule: two on each of 256 CUs (their rings fill 128
+// of a CU's 160 KB at head size 128).
+constexpr int kPagedSlots = 512;
 
-template <int DT, int D, int QW, int KW, int KB>
+// When units are cut. Whole, the launch lasts as long as its longest unit
+// (`longest` stages of 64 keys; one workgroup alone on a CU has the CU's whole
+// bandwidth and issue); cut, every workgroup has the same share, but a piece's
+// rows are written and read once more (fp32), by a second launch of 5 to 11
+// us. So units are cut where the longest is more than a even shares and c
+// stages. Measured, cut against whole, in us (D 128):
+//   one row block: 1 sequence of 2000 tokens, 8 key heads: 13 / 42; 16 of up to
+//   4000: 50 / 76; 64 of up to 500, 4 heads: 24 / 18; 64 of up to 1800, 8
+//   heads: 89 / 81;
+//   two: 8 trees of 16 over 3000, 8 heads: 31 / 52; 32: 89 / 81;
+//   four: 8 trees of 61 over 2900, 8 heads: 57 / 72; 16: 78 / 74; 1000 rows of a
+//   prompt over 8000, 4 heads of 7: 166 / 184; 2048 rows: 321 / 300.
+template <int QW> struct CutRule {
+    static constexpr float a = QW == 4 ? 2.0f : 2.6f;
+    static constexpr int c = QW == 1 ? 6 : QW == 2 ? 8 : 16;
+};
+
+template <int DT, int D, int QW, int KW, int KB, int NS>
 __global__ void __attribute__((amdgpu_flat_work_group_size(64 * QW * KW, 64 * QW * KW), amdgpu_waves_per_eu(2)))
 PagedKernel(PagedParams p)
 {
     static_assert(D == 64 || D == 128, "head_dim 64 or 128");
     constexpr int NW = QW * KW;
-    constexpr int THREADS = 64 * NW;
     constexpr int BLK = 32 * KB;            // keys of a stream's stage
     constexpr int SB = BLK * KW;            // keys of a workgroup's stage
     constexpr int RT = 32 * QW;             // rows of a unit
@@ -122,13 +153,16 @@ PagedKernel(PagedParams p)
     constexpr int DBLK = D / 32;            // 32-wide d blocks of O^T
     constexpr int RPD = 64 / DCH;           // rows per 1 KB DMA block
     constexpr int DPW = BLK / RPD / QW;     // DMA blocks per wave, operand and stage
+    constexpr int VAH = 4;                  // V fragments read ahead
+    constexpr int VM = 2 * DPW + 1;         // DMA instructions of a wave's stage
+    static_assert((NS - 1) * VM < 64, "vmcnt");
+    static_assert(SB == 64, "the host counts stages of 64 keys");
     constexpr uint64_t ALL = KB == 2 ? ~0ull : 0xffffffffull;
-    __shared__ __attribute__((aligned(1024))) uint16_t kring[2][KW][BLK * D];
-    __shared__ __attribute__((aligned(1024))) uint16_t vring[2][KW][BLK * D];
-    __shared__ __attribute__((aligned(256))) int32_t tab[NW][2][64];  // page ids of a stage's keys
+    __shared__ __attribute__((aligned(1024))) uint16_t kring[NS][KW][BLK * D];
+    __shared__ __attribute__((aligned(1024))) uint16_t vring[NS][KW][BLK * D];
+    __shared__ __attribute__((aligned(256))) int32_t tab[NW][NS][64];  // page ids of a stage's keys
     __shared__ int64_t offs[NW][64];                                  // and their rows' element offsets
-    __shared__ uint64_t odd[2][KW][QW];                               // keys whose values are not all finite
-    __shared__ int last_piece;
+    __shared__ uint64_t odd[NS][KW][QW];                               // keys whose values are not all finite
 
     const int lane = int(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
@@ -139,63 +173,79 @@ PagedKernel(PagedParams p)
     // work of a sequence: its units (key heads x row blocks), each of `sb` stages
     const auto seq_units = [&](const PagedSeq &s) { return p.HKV * ((s.n * p.G + RT - 1) / RT); };
     const auto seq_stages = [&](const PagedSeq &s) { return (s.total + SB - 1) / SB; };
-    int64_t units = 0, stages = 0;
+    int units = 0, stages = 0, longest = 0;
+    PagedSeq mine{};  // lane's sequence of the first 64
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int64_t u = 0, w = 0;
+        int u = 0, w = 0, most = 0;
         if (b0 + lane < p.seqs) {
             const PagedSeq s = LoadSeq(p, b0 + lane);
+            if (b0 == 0) mine = s;
             u = seq_units(s);
-            w = u * seq_stages(s);
+            most = u > 0 ? seq_stages(s) : 0;
+            w = u * most;
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             u += __shfl_xor(u, o, 64);
             w += __shfl_xor(w, o, 64);
+            most = max(most, __shfl_xor(most, o, 64));
         }
-        units += u;
-        stages += w;
+        longest = max(longest, Uni(most));
+        units += Uni(u);
+        stages += Uni(w);
     }
-    if (units == 0) return;
+    // sequence b, from the lane that has it
+    const auto get_seq = [&](int b) {
+        if (p.seqs > 64) return LoadSeq(p, b);
+        PagedSeq s;
+        s.first = __builtin_amdgcn_readlane(mine.first, b);
+        s.n = __builtin_amdgcn_readlane(mine.n, b);
+        s.len = __builtin_amdgcn_readlane(mine.len, b);
+        s.total = __builtin_amdgcn_readlane(mine.total, b);
+        return s;
+    };
     // cut: `slots` workgroups share out the stages evenly, in one line through
     // all units; else a workgroup has one unit
-    const bool cut = p.slots > 0 && units < 4 * int64_t(p.slots);
-    int64_t share = 1, x, x_end;  // this workgroup's stages (cut) or units
-    {
-        int64_t parts = units;
-        if (cut) {
-            share = max((stages + p.slots - 1) / p.slots, min(int64_t(kMinPiece), (stages + units - 1) / units));
-            parts = (stages + share - 1) / share;
-        }
-        if (int64_t(blockIdx.x) >= parts) return;
-        x = XcdChunk(int(blockIdx.x), 0, int(parts)) * share;
-        x_end = cut ? min(x + share, stages) : x + 1;
+    const bool cut =
+        p.slots > 0 && float(longest) > CutRule<QW>::a * float(stages) / float(p.slots) + float(CutRule<QW>::c);
+    int share = 1, parts = units;
+    if (cut) {
+        share = Uni(max((stages + p.slots - 1) / p.slots, min(p.min_piece, (stages + units - 1) / units)));
+        parts = Uni((stages + share - 1) / share);
     }
-    const int64_t part = cut ? x / share : 0;
-    // the sequence that holds x: base <= x < base + its size
-    int b = 0;
-    int64_t base = 0;
+    if (int(blockIdx.x) >= parts) {
+        if (p.slots > 0 && int(blockIdx.x) >= units && int(blockIdx.x) < p.max_units && threadIdx.x == 0)
+            p.joins[blockIdx.x].pieces = 0;  // (the grid has max_units workgroups at least: none stays unwritten)
+        return;
+    }
+    const int part = XcdChunk(int(blockIdx.x), 0, parts);
+    // this workgroup's stages (cut) or units, and the sequence that holds the
+    // first: base <= x < base + its size, after `ubase` units
+    int x = part * share, b = 0, base = 0, ubase = 0;
+    const int x_end = cut ? min(x + share, stages) : x + 1;
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int64_t w = 0;
+        int u = 0, w = 0;
         if (b0 + lane < p.seqs) {
-            const PagedSeq s = LoadSeq(p, b0 + lane);
-            w = int64_t(seq_units(s)) * (cut ? seq_stages(s) : 1);
+            const PagedSeq s = b0 == 0 ? mine : LoadSeq(p, b0 + lane);
+            u = seq_units(s);
+            w = u * (cut ? seq_stages(s) : 1);
         }
-        const int64_t incl = WaveScan(w, lane) + base;
+        const int incl = WaveScan(w, lane) + base, uincl = WaveScan(u, lane) + ubase;
         const uint64_t above = __ballot(incl > x);
+        const int at = above != 0 ? __builtin_ctzll(above) : 63;
+        base = Uni(__shfl(incl - (above != 0 ? w : 0), at, 64));
+        ubase = Uni(__shfl(uincl - (above != 0 ? u : 0), at, 64));
         if (above != 0) {
-            const int at = __builtin_ctzll(above);
             b = b0 + at;
-            base = __shfl(incl - w, at, 64);
             break;
         }
-        base = __shfl(incl, 63, 64);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
 
     // fragment addresses (elements inside a K / V block), as in kr_attn.hip
-    int kaddr[D / 16], vaddr[DBLK];
-#pragma unroll
-    for (int dc = 0; dc < D / 16; ++dc) kaddr[dc] = (lane & 31) * D + KSlot<D>(lane & 31, 2 * dc + hf) * 8;
+    // (K's chunk 2 dc + hf of row lane % 32: the slot is an XOR, so step dc is
+    // the first step's address XOR 16 dc)
+    const int kaddr = (lane & 31) * D + KSlot<D>(lane & 31, hf) * 8;
+    int vaddr[DBLK];
     {
         const int s16 = lane & 15, g1 = (lane >> 4) & 1, row = 4 * hf + (s16 >> 2);
 #pragma unroll
@@ -207,42 +257,31 @@ PagedKernel(PagedParams p)
 
     while (x < x_end) {
         // ---- one unit, or the part of it that is this workgroup's
-        const PagedSeq sq = LoadSeq(p, b);
+        const PagedSeq sq = get_seq(b);
         const int qt = (sq.n * p.G + RT - 1) / RT;
         const int sb = seq_stages(sq);
-        const int64_t size = int64_t(p.HKV) * qt * (cut ? sb : 1);
-        const int64_t in = x - base;
-        const int u = int(cut ? in / sb : in);
-        const int s_lo = cut ? int(in - int64_t(u) * sb) : 0;
-        const int s_hi = cut ? int(min(int64_t(sb), s_lo + (x_end - x))) : sb;
-        const int h = u / qt, t = qt - 1 - u % qt;  // a chunk's longest rows first
-        int pieces = 1;
-        if (cut) {
-            const int64_t u0 = x - s_lo, u1 = u0 + sb;  // the unit's stages in the line
-            pieces = int((u1 - 1) / share - u0 / share) + 1;
-        }
-        const int64_t unit0 = cut ? x - s_lo : x;
+        const int size = p.HKV * qt * (cut ? sb : 1);
+        const int u = Uni(cut ? (x - base) / sb : x - base);
+        const int s_lo = cut ? x - base - u * sb : 0;
+        const int s_hi = cut ? min(sb, s_lo + (x_end - x)) : sb;
+        const int h = Uni(u / qt), t = qt - 1 - (u - h * qt);  // a chunk's longest rows first
+        const int unit0 = x - s_lo;  // the unit's first stage in the line
+        const int first = cut ? Uni(unit0 / share) : 0;
+        const int pieces = cut ? Uni((unit0 + sb - 1) / share) - first + 1 : 1;
 
         const int R = sq.n * p.G;
         const int r0 = t * RT;
         const int r = min(r0 + wq * 32 + (lane & 31), R - 1);  // (rows past the end repeat the last)
         const int tok = r / p.G;
         const bool live = r0 + wq * 32 < R;
-        const int tok_lo = r0 / p.G;                            // of the unit
-        const int wtok_hi = min(r0 + wq * 32 + 31, R - 1) / p.G;  // of this wave
-        const int kend = p.tree != nullptr ? sq.total
-                                           : int(min(int64_t(sq.total), int64_t(sq.len) + min(r0 + RT - 1, R - 1) / p.G + 1));
+        const int tok_lo = Uni(r0 / p.G);                              // of the unit
+        const int wtok_hi = Uni(min(r0 + wq * 32 + 31, R - 1) / p.G);  // of this wave
+        const int kend = p.tree != nullptr ? sq.total : min(sq.total, sq.len + Uni(min(r0 + RT - 1, R - 1) / p.G) + 1);
         const int ns = max(0, min(s_hi, (kend + SB - 1) / SB) - s_lo);
         const int32_t *table = p.table + b * p.ld_table;
         const uint16_t *kh0 = p.k + h * p.head_stride, *vh0 = p.v + h * p.head_stride;
         const uint64_t *tree = p.tree + (p.tree != nullptr ? int64_t(sq.first + tok) * p.ld_tree : 0);
 
-        uint4 qf[D / 16];
-        {
-            const uint16_t *qrow = p.q + int64_t(sq.first + tok) * p.ldq + int64_t(h * p.G + r - tok * p.G) * D;
-#pragma unroll
-            for (int dc = 0; dc < D / 16; ++dc) qf[dc] = *reinterpret_cast<const uint4 *>(qrow + dc * 16 + hf * 8);
-        }
         f32x16 oacc[DBLK];
 #pragma unroll
         for (int d = 0; d < DBLK; ++d)
@@ -255,12 +294,12 @@ PagedKernel(PagedParams p)
         // page ids of stage st's keys -> tab (one DMA instruction)
         const auto fetch_tab = [&](int st) {
             const int pg = min(PageOf(p.div, key0(st) + (lane & (BLK - 1))), p.table_pages - 1);
-            DmaTouch4(table + pg, LdsAddr(&tab[wave][st & 1][0]));
+            DmaTouch4(table + pg, LdsAddr(&tab[wave][st % NS][0]));
         };
         // tab -> offs; returns which keys of stage st are there
         const auto rows_of = [&](int st) -> uint64_t {
             const int pos = key0(st) + (lane & (BLK - 1));
-            const int id = tab[wave][st & 1][lane];
+            const int id = tab[wave][st % NS][lane];
             const bool ok = pos < sq.total && uint32_t(id) < uint32_t(p.pages);
             const uint32_t in_page = uint32_t(pos - PageOf(p.div, pos) * p.div.size);
             const int64_t off = int64_t(uint64_t(uint32_t(id)) * p.page_stride + uint64_t(in_page) * p.token_stride);
@@ -270,8 +309,8 @@ PagedKernel(PagedParams p)
         };
         // keys and values of stage st -> ring (2 DPW DMA instructions)
         const auto fetch = [&](int st) {
-            const uint32_t kdst = LdsAddr(&kring[st & 1][ks][0]) + uint32_t(wq * DPW) * 1024u;
-            const uint32_t vdst = LdsAddr(&vring[st & 1][ks][0]) + uint32_t(wq * DPW) * 1024u;
+            const uint32_t kdst = LdsAddr(&kring[st % NS][ks][0]) + uint32_t(wq * DPW) * 1024u;
+            const uint32_t vdst = LdsAddr(&vring[st % NS][ks][0]) + uint32_t(wq * DPW) * 1024u;
 #pragma unroll
             for (int j = 0; j < DPW; ++j) {
                 const int row = (wq * DPW + j) * RPD + lane / DCH;
@@ -282,117 +321,160 @@ PagedKernel(PagedParams p)
         };
         // does every row of the unit see every key of stage st
         const auto whole = [&](int st, uint64_t there) {
-            const int64_t k0 = key0(st);
-            return there == ALL && (p.tree != nullptr ? k0 + BLK <= sq.len : k0 + BLK - 1 <= int64_t(sq.len) + tok_lo);
+            return there == ALL && key0(st) + BLK <= (p.tree != nullptr ? sq.len : sq.len + tok_lo + 1);
         };
         // the values that this wave fetched for stage st: rows that are not
-        // there become 0; returns the keys whose rows are not all finite
+        // there or not all finite become 0; returns the latter
         const auto clean = [&](int st, uint64_t there) -> uint64_t {
             uint64_t bad = 0;
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < DPW; ++j) {
                 const int row = (wq * DPW + j) * RPD + lane / DCH;
-                uint4 *a = reinterpret_cast<uint4 *>(&vring[st & 1][ks][(wq * DPW + j) * 512 + lane * 8]);
+                uint4 *a = reinterpret_cast<uint4 *>(&vring[st % NS][ks][(wq * DPW + j) * 512 + lane * 8]);
                 const bool here = ((there >> row) & 1) != 0;
-                const bool nf = here && AnyNonFinite<DT>(*a);
-                if (!here) *a = make_uint4(0, 0, 0, 0);
-                uint64_t hit = __ballot(nf);
+                uint64_t hit = __ballot(here && AnyNonFinite<DT>(*a));
+                uint64_t odd_lanes = 0;
                 while (hit != 0) {
                     const int g = __builtin_ctzll(hit) / DCH;
                     bad |= 1ull << ((wq * DPW + j) * RPD + g);
-                    hit &= ~(((1ull << DCH) - 1) << (g * DCH));
+                    odd_lanes |= ((1ull << DCH) - 1) << (g * DCH);
+                    hit &= ~odd_lanes;
                 }
+                if (!here || ((odd_lanes >> lane) & 1) != 0) *a = make_uint4(0, 0, 0, 0);
             }
             WaveLdsOrder();
             return bad;
         };
         // which keys of stage st this lane's row sees
         const auto seen = [&](int st, uint64_t there) -> uint64_t {
-            const int64_t j0 = int64_t(key0(st)) - sq.len;  // new token of the first key
+            const int j0 = key0(st) - sq.len;  // new token of the first key
             if (p.tree == nullptr) {
-                const int64_t nb = tok - j0 + 1;
+                const int nb = tok - j0 + 1;
                 return there & (nb >= 64 ? ~0ull : nb <= 0 ? 0ull : (1ull << nb) - 1);
             }
-            const auto word = [&](int64_t i) { return i < p.tree_words ? tree[i] : 0ull; };
+            const auto word = [&](int i) { return i < p.tree_words ? tree[i] : 0ull; };
             uint64_t w;
             if (j0 >= 0) {
-                const int sh = int(j0 & 63);
+                const int sh = j0 & 63;
                 w = word(j0 >> 6) >> sh;
                 if (sh != 0) w |= word((j0 >> 6) + 1) << (64 - sh);
             } else {
-                const int c = int(min(-j0, int64_t(64)));
-                w = c >= 64 ? ~0ull : ((1ull << c) - 1) | (word(0) << c);
+                w = -j0 >= 64 ? ~0ull : ((1ull << -j0) - 1) | (word(0) << -j0);
             }
             return there & w;
         };
 
-        // ---- the loop over stages: stage st + 1 is fetched while st is worked
-        uint64_t there = 0, next = 0;
+        // ---- the loop over stages: up to NS - 1 later ones are in flight while
+        // one is worked; the page ids of a stage travel NS - 1 stages ahead of
+        // its rows, so that they are older than every row still in flight
+        uint4 qf[D / 16];
+        {
+            const uint16_t *qrow = p.q + int64_t(sq.first + tok) * p.ldq + int64_t(h * p.G + r - tok * p.G) * D;
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) qf[dc] = *reinterpret_cast<const uint4 *>(qrow + dc * 16 + hf * 8);
+        }
+        uint64_t there[NS];  // keys that are there: of the stage worked on and those in flight
+#pragma unroll
+        for (int i = 0; i < NS; ++i) there[i] = 0;
         if (ns > 0) {
-            fetch_tab(0);
-            KR_WAIT_VM(0);
-            there = rows_of(0);
-            if (ns > 1) fetch_tab(1);
-            fetch(0);
+#pragma unroll
+            for (int i = 0; i < NS - 1; ++i) fetch_tab(i);
+        }
+        // q is used here, on every path: a load that the compiler still counts
+        // in the loop would make it wait for the DMA there, stage by stage
+#pragma unroll
+        for (int dc = 0; dc < D / 16; ++dc) {
+            U32x4 v = __builtin_bit_cast(U32x4, qf[dc]);
+            asm volatile("" : "+v"(v));
+            qf[dc] = __builtin_bit_cast(uint4, v);
+        }
+        KR_WAIT_VM(0);
+        if (ns > 0) {
+#pragma unroll
+            for (int i = 0; i < NS - 1; ++i) {
+                fetch_tab(NS - 1 + i);
+                there[i] = rows_of(i);
+                fetch(i);
+            }
             if constexpr (QW > 1) {
-                KR_WAIT_VM(0);
-                if (!whole(0, there)) {
-                    const uint64_t bad = clean(0, there);
+                KR_WAIT_VM((NS - 2) * VM);
+                if (!whole(0, there[0])) {
+                    const uint64_t bad = clean(0, there[0]);
                     if (lane == 0) odd[0][ks][wq] = bad;
                 }
                 __syncthreads();
             }
         }
         for (int st = 0; st < ns; ++st) {
-            if (st + 1 < ns) {
-                if constexpr (QW == 1) KR_WAIT_VM(2 * DPW);  // the table entries of st + 1 (before the rows of st)
-                next = rows_of(st + 1);
-                if (st + 2 < ns) fetch_tab(st + 2);
-                fetch(st + 1);
-                if constexpr (QW == 1) {
-                    if (st + 2 < ns) KR_WAIT_VM(2 * DPW + 1);  // the rows of st
-                    else KR_WAIT_VM(2 * DPW);
-                }
-            } else if constexpr (QW == 1) {
-                KR_WAIT_VM(0);
-            }
-            const bool all = whole(st, there);
+            // (past the last stage the fetches go on, into slots that nobody
+            // reads: every stage issues the same count)
+            fetch_tab(st + 2 * NS - 2);
+            if constexpr (QW == 1) KR_WAIT_VM((NS - 1) * VM);  // the page ids of stage st + NS - 1
+            there[NS - 1] = rows_of(st + NS - 1);
+            fetch(st + NS - 1);
+            if constexpr (QW == 1) KR_WAIT_VM((NS - 1) * VM);  // the rows of st
+            const bool all = whole(st, there[0]);
             uint64_t bad = 0;
             if (!all) {
                 if constexpr (QW == 1) {
-                    bad = clean(st, there);
+                    bad = clean(st, there[0]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < QW; ++i) bad |= odd[st & 1][ks][i];
+                    for (int i = 0; i < QW; ++i) bad |= odd[st % NS][ks][i];
                 }
             }
             // skipped: no key is there, or all lie in this wave's future
-            const bool future = p.tree == nullptr && key0(st) > int64_t(sq.len) + wtok_hi;
-            if (live && there != 0 && !future) {
-                const uint16_t *K = &kring[st & 1][ks][0];
-                uint16_t *V = &vring[st & 1][ks][0];
+            const bool future = p.tree == nullptr && key0(st) > sq.len + wtok_hi;
+            if (live && there[0] != 0 && !future) {
+                const uint16_t *K = &kring[st % NS][ks][0];
+                uint16_t *V = &vring[st % NS][ks][0];
                 f32x16 sacc[KB];
 #pragma unroll
                 for (int kh = 0; kh < KB; ++kh)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) sacc[kh][v] = 0.0f;
+                {
+                    // the K fragments of step dc are read KAH steps ahead of
+                    // their MFMAs, as in kr_attn.hip
+                    constexpr int NP = D / 16, KAH = 3;
+                    uint4 kf[KB][NP];
+                    const auto rd = [&](int dc) {
 #pragma unroll
-                for (int dc = 0; dc < D / 16; ++dc)
+                        for (int kh = 0; kh < KB; ++kh)
+                            kf[kh][dc] = *reinterpret_cast<const uint4 *>(K + kh * 32 * D + (kaddr ^ (dc * 16)));
+                    };
 #pragma unroll
-                    for (int kh = 0; kh < KB; ++kh)
-                        sacc[kh] = Mfma<DT>(*reinterpret_cast<const uint4 *>(K + kh * 32 * D + kaddr[dc]), qf[dc], sacc[kh]);
+                    for (int dc = 0; dc < KAH; ++dc) rd(dc);
+#pragma unroll
+                    for (int dc = 0; dc < NP; ++dc) {
+#pragma unroll
+                        for (int kh = 0; kh < KB; ++kh) sacc[kh] = Mfma<DT>(kf[kh][dc], qf[dc], sacc[kh]);
+                        if (dc + KAH < NP) rd(dc + KAH);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x100, KB * KAH, 0);  // 0x100 LDS read, 0x008 MFMA
+#pragma unroll
+                    for (int i = 0; i < NP - KAH; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, KB, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, KB * KAH, 0);
+                }
                 // register v of half kh holds key kh*32 + 8 (v/4) + 4 hf + v%4
-                uint64_t mine = ALL;
+                uint64_t sees = ALL;
                 if (!all) {
-                    mine = seen(st, there);
-                    const uint64_t bits = mine >> (4 * hf);
+                    sees = seen(st, there[0]);
+                    const uint64_t bits = sees >> (4 * hf);
+                    const auto sees_key = [&](int i) { return ((uint32_t(bits >> (i & 32)) >> (i & 31)) & 1) != 0; };
 #pragma unroll
                     for (int kh = 0; kh < KB; ++kh)
 #pragma unroll
                         for (int v = 0; v < 16; ++v)
-                            sacc[kh][v] = ((uint32_t(bits >> (32 * kh)) >> (8 * (v >> 2) + (v & 3))) & 1) != 0 ? sacc[kh][v]
-                                                                                                          : -INFINITY;
+                            sacc[kh][v] = sees_key(kh * 32 + 8 * (v >> 2) + (v & 3)) ? sacc[kh][v] : -INFINITY;
                 }
+                // two workgroups of four row blocks share a CU: the wave in its
+                // softmax goes first (2048 rows over 8000: 311 -> 302 us), as
+                // in kr_attn.hip
+                if constexpr (QW == 4) __builtin_amdgcn_s_setprio(2);
                 float mloc = sacc[0][0];
 #pragma unroll
                 for (int kh = 0; kh < KB; ++kh)
@@ -431,69 +513,91 @@ PagedKernel(PagedParams p)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) oacc[d][v] *= alpha;
                 }
-                if (__builtin_expect(bad == 0, 1)) {
+                if constexpr (QW == 4) __builtin_amdgcn_s_setprio(0);
+                {
+                    // step i: 16 keys i / DBLK, d block i % DBLK; its V fragment
+                    // is read VAH steps ahead of its MFMA
+                    constexpr int NP = 2 * KB * DBLK;
+                    const auto rd = [&](int i) {
+                        const uint16_t *at = V + (i / DBLK) * 16 * D + vaddr[i % DBLK];
+                        const AttnS4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(const_cast<uint16_t *>(at)));
+                        const AttnS4 hi =
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(const_cast<uint16_t *>(at) + 8 * D));
+                        const AttnU2 a = __builtin_bit_cast(AttnU2, lo), z = __builtin_bit_cast(AttnU2, hi);
+                        return make_uint4(a.x, a.y, z.x, z.y);
+                    };
+                    uint4 vf[NP];
 #pragma unroll
-                    for (int c = 0; c < 2 * KB; ++c)
+                    for (int i = 0; i < VAH; ++i) vf[i] = rd(i);
 #pragma unroll
-                        for (int d = 0; d < DBLK; ++d) {
-                            const AttnS4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(V + c * 16 * D + vaddr[d]));
-                            const AttnS4 hi =
-                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(V + (c * 16 + 8) * D + vaddr[d]));
-                            const AttnU2 a = __builtin_bit_cast(AttnU2, lo), z = __builtin_bit_cast(AttnU2, hi);
-                            oacc[d] = Mfma<DT>(make_uint4(a.x, a.y, z.x, z.y), pf[c], oacc[d]);
-                        }
-                } else {
-                    // a value that is no finite number, and rows that do not
-                    // see it: only those that do may touch it
-                    uint32_t w[8 * KB];
+                    for (int i = 0; i < NP; ++i) {
+                        oacc[i % DBLK] = Mfma<DT>(vf[i], pf[i / DBLK], oacc[i % DBLK]);
+                        if (i + VAH < NP) vf[i + VAH] = rd(i + VAH);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * VAH, 0);
+#pragma unroll
+                    for (int i = 0; i < NP - VAH; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, VAH, 0);
+                }
+                // keys whose values are not all finite (zeroed in the ring):
+                // added to the rows that see them, and to no others
+                while (__builtin_expect(bad != 0, 0)) {
+                    const int key = __builtin_ctzll(bad);
+                    bad &= bad - 1;
+                    // key 16 c + 8 e2 + 4 half + e: half word e % 2 of word 4 c + 2 e2 + e / 2 in that half's lanes
+                    const int at = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);
+                    uint32_t w = 0;
 #pragma unroll
                     for (int c = 0; c < 2 * KB; ++c) {
-                        w[4 * c] = pf[c].x;
-                        w[4 * c + 1] = pf[c].y;
-                        w[4 * c + 2] = pf[c].z;
-                        w[4 * c + 3] = pf[c].w;
+                        w = at == 4 * c ? pf[c].x : w;
+                        w = at == 4 * c + 1 ? pf[c].y : w;
+                        w = at == 4 * c + 2 ? pf[c].z : w;
+                        w = at == 4 * c + 3 ? pf[c].w : w;
                     }
-#pragma unroll 1
-                    for (int i = 0; i < 8 * KB; ++i) {  // word i of the packed weights, rotated into w[0]
-                        const uint32_t own = w[0], other = uint32_t(__shfl_xor(int(own), 32, 64));
+                    w = uint32_t(__shfl(int(w), (lane & 31) + 32 * ((key >> 2) & 1), 64));
+                    const float pk = Elem<DT>::Load(uint16_t(w >> (16 * (key & 1))));
+                    const bool here = ((sees >> key) & 1) != 0;
+                    const int pos = key0(st) + key, pg = PageOf(p.div, pos);
+                    const uint16_t *row = vh0 + int64_t(uint64_t(uint32_t(table[pg])) * p.page_stride +
+                                                        uint64_t(uint32_t(pos - pg * p.div.size)) * p.token_stride);
 #pragma unroll
-                        for (int e = 0; e + 1 < 8 * KB; ++e) w[e] = w[e + 1];
-#pragma unroll 1
-                        for (int k4 = 0; k4 < 4; ++k4) {
-                            const int e = 2 * (i & 3) + (k4 & 1), kf = k4 >> 1;
-                            const int key = (i >> 2) * 16 + 8 * (e >> 2) + 4 * kf + (e & 3);
-                            const float pk = Elem<DT>::Load(uint16_t((hf == kf ? own : other) >> (16 * (k4 & 1))));
-                            const bool sees = ((mine >> key) & 1) != 0;
+                    for (int d = 0; d < DBLK; ++d)
 #pragma unroll
-                            for (int d = 0; d < DBLK; ++d)
+                        for (int g = 0; g < 4; ++g) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(row + d * 32 + 8 * g + 4 * hf);
+                            const uint32_t half[4] = {x.x, x.x >> 16, x.y, x.y >> 16};
 #pragma unroll
-                                for (int v = 0; v < 16; ++v) {
-                                    const int col = d * 32 + 8 * (v >> 2) + 4 * hf + (v & 3);
-                                    const float val = Elem<DT>::Load(V[key * D + VSlot<D>(key, col / 8) * 8 + (col & 7)]);
-                                    oacc[d][v] = sees ? __builtin_fmaf(pk, val, oacc[d][v]) : oacc[d][v];
-                                }
+                            for (int e = 0; e < 4; ++e)
+                                oacc[d][4 * g + e] =
+                                    here ? __builtin_fmaf(pk, Elem<DT>::Load(uint16_t(half[e])), oacc[d][4 * g + e])
+                                         : oacc[d][4 * g + e];
                         }
-                    }
                 }
             }
-            there = next;
+#pragma unroll
+            for (int i = 0; i + 1 < NS; ++i) there[i] = there[i + 1];
             if constexpr (QW > 1) {
-                KR_WAIT_VM(0);  // this wave's part of stage st + 1 has landed
-                if (st + 1 < ns && !whole(st + 1, next)) {
-                    const uint64_t nf = clean(st + 1, next);
-                    if (lane == 0) odd[(st + 1) & 1][ks][wq] = nf;
+                KR_WAIT_VM((NS - 2) * VM);  // this wave's part of stage st + 1 has landed
+                if (st + 1 < ns && !whole(st + 1, there[0])) {
+                    const uint64_t nf = clean(st + 1, there[0]);
+                    if (lane == 0) odd[(st + 1) % NS][ks][wq] = nf;
                 }
                 __syncthreads();
             }
         }
+        KR_WAIT_VM(0);  // (the fetches past the end too: the rings are used again)
 
         // ---- the key streams' states into stream 0's (through the rings)
         if constexpr (KW > 1) {
             constexpr int NE = DBLK * 16;
-            static_assert((KW - 1) * QW * NE * 64 * 4 <= int(sizeof(kring)) && (KW - 1) * QW * 128 * 4 <= int(sizeof(vring)),
-                          "merge area");
+            static_assert((KW - 1) * QW * NE * 64 * 4 <= int(sizeof(kring)), "merge area");
+            static_assert((KW - 1) * QW * 128 * 4 <= int(sizeof(vring)), "merge area");
             __syncthreads();
-            float *og = reinterpret_cast<float *>(&kring[0][0][0]) + lane, *mg = reinterpret_cast<float *>(&vring[0][0][0]) + lane;
+            float *og = reinterpret_cast<float *>(&kring[0][0][0]) + lane;
+            float *mg = reinterpret_cast<float *>(&vring[0][0][0]) + lane;
             if (ks > 0) {
                 const int at = (ks - 1) * QW + wq;
 #pragma unroll
@@ -524,9 +628,9 @@ PagedKernel(PagedParams p)
         }
         l += __shfl_xor(l, 32, 64);  // the two halves of a row's keys
 
-        const bool mine = live && ks == 0 && r0 + wq * 32 + (lane & 31) < R;
+        const bool out_row = live && ks == 0 && r0 + wq * 32 + (lane & 31) < R;
         if (pieces == 1) {
-            if (mine) {
+            if (out_row) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 uint16_t *orow = p.o + int64_t(sq.first + tok) * p.ldo + int64_t(h * p.G + r - tok * p.G) * D;
 #pragma unroll
@@ -541,99 +645,125 @@ PagedKernel(PagedParams p)
             }
         } else {
             // a piece of a cut unit: its (O, m, l) to a slot of this workgroup
-            // (0: the unit began before the workgroup's part, 1: in it), with
-            // device-scope stores; the last piece to arrive sums all of them
-            // in the line's order
-            constexpr int SLOT = RT * (D + 2);  // floats: O rows, then (m, l) pairs
-            float *slot = p.ws + (2 * part + (s_lo == 0 ? 1 : 0)) * SLOT;
-            if (mine) {
-                const int row = wq * 32 + (lane & 31);
+            // (0: the unit began before the workgroup's part, 1: in it), for
+            // the second launch
+            float *slot = p.ws + int64_t(2 * part + (s_lo == 0 ? 1 : 0)) * (RT * (D + 2));
+            if (out_row) {
 #pragma unroll
                 for (int d = 0; d < DBLK; ++d)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
-                        PutU128(slot + row * D + d * 32 + 8 * g + 4 * hf,
-                                make_uint4(__float_as_uint(oacc[d][4 * g]), __float_as_uint(oacc[d][4 * g + 1]),
-                                           __float_as_uint(oacc[d][4 * g + 2]), __float_as_uint(oacc[d][4 * g + 3])),
-                                true);
-                if (hf == 0) {
-                    PutU32(slot + RT * D + 2 * row, __float_as_uint(m), true);
-                    PutU32(slot + RT * D + 2 * row + 1, __float_as_uint(l), true);
-                }
+                        *reinterpret_cast<float4 *>(slot + ((wq * DBLK * 4 + d * 4 + g) * 64 + lane) * 4) = make_float4(
+                            oacc[d][4 * g], oacc[d][4 * g + 1], oacc[d][4 * g + 2], oacc[d][4 * g + 3]);
+                if (hf == 0) *reinterpret_cast<float2 *>(slot + RT * D + 2 * (wq * 32 + lane)) = make_float2(m, l);
             }
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's part is written
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                int32_t *c = p.cnt + (int64_t(b) * p.HKV + h) * p.qt_max + t;
-                const int32_t k = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                last_piece = k == pieces - 1;
-                if (last_piece) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            __syncthreads();
-            if (last_piece) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-                const int64_t p0 = unit0 / share;  // the unit's first workgroup
-                const int nrow = min(RT, R - r0);
-                for (int ch = int(threadIdx.x); ch < nrow * (D / 4); ch += THREADS) {
-                    const int row = ch / (D / 4);
-                    float acc[4] = {}, mm = -INFINITY, ll = 0.0f;
-                    constexpr int UN = 8;  // pieces in flight
-                    for (int i0 = 0; i0 < pieces; i0 += UN) {
-                        uint4 ov[UN];
-                        float mp[UN], lp[UN];
-#pragma unroll
-                        for (int i = 0; i < UN; ++i) {
-                            mp[i] = -INFINITY;
-                            lp[i] = 0.0f;
-                            ov[i] = make_uint4(0, 0, 0, 0);
-                            if (i0 + i < pieces) {
-                                const int64_t pt = p0 + i0 + i;
-                                const float *s = p.ws + (2 * pt + (pt * share <= unit0 ? 1 : 0)) * SLOT;
-                                ov[i] = LoadU128Dev(s, ch * 16);
-                                mp[i] = __hip_atomic_load(s + RT * D + 2 * row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                                lp[i] = __hip_atomic_load(s + RT * D + 2 * row + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                            }
-                        }
-                        float mn = mm;
-#pragma unroll
-                        for (int i = 0; i < UN; ++i) mn = __builtin_elementwise_maximum(mn, mp[i]);
-                        const float ms = mn == -INFINITY ? 0.0f : mn;
-                        const float a0 = __builtin_amdgcn_exp2f(mm - ms);
-                        ll *= a0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[e] *= a0;
-#pragma unroll
-                        for (int i = 0; i < UN; ++i) {
-                            const float a = __builtin_amdgcn_exp2f(mp[i] - ms);
-                            ll = __builtin_fmaf(lp[i], a, ll);
-                            acc[0] = __builtin_fmaf(__uint_as_float(ov[i].x), a, acc[0]);
-                            acc[1] = __builtin_fmaf(__uint_as_float(ov[i].y), a, acc[1]);
-                            acc[2] = __builtin_fmaf(__uint_as_float(ov[i].z), a, acc[2]);
-                            acc[3] = __builtin_fmaf(__uint_as_float(ov[i].w), a, acc[3]);
-                        }
-                        mm = mn;
-                    }
-                    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-                    const int tk = (r0 + row) / p.G, g = r0 + row - tk * p.G;
-                    uint2 w;
-                    w.x = Pack2<DT>(acc[0] * inv, acc[1] * inv);
-                    w.y = Pack2<DT>(acc[2] * inv, acc[3] * inv);
-                    *reinterpret_cast<uint2 *>(p.o + int64_t(sq.first + tk) * p.ldo + int64_t(h * p.G + g) * D +
-                                               (ch - row * (D / 4)) * 4) = w;
-                }
-            }
+        }
+        if (p.slots > 0 && s_lo == 0 && threadIdx.x == 0 && ubase + u < p.max_units) {
+            PagedJoin &j = p.joins[ubase + u];
+            j.pieces = pieces;
+            j.part = part;
+            j.first = sq.first;
+            j.r0 = r0;
+            j.nrow = min(RT, R - r0);
+            j.head = h * p.G;
         }
         x += cut ? s_hi - s_lo : 1;
         if (x < x_end) {
-            __syncthreads();  // the rings and last_piece are free again
+            __syncthreads();  // the rings are free again
             if (x >= base + size) {  // on to the next sequence with new tokens
                 base += size;
+                ubase += p.HKV * qt;
                 do {
-                    if (++b >= p.seqs) return;
-                } while (seq_units(LoadSeq(p, b)) == 0);
+                    ++b;
+                } while (b < p.seqs && seq_units(get_seq(b)) == 0);
+                if (b >= p.seqs) break;
             }
         }
     }
+}
+
+// The second launch: sums the pieces of the cut units, in the line's order.
+// Workgroup (x, y) takes 256 / SP chunks of 4 columns of unit x, SP threads to
+// a chunk with a share of its pieces each, UN of them in flight: units of few
+// rows come in up to 64 pieces, those of many in a few.
+template <int QW> struct JoinShape {
+    static constexpr int SP = 4 / QW, UN = QW == 4 ? 4 : 8, CH = 256 / SP;
+};
+
+template <int DT, int D, int QW>
+__global__ void __launch_bounds__(256)
+PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ldo, int G)
+{
+    constexpr int RT = 32 * QW, DBLK = D / 32, SLOT = RT * (D + 2);
+    constexpr int SP = JoinShape<QW>::SP, UN = JoinShape<QW>::UN, CH = JoinShape<QW>::CH;
+    __shared__ float part_sum[SP > 1 ? SP - 1 : 1][6][CH];
+    const PagedJoin j = joins[blockIdx.x];
+    if (j.pieces < 2 || int(blockIdx.y) * CH >= j.nrow * (D / 4)) return;
+    const int tx = int(threadIdx.x) % CH, sp = int(threadIdx.x) / CH;
+    const int ch = min(int(blockIdx.y) * CH + tx, j.nrow * (D / 4) - 1);
+    // columns 4 cc.. of row ch % nrow, and the lane and store that hold them:
+    // d = cc / 8, g = cc / 2 % 4, lane half cc % 2
+    const int cc = ch / j.nrow, row = ch - cc * j.nrow;
+    const int at = ((row >> 5) * DBLK * 4 + (cc >> 1)) * 64 + (cc & 1) * 32 + (row & 31);
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+    const int i_lo = j.pieces * sp / SP, i_hi = j.pieces * (sp + 1) / SP;
+    for (int i0 = i_lo; i0 < i_hi; i0 += UN) {
+        float4 ov[UN];
+        float2 ml[UN];
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int pc = min(i0 + i, i_hi - 1);  // (past the end the last again, left out below)
+            const float *s = ws + int64_t(2 * (j.part + pc) + (pc == 0 ? 1 : 0)) * SLOT;
+            ml[i] = *reinterpret_cast<const float2 *>(s + RT * D + 2 * row);
+            ov[i] = *reinterpret_cast<const float4 *>(s + at * 4);
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) mn = __builtin_elementwise_maximum(mn, ml[i].x);
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        const float a0 = __builtin_amdgcn_exp2f(m - ms);
+        l *= a0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= a0;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const bool in = i0 + i < i_hi;
+            const float a = __builtin_amdgcn_exp2f(ml[i].x - ms);
+            l = in ? __builtin_fmaf(ml[i].y, a, l) : l;
+            acc[0] = in ? __builtin_fmaf(ov[i].x, a, acc[0]) : acc[0];
+            acc[1] = in ? __builtin_fmaf(ov[i].y, a, acc[1]) : acc[1];
+            acc[2] = in ? __builtin_fmaf(ov[i].z, a, acc[2]) : acc[2];
+            acc[3] = in ? __builtin_fmaf(ov[i].w, a, acc[3]) : acc[3];
+        }
+        m = mn;
+    }
+    if constexpr (SP > 1) {
+        if (sp > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part_sum[sp - 1][e][tx] = acc[e];
+            part_sum[sp - 1][4][tx] = m;
+            part_sum[sp - 1][5][tx] = l;
+        }
+        __syncthreads();
+        if (sp > 0) return;
+#pragma unroll
+        for (int i = 0; i < SP - 1; ++i) {
+            const float m1 = part_sum[i][4][tx], mn = __builtin_elementwise_maximum(m, m1);
+            const float ms = mn == -INFINITY ? 0.0f : mn;
+            const float a0 = __builtin_amdgcn_exp2f(m - ms), a1 = __builtin_amdgcn_exp2f(m1 - ms);
+            l = __builtin_fmaf(part_sum[i][5][tx], a1, l * a0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part_sum[i][e][tx], a1, acc[e] * a0);
+            m = mn;
+        }
+    }
+    if (int(blockIdx.y) * CH + tx >= j.nrow * (D / 4)) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int tok = (j.r0 + row) / G, g = j.r0 + row - tok * G;
+    uint2 w;
+    w.x = Pack2<DT>(acc[0] * inv, acc[1] * inv);
+    w.y = Pack2<DT>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2 *>(o + int64_t(j.first + tok) * ldo + int64_t(j.head + g) * D + cc * 4) = w;
 }
 
 // Rows a unit holds for this many rows of a sequence and key head.
@@ -642,9 +772,9 @@ int UnitWaves(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 template <int DT, int D, int QW>
 const void *PagedFn()
 {
-    if constexpr (QW == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1>);
-    else if constexpr (QW == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1>);
-    else return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2>);
+    if constexpr (QW == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1, 2>);
+    else if constexpr (QW == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1, 2>);
+    else return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2, 2>);
 }
 
 int PagedThreads(int qw) { return qw == 1 ? 128 : 256; }
@@ -662,14 +792,11 @@ const void *PagedFor(int dtype, int D, int qw)
     return pick(PagedFn<kF16, 64, 4>, PagedFn<kF16, 128, 4>);
 }
 
-// Workgroups of the cut schedule: two on each of 256 CUs (their rings fill 128
-// of a CU's 160 KB at head size 128).
-constexpr int kPagedSlots = 512;
-
 struct PagedShape {
-    int qw, qt_max;
+    int qw;
+    int64_t units;  // at most
     size_t ws_bytes;
-    int64_t counters;
+    int counters;
 };
 
 PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
@@ -681,11 +808,31 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     PagedShape r;
     r.qw = UnitWaves(most);
     const int64_t qt = (most + 32 * r.qw - 1) / (32 * r.qw);
-    r.counters = qt * c.heads * s.seqs;
-    if (r.counters >= (int64_t(1) << 31)) throw std::runtime_error("attention_paged: too many rows for one launch");
-    r.qt_max = int(qt);
-    r.ws_bytes = r.counters == 0 ? 0 : size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4;
+    r.units = qt * c.heads * s.seqs;
+    if (r.units >= (int64_t(1) << 31)) throw std::runtime_error("attention_paged: too many rows for one launch");
+    // nothing is cut where the table holds no unit long enough, or the line of
+    // stages (64 keys each) would not fit 32 bits
+    const int64_t most_stages = (int64_t(s.table_pages) * c.page_size + 63) / 64;
+    const int at_least = r.qw == 1 ? CutRule<1>::c : r.qw == 2 ? CutRule<2>::c : CutRule<4>::c;
+    const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 31);
+    r.ws_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
+    if (r.units > (int64_t(1) << 31) / 8 - 1) throw std::runtime_error("attention_paged: too many rows for one launch");
+    r.counters = cuts ? int(r.units) * int(sizeof(PagedJoin) / 4) : 0;
     return r;
+}
+
+template <int DT, int D>
+void JoinGo(int qw, const PagedParams &p, hipStream_t stream)
+{
+    const int64_t rows = std::min(int64_t(p.max_new) * p.G, int64_t(32 * qw));
+    const int64_t per = qw == 1 ? JoinShape<1>::CH : qw == 2 ? JoinShape<2>::CH : JoinShape<4>::CH;
+    const dim3 grid(unsigned(p.max_units), unsigned((rows * (D / 4) + per - 1) / per));
+    const auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p.ws, p.joins, p.o, p.ldo, p.G);
+    };
+    if (qw == 1) go(PagedJoinKernel<DT, D, 1>);
+    else if (qw == 2) go(PagedJoinKernel<DT, D, 2>);
+    else go(PagedJoinKernel<DT, D, 4>);
 }
 
 }  // namespace
@@ -696,7 +843,7 @@ void PagedAttnNeeds(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *
     CheckSeqs(seqs, "attention_paged");
     const PagedShape f = ShapeOf(c, *seqs, HQ);
     *ws_bytes = f.ws_bytes;
-    *counters = int(f.counters);
+    *counters = f.counters;
 }
 
 void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
@@ -744,26 +891,33 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     p.HQ = d.HQ;
     p.HKV = c.heads;
     p.G = d.HQ / c.heads;
-    p.qt_max = f.qt_max;
     p.scale_log2 = d.scale * 1.4426950408889634f;
     p.div = MakePageDiv(c.page_size);
-    if (d.ws != nullptr) {
+    // a piece's cost grows with its rows (measured: 1 to 8 tokens of 4 heads best at 2 to 4, 32 and more at 8 to 12)
+    p.min_piece = 2 + int(std::min<int64_t>(int64_t(s.max_new) * p.G, 128)) / 16;
+    if (d.ws != nullptr && f.ws_bytes > 0) {
         if (d.cnt == nullptr || d.ws_bytes < f.ws_bytes || d.cnt_len < f.counters ||
-            (reinterpret_cast<uintptr_t>(d.ws) & 15) != 0)
+            ((reinterpret_cast<uintptr_t>(d.ws) | reinterpret_cast<uintptr_t>(d.cnt)) & 15) != 0)
             refuse("the workspace is too small or misaligned");
         p.ws = static_cast<float *>(d.ws);
-        p.cnt = d.cnt;
+        p.joins = reinterpret_cast<PagedJoin *>(d.cnt);
         p.slots = kPagedSlots;
     }
     // whole units: at most one more row block per sequence than its rows fill
     const int64_t units =
-        std::min(f.counters, int64_t(c.heads) * (int64_t(d.rows) * p.G / (32 * f.qw) + std::min(s.seqs, d.rows)));
+        std::min(f.units, int64_t(c.heads) * (int64_t(d.rows) * p.G / (32 * f.qw) + std::min(s.seqs, d.rows)));
+    p.max_units = int(units);
     const int64_t wg = std::max<int64_t>(units, p.slots);
     if (wg >= (int64_t(1) << 31)) refuse("too many rows for one launch");
     void *args[] = {&p};
     Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw), dim3(unsigned(wg)), dim3(unsigned(PagedThreads(f.qw))),
                           args, 0, stream),
           "attention_paged launch");
+    if (p.slots > 0) {
+        const bool bf = c.dtype == kBF16;
+        if (c.head_dim == 64) bf ? JoinGo<kBF16, 64>(f.qw, p, stream) : JoinGo<kF16, 64>(f.qw, p, stream);
+        else bf ? JoinGo<kBF16, 128>(f.qw, p, stream) : JoinGo<kF16, 128>(f.qw, p, stream);
+    }
     Check(hipGetLastError(), "attention_paged launch");
 }
 
