@@ -339,10 +339,10 @@ int kr_op_qk_norm_rope_cache(const kr_rope *rope, const kr_cache *cache, int lay
  * included. ws / counters: caller-owned device memory of at least the sizes
  * kr_op_attention_paged_workspace reports (functions of the handles' host
  * fields alone; both 0 where no sequence is long enough), with which long
- * sequences are cut into pieces that run side by side and are summed in order
- * by a second launch. They need not be initialised and hold nothing between
- * calls; calls sharing them must be ordered. NULL: uncut. The bits depend on
- * the batch's lengths, not on which piece ends when. */
+ * sequences are cut into pieces that run side by side and are summed in order;
+ * the counters must be zero before the first call and are left zero; calls
+ * sharing them must be ordered. NULL: uncut. The bits depend on the batch's
+ * lengths, not on which piece ends when. */
 int kr_op_attention_paged_workspace(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_bytes,
                                     int *counters);
 int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,

@@ -37,6 +37,7 @@
 #include "kr_attncore.h"
 #include "kr_dma.h"
 #include "kr_paged.h"
+#include "kr_rowcore.h"
 
 namespace kr {
 
@@ -62,8 +63,9 @@ struct PagedParams {
     int cap, pages, table_pages, seqs, rows, max_new, tree_words, HQ, HKV, G;
     float scale_log2;
     PageDiv div;
+    int32_t *cnt;      // [max_units] arrival tickets, zero between launches; or NULL: a second launch sums
     float *ws;         // two partial slots per workgroup of the cut schedule
-    PagedJoin *joins;  // [max_units], unit by unit as they come in the line
+    PagedJoin *joins;  // [max_units], unit by unit as they come in the line; or NULL: tickets
     int max_units;
     int min_piece;     // stages of a piece, unless the units are shorter
     int slots;         // workgroups of the cut schedule; 0: whole units only
@@ -109,6 +111,17 @@ __device__ __forceinline__ void WaveLdsOrder()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// 8 bytes at byte offset `off` of a wave-uniform base, at device scope (as
+// LoadU128Dev).
+__device__ __forceinline__ uint2 LoadU64Dev(const void *base, int off)
+{
+    typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), short(0), 0x7fffffff, 0x00020000);
+    const U32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 16 /* sc1 */);
+    return make_uint2(v.x, v.y);
+}
+
 // Any 16-bit value of the eight that is an infinity or a NaN.
 template <int DT>
 __device__ __forceinline__ bool AnyNonFinite(const uint4 &x)
@@ -117,6 +130,88 @@ __device__ __forceinline__ bool AnyNonFinite(const uint4 &x)
     bool bad = false;
     for (const uint32_t w : {x.x, x.y, x.z, x.w}) bad = bad || (w & E) == E || ((w >> 16) & E) == E;
     return bad;
+}
+
+// Sums pieces lo .. hi - 1 of a unit whose first piece is slot 1 of workgroup
+// `part` (the others slot 0 of the next ones) for one chunk: 4 columns of a
+// row, UN pieces in flight. DEV: written by workgroups of the running launch,
+// so read at device scope.
+struct PieceSum {
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+};
+
+// Chunk ch of a unit's nrow rows: columns 4 cc.. of row ch % nrow, and where a
+// slot has them: lane and store as d = cc / 8, g = cc / 2 % 4, half cc % 2.
+template <int D> struct PieceChunk {
+    int cc, row, at;
+    __device__ __forceinline__ PieceChunk(int ch, int nrow)
+    {
+        cc = ch / nrow;
+        row = ch - cc * nrow;
+        at = ((row >> 5) * (D / 8) + (cc >> 1)) * 64 + (cc & 1) * 32 + (row & 31);
+    }
+};
+
+template <int D, int QW, int UN, bool DEV>
+__device__ __forceinline__ PieceSum SumPieces(const float *ws, int part, int lo, int hi, const PieceChunk<D> &c)
+{
+    constexpr int RT = 32 * QW, SLOT = RT * (D + 2);
+    PieceSum s;
+    for (int i0 = lo; i0 < hi; i0 += UN) {
+        float ov[UN][4], mp[UN], lp[UN];
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int pc = min(i0 + i, hi - 1);  // (past the end the last again, left out below)
+            const float *slot = ws + int64_t(2 * (part + pc) + (pc == 0 ? 1 : 0)) * SLOT;
+            uint4 o;
+            uint2 ml;
+            if constexpr (DEV) {
+                o = LoadU128Dev(slot, c.at * 16);
+                ml = LoadU64Dev(slot, (RT * D + 2 * c.row) * 4);
+            } else {
+                o = *reinterpret_cast<const uint4 *>(slot + c.at * 4);
+                ml = *reinterpret_cast<const uint2 *>(slot + RT * D + 2 * c.row);
+            }
+            ov[i][0] = __uint_as_float(o.x);
+            ov[i][1] = __uint_as_float(o.y);
+            ov[i][2] = __uint_as_float(o.z);
+            ov[i][3] = __uint_as_float(o.w);
+            mp[i] = __uint_as_float(ml.x);
+            lp[i] = __uint_as_float(ml.y);
+        }
+        float mn = s.m;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) mn = __builtin_elementwise_maximum(mn, mp[i]);
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        const float a0 = __builtin_amdgcn_exp2f(s.m - ms);
+        s.l *= a0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.acc[e] *= a0;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const bool in = i0 + i < hi;
+            const float a = __builtin_amdgcn_exp2f(mp[i] - ms);
+            s.l = in ? __builtin_fmaf(lp[i], a, s.l) : s.l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s.acc[e] = in ? __builtin_fmaf(ov[i][e], a, s.acc[e]) : s.acc[e];
+        }
+        s.m = mn;
+    }
+    return s;
+}
+
+// A chunk's result to its row: row r of the unit's packed rows is new token
+// r / G, query head `head` + r % G.
+template <int DT>
+__device__ __forceinline__ void StoreSum(const PieceSum &s, uint16_t *o, int64_t ldo, int first, int r, int head, int G,
+                                         int D, int cc)
+{
+    const float inv = s.l == 0.0f ? 0.0f : 1.0f / s.l;
+    const int tok = r / G;
+    uint2 w;
+    w.x = Pack2<DT>(s.acc[0] * inv, s.acc[1] * inv);
+    w.y = Pack2<DT>(s.acc[2] * inv, s.acc[3] * inv);
+    *reinterpret_cast<uint2 *>(o + int64_t(first + tok) * ldo + int64_t(head + r - tok * G) * D + cc * 4) = w;
 }
 
 // Workgroups of the cut schedule: two on each of 256 CUs (their rings fill 128
@@ -163,6 +258,7 @@ PagedKernel(PagedParams p)
     __shared__ __attribute__((aligned(256))) int32_t tab[NW][NS][64];  // page ids of a stage's keys
     __shared__ int64_t offs[NW][64];                                  // and their rows' element offsets
     __shared__ uint64_t odd[NS][KW][QW];                               // keys whose values are not all finite
+    __shared__ int last_piece;
 
     const int lane = int(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
@@ -214,7 +310,7 @@ PagedKernel(PagedParams p)
         parts = Uni((stages + share - 1) / share);
     }
     if (int(blockIdx.x) >= parts) {
-        if (p.slots > 0 && int(blockIdx.x) >= units && int(blockIdx.x) < p.max_units && threadIdx.x == 0)
+        if (p.joins != nullptr && int(blockIdx.x) >= units && int(blockIdx.x) < p.max_units && threadIdx.x == 0)
             p.joins[blockIdx.x].pieces = 0;  // (the grid has max_units workgroups at least: none stays unwritten)
         return;
     }
@@ -645,20 +741,48 @@ PagedKernel(PagedParams p)
             }
         } else {
             // a piece of a cut unit: its (O, m, l) to a slot of this workgroup
-            // (0: the unit began before the workgroup's part, 1: in it), for
-            // the second launch
+            // (0: the unit began before the workgroup's part, 1: in it). With
+            // tickets by device-scope stores, else for the second launch.
+            const bool coh = p.cnt != nullptr;
             float *slot = p.ws + int64_t(2 * part + (s_lo == 0 ? 1 : 0)) * (RT * (D + 2));
             if (out_row) {
 #pragma unroll
                 for (int d = 0; d < DBLK; ++d)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
-                        *reinterpret_cast<float4 *>(slot + ((wq * DBLK * 4 + d * 4 + g) * 64 + lane) * 4) = make_float4(
-                            oacc[d][4 * g], oacc[d][4 * g + 1], oacc[d][4 * g + 2], oacc[d][4 * g + 3]);
-                if (hf == 0) *reinterpret_cast<float2 *>(slot + RT * D + 2 * (wq * 32 + lane)) = make_float2(m, l);
+                        PutU128(slot + ((wq * DBLK * 4 + d * 4 + g) * 64 + lane) * 4,
+                                make_uint4(__float_as_uint(oacc[d][4 * g]), __float_as_uint(oacc[d][4 * g + 1]),
+                                           __float_as_uint(oacc[d][4 * g + 2]), __float_as_uint(oacc[d][4 * g + 3])),
+                                coh);
+                if (hf == 0) {
+                    float *ml = slot + RT * D + 2 * (wq * 32 + lane);
+                    PutU32(ml, __float_as_uint(m), coh);
+                    PutU32(ml + 1, __float_as_uint(l), coh);
+                }
+            }
+            if (coh && ubase + u < p.max_units) {
+                // the last piece to arrive sums all of them, in the line's order
+                __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's part is written
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    int32_t *c = p.cnt + ubase + u;
+                    const int32_t k = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    last_piece = k == pieces - 1;
+                    if (last_piece) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (last_piece) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                    const int nrow = min(RT, R - r0);
+                    for (int ch = int(threadIdx.x); ch < nrow * (D / 4); ch += 64 * NW) {
+                        const PieceChunk<D> c(ch, nrow);
+                        const PieceSum s = SumPieces<D, QW, 8, true>(p.ws, first, 0, pieces, c);
+                        StoreSum<DT>(s, p.o, p.ldo, sq.first, r0 + c.row, h * p.G, p.G, D, c.cc);
+                    }
+                }
             }
         }
-        if (p.slots > 0 && s_lo == 0 && threadIdx.x == 0 && ubase + u < p.max_units) {
+        if (p.joins != nullptr && s_lo == 0 && threadIdx.x == 0 && ubase + u < p.max_units) {
             PagedJoin &j = p.joins[ubase + u];
             j.pieces = pieces;
             j.part = part;
@@ -694,76 +818,37 @@ template <int DT, int D, int QW>
 __global__ void __launch_bounds__(256)
 PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ldo, int G)
 {
-    constexpr int RT = 32 * QW, DBLK = D / 32, SLOT = RT * (D + 2);
-    constexpr int SP = JoinShape<QW>::SP, UN = JoinShape<QW>::UN, CH = JoinShape<QW>::CH;
+    constexpr int SP = JoinShape<QW>::SP, CH = JoinShape<QW>::CH;
     __shared__ float part_sum[SP > 1 ? SP - 1 : 1][6][CH];
     const PagedJoin j = joins[blockIdx.x];
-    if (j.pieces < 2 || int(blockIdx.y) * CH >= j.nrow * (D / 4)) return;
+    const int chunks = j.nrow * (D / 4);
+    if (j.pieces < 2 || int(blockIdx.y) * CH >= chunks) return;
     const int tx = int(threadIdx.x) % CH, sp = int(threadIdx.x) / CH;
-    const int ch = min(int(blockIdx.y) * CH + tx, j.nrow * (D / 4) - 1);
-    // columns 4 cc.. of row ch % nrow, and the lane and store that hold them:
-    // d = cc / 8, g = cc / 2 % 4, lane half cc % 2
-    const int cc = ch / j.nrow, row = ch - cc * j.nrow;
-    const int at = ((row >> 5) * DBLK * 4 + (cc >> 1)) * 64 + (cc & 1) * 32 + (row & 31);
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-    const int i_lo = j.pieces * sp / SP, i_hi = j.pieces * (sp + 1) / SP;
-    for (int i0 = i_lo; i0 < i_hi; i0 += UN) {
-        float4 ov[UN];
-        float2 ml[UN];
-#pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const int pc = min(i0 + i, i_hi - 1);  // (past the end the last again, left out below)
-            const float *s = ws + int64_t(2 * (j.part + pc) + (pc == 0 ? 1 : 0)) * SLOT;
-            ml[i] = *reinterpret_cast<const float2 *>(s + RT * D + 2 * row);
-            ov[i] = *reinterpret_cast<const float4 *>(s + at * 4);
-        }
-        float mn = m;
-#pragma unroll
-        for (int i = 0; i < UN; ++i) mn = __builtin_elementwise_maximum(mn, ml[i].x);
-        const float ms = mn == -INFINITY ? 0.0f : mn;
-        const float a0 = __builtin_amdgcn_exp2f(m - ms);
-        l *= a0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] *= a0;
-#pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const bool in = i0 + i < i_hi;
-            const float a = __builtin_amdgcn_exp2f(ml[i].x - ms);
-            l = in ? __builtin_fmaf(ml[i].y, a, l) : l;
-            acc[0] = in ? __builtin_fmaf(ov[i].x, a, acc[0]) : acc[0];
-            acc[1] = in ? __builtin_fmaf(ov[i].y, a, acc[1]) : acc[1];
-            acc[2] = in ? __builtin_fmaf(ov[i].z, a, acc[2]) : acc[2];
-            acc[3] = in ? __builtin_fmaf(ov[i].w, a, acc[3]) : acc[3];
-        }
-        m = mn;
-    }
+    const int ch = int(blockIdx.y) * CH + tx;
+    const PieceChunk<D> c(min(ch, chunks - 1), j.nrow);
+    const int lo = j.pieces * sp / SP, hi = j.pieces * (sp + 1) / SP;
+    PieceSum s = SumPieces<D, QW, JoinShape<QW>::UN, false>(ws, j.part, lo, hi, c);
     if constexpr (SP > 1) {
         if (sp > 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part_sum[sp - 1][e][tx] = acc[e];
-            part_sum[sp - 1][4][tx] = m;
-            part_sum[sp - 1][5][tx] = l;
+            for (int e = 0; e < 4; ++e) part_sum[sp - 1][e][tx] = s.acc[e];
+            part_sum[sp - 1][4][tx] = s.m;
+            part_sum[sp - 1][5][tx] = s.l;
         }
         __syncthreads();
         if (sp > 0) return;
 #pragma unroll
         for (int i = 0; i < SP - 1; ++i) {
-            const float m1 = part_sum[i][4][tx], mn = __builtin_elementwise_maximum(m, m1);
+            const float m1 = part_sum[i][4][tx], mn = __builtin_elementwise_maximum(s.m, m1);
             const float ms = mn == -INFINITY ? 0.0f : mn;
-            const float a0 = __builtin_amdgcn_exp2f(m - ms), a1 = __builtin_amdgcn_exp2f(m1 - ms);
-            l = __builtin_fmaf(part_sum[i][5][tx], a1, l * a0);
+            const float a0 = __builtin_amdgcn_exp2f(s.m - ms), a1 = __builtin_amdgcn_exp2f(m1 - ms);
+            s.l = __builtin_fmaf(part_sum[i][5][tx], a1, s.l * a0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part_sum[i][e][tx], a1, acc[e] * a0);
-            m = mn;
+            for (int e = 0; e < 4; ++e) s.acc[e] = __builtin_fmaf(part_sum[i][e][tx], a1, s.acc[e] * a0);
+            s.m = mn;
         }
     }
-    if (int(blockIdx.y) * CH + tx >= j.nrow * (D / 4)) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int tok = (j.r0 + row) / G, g = j.r0 + row - tok * G;
-    uint2 w;
-    w.x = Pack2<DT>(acc[0] * inv, acc[1] * inv);
-    w.y = Pack2<DT>(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2 *>(o + int64_t(j.first + tok) * ldo + int64_t(j.head + g) * D + cc * 4) = w;
+    if (ch < chunks) StoreSum<DT>(s, o, ldo, j.first, j.r0 + c.row, j.head, G, D, c.cc);
 }
 
 // Rows a unit holds for this many rows of a sequence and key head.
@@ -792,10 +877,19 @@ const void *PagedFor(int dtype, int D, int qw)
     return pick(PagedFn<kF16, 64, 4>, PagedFn<kF16, 128, 4>);
 }
 
+// Units from which the pieces of a cut one are summed by the last of them
+// (tickets) instead of a second launch. That many units are cut only where
+// their lengths differ a lot, and the launch costs 2 to 4 us all the same (64
+// sequences of up to 500 tokens, 4 key heads: 20 with it, 18 us without); where
+// cutting is the rule it is the faster (4 sequences of up to 2000, 2 key heads:
+// 13 us against 15).
+constexpr int kTicketUnits = 192;
+
 struct PagedShape {
     int qw;
     int64_t units;  // at most
-    size_t ws_bytes;
+    bool tickets;
+    size_t part_bytes, ws_bytes;
     int counters;
 };
 
@@ -815,9 +909,11 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     const int64_t most_stages = (int64_t(s.table_pages) * c.page_size + 63) / 64;
     const int at_least = r.qw == 1 ? CutRule<1>::c : r.qw == 2 ? CutRule<2>::c : CutRule<4>::c;
     const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 31);
-    r.ws_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
-    if (r.units > (int64_t(1) << 31) / 8 - 1) throw std::runtime_error("attention_paged: too many rows for one launch");
-    r.counters = cuts ? int(r.units) * int(sizeof(PagedJoin) / 4) : 0;
+    // a ticket, or a note for the second launch, per unit
+    r.tickets = cuts && r.units >= kTicketUnits;
+    r.part_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
+    r.ws_bytes = r.part_bytes + (cuts && !r.tickets ? size_t(r.units) * sizeof(PagedJoin) : 0);
+    r.counters = r.tickets ? int(r.units) : 0;
     return r;
 }
 
@@ -896,11 +992,12 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     // a piece's cost grows with its rows (measured: 1 to 8 tokens of 4 heads best at 2 to 4, 32 and more at 8 to 12)
     p.min_piece = 2 + int(std::min<int64_t>(int64_t(s.max_new) * p.G, 128)) / 16;
     if (d.ws != nullptr && f.ws_bytes > 0) {
-        if (d.cnt == nullptr || d.ws_bytes < f.ws_bytes || d.cnt_len < f.counters ||
-            ((reinterpret_cast<uintptr_t>(d.ws) | reinterpret_cast<uintptr_t>(d.cnt)) & 15) != 0)
+        if (d.ws_bytes < f.ws_bytes || (f.tickets && (d.cnt == nullptr || d.cnt_len < f.counters)) ||
+            (reinterpret_cast<uintptr_t>(d.ws) & 15) != 0 || (reinterpret_cast<uintptr_t>(d.cnt) & 3) != 0)
             refuse("the workspace is too small or misaligned");
         p.ws = static_cast<float *>(d.ws);
-        p.joins = reinterpret_cast<PagedJoin *>(d.cnt);
+        if (f.tickets) p.cnt = d.cnt;
+        else p.joins = reinterpret_cast<PagedJoin *>(static_cast<char *>(d.ws) + f.part_bytes);
         p.slots = kPagedSlots;
     }
     // whole units: at most one more row block per sequence than its rows fill
@@ -913,7 +1010,7 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw), dim3(unsigned(wg)), dim3(unsigned(PagedThreads(f.qw))),
                           args, 0, stream),
           "attention_paged launch");
-    if (p.slots > 0) {
+    if (p.joins != nullptr) {
         const bool bf = c.dtype == kBF16;
         if (c.head_dim == 64) bf ? JoinGo<kBF16, 64>(f.qw, p, stream) : JoinGo<kF16, 64>(f.qw, p, stream);
         else bf ? JoinGo<kBF16, 128>(f.qw, p, stream) : JoinGo<kF16, 128>(f.qw, p, stream);

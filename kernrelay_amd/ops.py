@@ -518,8 +518,8 @@ def attention_paged_workspace(cache, seqs, HQ):
 def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
     """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
     cache; their own keys and values are in the cache already. ws (uint8) and
-    counters (int32): of attention_paged_workspace's sizes, their contents of no
-    matter, for one stream at a time; None: no sequence is cut into pieces."""
+    counters (int32, zero before the first call): of attention_paged_workspace's
+    sizes, for one stream at a time; None: no sequence is cut into pieces."""
     who = "attention_paged"
     _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
     shape, dt, dev = q.shape, cache.torch_dtype, cache.device

@@ -222,7 +222,7 @@ class Batch:
     def space(self):
         nbytes, ncnt = ops.attention_paged_workspace(self.cache, self.seqs, self.HQ)
         return dict(ws=torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda"),
-                    counters=torch.full((ncnt,), -1, dtype=torch.int32, device="cuda"))
+                    counters=torch.zeros(ncnt, dtype=torch.int32, device="cuda"))
 
     def run(self, scale=None, cut=True, **kw):
         out = torch.full_like(self.q, 9.0)
@@ -307,6 +307,33 @@ def test_attention_long_chunks(gpu, lens, news):
     b.check(b.run())
     b = Batch(3, 7, 1, 128, HF, 40, lens, news)
     b.check(b.run())
+
+
+@pytest.mark.parametrize("D,HQ,HKV,dt", [(128, 28, 4, BF), (64, 14, 2, HF)])
+@pytest.mark.parametrize("most", [1, 9, 17])
+def test_attention_uneven_batches(gpu, most, D, HQ, HKV, dt):
+    """One long sequence among many short ones, some without new tokens, in 32,
+    64 and 128 packed rows: its units are cut though there are hundreds; every
+    call leaves the counters zero and gives the same bits."""
+    announce("attention_paged uneven %s" % ((most, D, HQ, HKV, dt),))
+    rng = random.Random(most)
+    n = 400 // HKV
+    lens = [rng.randint(0, 40) for _ in range(n)]
+    lens[n // 3] = 9000
+    news = [rng.choice((0, 1, most, most)) for _ in range(n)]
+    news[n // 3] = most
+    b = Batch(15, HQ, HKV, D, dt, 16, lens, news, form="causal" if most == 1 else "tree")
+    sp = b.space()
+    assert sp["counters"].numel() > 0
+    outs = []
+    for _ in range(3):
+        out = torch.full_like(b.q, 9.0)
+        ops.attention_paged(b.cache, 1, b.seqs, b.q, out, **sp)
+        outs.append(out)
+    b.check(outs[0])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert int(sp["counters"].abs().sum()) == 0
+    b.check(b.run(cut=False))
 
 
 @pytest.mark.parametrize("layout", ["heads", "inside"])
@@ -463,6 +490,7 @@ def test_replayed_graph_follows_its_arrays(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, b.run())
+            assert int(sp["counters"].abs().sum()) == 0
 
 
 def test_two_calls_side_by_side(gpu):
