@@ -381,7 +381,7 @@ void CopyPagesLaunch(const kr_cache *cache, const int32_t *src, const int32_t *d
     p.segs = (p.chunks + 256 * kCopyUnroll - 1) / (256 * kCopyUnroll);
     for (int at = 0; at < n; at += kCopyPairs) {
         const int m = std::min(kCopyPairs, n - at);
-        if (int64_t(m) * p.segs >= (int64_t(1) << 31)) Refuse(who, "pages are too large");
+        if (int64_t(m) * p.segs >= kMaxGrid) Refuse(who, "pages are too large");
         std::copy(src + at, src + at + m, p.src);
         std::copy(dst + at, dst + at + m, p.dst);
         std::fill(p.src + m, p.src + kCopyPairs, 0);
@@ -498,7 +498,7 @@ void CompactLaunch(const kr_cache *cache, const kr_seqs *s, const int32_t *path,
     // that a short path keeps its workgroups full
     const int lpr = width <= 8 ? 32 : width <= 16 ? 16 : 8;
     p.slices = (c.heads * p.dch + lpr - 1) / lpr;
-    if (int64_t(p.slices) * s->seqs >= (int64_t(1) << 31)) Refuse(who, "too many sequences");
+    if (int64_t(p.slices) * s->seqs >= kMaxGrid) Refuse(who, "too many sequences");
     const auto go = [&](auto kern, int pl) {
         const dim3 grid(unsigned(p.slices) * unsigned(s->seqs), unsigned((p.planes + pl - 1) / pl));
         hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p);

@@ -36,6 +36,10 @@ __device__ __forceinline__ int PageOf(const PageDiv &d, int n)
     return int(__umulhi(uint32_t(n) * 2u, d.mul) >> d.shift);
 }
 
+// Workgroups of up to 256 threads that a launch may have in x (the runtime
+// counts its threads in 32 bits).
+constexpr int64_t kMaxGrid = int64_t(1) << 23;
+
 // Throws unless the cache handle describes memory that the kernels can walk:
 // known type, head size 64 or 128, 16-byte aligned rows, strides in range.
 // Strides of dimensions of one element are not looked at (and set to 0).

@@ -523,7 +523,7 @@ PagedKernel(PagedParams p)
             const bool future = p.tree == nullptr && key0(st) > sq.len + wtok_hi;
             if (live && there[0] != 0 && !future) {
                 const uint16_t *K = &kring[st % NS][ks][0];
-                uint16_t *V = &vring[st % NS][ks][0];
+                const uint16_t *V = &vring[st % NS][ks][0];
                 f32x16 sacc[KB];
 #pragma unroll
                 for (int kh = 0; kh < KB; ++kh)
@@ -905,10 +905,10 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     r.units = qt * c.heads * s.seqs;
     if (r.units >= (int64_t(1) << 31)) throw std::runtime_error("attention_paged: too many rows for one launch");
     // nothing is cut where the table holds no unit long enough, or the line of
-    // stages (64 keys each) would not fit 32 bits
+    // stages (64 keys each) and a share more would not fit 32 bits
     const int64_t most_stages = (int64_t(s.table_pages) * c.page_size + 63) / 64;
     const int at_least = r.qw == 1 ? CutRule<1>::c : r.qw == 2 ? CutRule<2>::c : CutRule<4>::c;
-    const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 31);
+    const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 30);
     // a ticket, or a note for the second launch, per unit
     r.tickets = cuts && r.units >= kTicketUnits;
     r.part_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
@@ -1005,7 +1005,7 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
         std::min(f.units, int64_t(c.heads) * (int64_t(d.rows) * p.G / (32 * f.qw) + std::min(s.seqs, d.rows)));
     p.max_units = int(units);
     const int64_t wg = std::max<int64_t>(units, p.slots);
-    if (wg >= (int64_t(1) << 31)) refuse("too many rows for one launch");
+    if (wg >= kMaxGrid) refuse("too many rows for one launch");
     void *args[] = {&p};
     Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw), dim3(unsigned(wg)), dim3(unsigned(PagedThreads(f.qw))),
                           args, 0, stream),

@@ -185,6 +185,7 @@ class PagedCache:
         seqs = ops.make_seqs(self._ints([i + [-1] * (width - len(i)) for i in ids], torch.int32).view(-1, width),
                              self._ints([self.tables.tokens(s) for s in news], torch.int32),
                              self._ints(starts, torch.int32), max(news.values(), default=0), tree=tree)
+        seqs.news = dict(news)
         return seqs, self._ints(positions, torch.int64), self._ints(slots, torch.int64)
 
     def commit(self, news):
@@ -194,8 +195,15 @@ class PagedCache:
 
     def accept(self, seqs, paths):
         """Of the drafts of a batch (its handle), paths[seq] are kept, in this
-        order: their rows move up behind the sequence's tokens."""
+        order: their rows move up behind the sequence's tokens. Every sequence
+        of the batch has a path, an empty one where none is kept."""
         import torch
+        self._current()
+        if list(paths) != list(seqs.news):
+            raise ValueError("paths must be of the batch's sequences, in its order")
+        for s, p in paths.items():
+            if len(set(p)) != len(p) or any(not 0 <= i < seqs.news[s] for i in p):
+                raise ValueError("the path of sequence %r must name its drafts, each once" % (s,))
         width = max([1] + [len(p) for p in paths.values()])
         path = self._ints([list(p) + [-1] * (width - len(p)) for p in paths.values()], torch.int32).view(-1, width)
         ops.cache_compact(self.handle, seqs, path, self._ints([len(p) for p in paths.values()], torch.int32))

@@ -670,5 +670,10 @@ def test_drafts_forks_and_steps(gpu):
     tokens({b: 1, c: 20})
     drafts({b: 17, c: 1})
     tokens({c: 1, b: 1})
+    seqs, _, _ = cache.batch({b: 3, c: 2})
+    for bad in ({c: [0], b: [1]}, {b: [1]}, {b: [3], c: []}, {b: [1, 1], c: []}, {b: [-1], c: []}):
+        with pytest.raises(ValueError):
+            cache.accept(seqs, bad)
+    cache.accept(seqs, {b: [], c: []})
     used = sum(-(-cache.tables.tokens(s) // page) for s in (b, c))
     assert cache.tables.free_pages() == 64 - used
