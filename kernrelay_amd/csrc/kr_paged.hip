@@ -251,7 +251,7 @@ PagedKernel(PagedParams p)
     constexpr int VAH = 4;                  // V fragments read ahead
     constexpr int VM = 2 * DPW + 1;         // DMA instructions of a wave's stage
     static_assert((NS - 1) * VM < 64, "vmcnt");
-    static_assert(SB == 64, "the host counts stages of 64 keys");
+    static_assert(SB >= 64, "the host bounds the line by stages of 64 keys");
     constexpr uint64_t ALL = KB == 2 ? ~0ull : 0xffffffffull;
     __shared__ __attribute__((aligned(1024))) uint16_t kring[NS][KW][BLK * D];
     __shared__ __attribute__((aligned(1024))) uint16_t vring[NS][KW][BLK * D];
@@ -302,8 +302,8 @@ PagedKernel(PagedParams p)
     };
     // cut: `slots` workgroups share out the stages evenly, in one line through
     // all units; else a workgroup has one unit
-    const bool cut =
-        p.slots > 0 && float(longest) > CutRule<QW>::a * float(stages) / float(p.slots) + float(CutRule<QW>::c);
+    const bool cut = p.slots > 0 && float(longest) > CutRule<QW>::a * float(stages) / float(p.slots) +
+                                                         float(CutRule<QW>::c * 64 / SB);
     int share = 1, parts = units;
     if (cut) {
         share = Uni(max((stages + p.slots - 1) / p.slots, min(p.min_piece, (stages + units - 1) / units)));
@@ -854,27 +854,22 @@ PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ld
 // Rows a unit holds for this many rows of a sequence and key head.
 int UnitWaves(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
-template <int DT, int D, int QW>
-const void *PagedFn()
+// The kernels: one row block with two key streams, or with four (the whole
+// CU's rings in one workgroup); two with two streams; four with one, 64 keys a
+// stage.
+template <int DT, int D>
+const void *PagedFor(int qw, bool wide)
 {
-    if constexpr (QW == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1, 2>);
-    else if constexpr (QW == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1, 2>);
-    else return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2, 2>);
+    if (qw == 1 && wide) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 4, 1, 2>);
+    if (qw == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1, 2>);
+    if (qw == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1, 2>);
+    return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2, 2>);
 }
 
-int PagedThreads(int qw) { return qw == 1 ? 128 : 256; }
-
-const void *PagedFor(int dtype, int D, int qw)
+const void *PagedFor(int dtype, int D, int qw, bool wide)
 {
-    const auto pick = [&](auto d64, auto d128) { return D == 64 ? d64() : d128(); };
-    if (dtype == kBF16) {
-        if (qw == 1) return pick(PagedFn<kBF16, 64, 1>, PagedFn<kBF16, 128, 1>);
-        if (qw == 2) return pick(PagedFn<kBF16, 64, 2>, PagedFn<kBF16, 128, 2>);
-        return pick(PagedFn<kBF16, 64, 4>, PagedFn<kBF16, 128, 4>);
-    }
-    if (qw == 1) return pick(PagedFn<kF16, 64, 1>, PagedFn<kF16, 128, 1>);
-    if (qw == 2) return pick(PagedFn<kF16, 64, 2>, PagedFn<kF16, 128, 2>);
-    return pick(PagedFn<kF16, 64, 4>, PagedFn<kF16, 128, 4>);
+    if (D == 64) return dtype == kBF16 ? PagedFor<kBF16, 64>(qw, wide) : PagedFor<kF16, 64>(qw, wide);
+    return dtype == kBF16 ? PagedFor<kBF16, 128>(qw, wide) : PagedFor<kF16, 128>(qw, wide);
 }
 
 // Units from which the pieces of a cut one are summed by the last of them
@@ -885,8 +880,17 @@ const void *PagedFor(int dtype, int D, int qw)
 // 13 us against 15).
 constexpr int kTicketUnits = 192;
 
+// Up to that many units of one row block (and from kTicketUnits) a workgroup
+// has its CU to itself for the most part: it takes four key streams. 64
+// sequences of up to 4000 tokens, 4 key heads: 94 us with two, 89 with four; 128
+// units are better cut for two streams (16 sequences of up to 4000, 8 heads: 50
+// us, four streams 61), and more than 256 better off two to a CU (200 of up to
+// 500, 4 heads: 50, four streams 73).
+constexpr int kWideUnits = 256;
+
 struct PagedShape {
     int qw;
+    bool wide;
     int64_t units;  // at most
     bool tickets;
     size_t part_bytes, ws_bytes;
@@ -909,6 +913,7 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     const int64_t most_stages = (int64_t(s.table_pages) * c.page_size + 63) / 64;
     const int at_least = r.qw == 1 ? CutRule<1>::c : r.qw == 2 ? CutRule<2>::c : CutRule<4>::c;
     const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 30);
+    r.wide = r.qw == 1 && r.units >= kTicketUnits && r.units <= kWideUnits;
     // a ticket, or a note for the second launch, per unit
     r.tickets = cuts && r.units >= kTicketUnits;
     r.part_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
@@ -998,7 +1003,7 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
         p.ws = static_cast<float *>(d.ws);
         if (f.tickets) p.cnt = d.cnt;
         else p.joins = reinterpret_cast<PagedJoin *>(static_cast<char *>(d.ws) + f.part_bytes);
-        p.slots = kPagedSlots;
+        p.slots = f.wide ? kPagedSlots / 2 : kPagedSlots;
     }
     // whole units: at most one more row block per sequence than its rows fill
     const int64_t units =
@@ -1007,8 +1012,8 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     const int64_t wg = std::max<int64_t>(units, p.slots);
     if (wg >= kMaxGrid) refuse("too many rows for one launch");
     void *args[] = {&p};
-    Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw), dim3(unsigned(wg)), dim3(unsigned(PagedThreads(f.qw))),
-                          args, 0, stream),
+    const dim3 threads(f.qw == 1 && !f.wide ? 128 : 256);
+    Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw, f.wide), dim3(unsigned(wg)), threads, args, 0, stream),
           "attention_paged launch");
     if (p.joins != nullptr) {
         const bool bf = c.dtype == kBF16;

@@ -336,6 +336,22 @@ def test_attention_uneven_batches(gpu, most, D, HQ, HKV, dt):
     b.check(b.run(cut=False))
 
 
+@pytest.mark.parametrize("D,HQ,HKV,dt", [(128, 28, 4, HF), (64, 14, 2, BF)])
+@pytest.mark.parametrize("longest", [30000, 300])
+def test_attention_one_unit_per_cu(gpu, longest, D, HQ, HKV, dt):
+    """As many units of few rows as the device has CUs, one long sequence among
+    them (cut) or none (whole)."""
+    announce("attention_paged one unit per cu %s" % ((longest, D, HQ, HKV, dt),))
+    rng = random.Random(longest)
+    n = 240 // HKV
+    lens = [rng.randint(0, 300) for _ in range(n)]
+    lens[7] = longest
+    b = Batch(16, HQ, HKV, D, dt, 24, lens, [1] * n)
+    b.check(b.run())
+    assert torch.equal(b.run(), b.run())
+    b.check(b.run(cut=False))
+
+
 @pytest.mark.parametrize("layout", ["heads", "inside"])
 def test_attention_layouts(gpu, layout):
     announce("attention_paged layout " + layout)
