@@ -309,11 +309,12 @@ PagedKernel(PagedParams p)
         share = Uni(max((stages + p.slots - 1) / p.slots, min(p.min_piece, (stages + units - 1) / units)));
         parts = Uni((stages + share - 1) / share);
     }
-    if (int(blockIdx.x) >= parts) {
-        if (p.joins != nullptr && int(blockIdx.x) >= units && int(blockIdx.x) < p.max_units && threadIdx.x == 0)
-            p.joins[blockIdx.x].pieces = 0;  // (the grid has max_units workgroups at least: none stays unwritten)
-        return;
-    }
+    // notes past the units there are, by workgroups with a part of the line or
+    // without: the workspace may hold anything, and the second launch reads
+    // max_units notes (as many workgroups as there are at least)
+    if (p.joins != nullptr && int(blockIdx.x) >= units && int(blockIdx.x) < p.max_units && threadIdx.x == 0)
+        p.joins[blockIdx.x].pieces = 0;
+    if (int(blockIdx.x) >= parts) return;
     const int part = XcdChunk(int(blockIdx.x), 0, parts);
     // this workgroup's stages (cut) or units, and the sequence that holds the
     // first: base <= x < base + its size, after `ubase` units

@@ -352,6 +352,23 @@ def test_attention_one_unit_per_cu(gpu, longest, D, HQ, HKV, dt):
     b.check(b.run(cut=False))
 
 
+@pytest.mark.parametrize("lens,news", [([3000, 10, 5, 0], [40, 20, 0, 7]), ([2000, 0, 30], [1, 0, 1]),
+                                       ([0, 1800, 64, 9], [9, 15, 0, 2])])
+def test_attention_workspace_may_hold_anything(gpu, lens, news):
+    """Fewer units than the handles allow for, on a workspace that reads as notes
+    of cut units (each number 2: all inside the tensors, of a row that belongs
+    to no sequence): they have no part, and that row stays as it was."""
+    announce("attention_paged old workspace %s" % ((lens, news),))
+    b = Batch(17, 8, 2, 128, BF, 16, lens, news, gap=3)
+    sp = b.space()
+    assert sp["ws"].numel() > 0
+    for _ in range(2):
+        sp["ws"].view(torch.int32).fill_(2)
+        out = torch.full_like(b.q, 9.0)
+        ops.attention_paged(b.cache, 1, b.seqs, b.q, out, **sp)
+        b.check(out)
+
+
 @pytest.mark.parametrize("layout", ["heads", "inside"])
 def test_attention_layouts(gpu, layout):
     announce("attention_paged layout " + layout)
