@@ -379,6 +379,15 @@ def _vector(t, dtype, n, who, name):
     raise ValueError("%s: %s must be a contiguous %s vector of %d" % (who, name, dtype, n))
 
 
+def _pitch(t, who, name):
+    """Row stride of a [rows, n] tensor with contiguous rows."""
+    rows, n = t.shape
+    if rows <= 1:
+        return n
+    _need(t.stride(0) >= n, who, "%s: rows overlap" % name)
+    return t.stride(0)
+
+
 def _launch_stream(stream, who, dev, other, *tensors):
     """The stream's handle. Kernels go to the current device's streams: the
     handles' tensors and the call's must be on it."""
@@ -428,16 +437,17 @@ def make_seqs(table, lens, starts, max_new, tree=None):
     for v, size, name in ((lens, n, "lens"), (starts, n + 1, "starts")):
         _need(v.dtype == torch.int32 and v.shape == (size,) and v.is_contiguous(), who,
               "%s must be a contiguous int32 vector of %d" % (name, size))
-    _need(max_new >= 0, who, "max_new must not be negative")
+    _need(0 <= max_new < 1 << 31, who, "max_new must not be negative, nor past 32 bits")
+    ld_table = _pitch(table, who, "table")
     words = ld = 0
     if tree is not None:
         _need(tree.dtype == torch.int64 and tree.dim() == 2 and (tree.shape[1] <= 1 or tree.stride(1) == 1), who,
               "tree must be int64 [rows, words] with contiguous rows")
-        words, ld = tree.shape[1], max(tree.stride(0), tree.shape[1])
+        words, ld = tree.shape[1], _pitch(tree, who, "tree")
         _need(max_new <= 64 * words, who, "the tree has too few words for max_new")
     tensors = [t for t in (table, lens, starts, tree) if t is not None]
     _need(len({t.device for t in tensors}) == 1, who, "the tensors must be on one device")
-    s = KrSeqs(_ptr(table), max(table.stride(0), table.shape[1]), _ptr(lens), _ptr(starts), _ptr(tree), ld,
+    s = KrSeqs(_ptr(table), ld_table, _ptr(lens), _ptr(starts), _ptr(tree), ld,
                table.shape[1], n, max_new, words)
     s.keep, s.device, s.rows = tensors, table.get_device(), None if tree is None else tree.shape[0]
     return s
@@ -558,5 +568,5 @@ def cache_compact(cache, seqs, path, path_lens, stream=None):
           who, "path must be int32 [seqs, width] with contiguous rows")
     lens = _vector(path_lens, i32, n, who, "path_lens")
     width = path.shape[1]
-    _check(_lib().kr_op_cache_compact(cache, seqs, path.data_ptr(), max(path.stride(0), width), width, lens,
+    _check(_lib().kr_op_cache_compact(cache, seqs, path.data_ptr(), _pitch(path, who, "path"), width, lens,
                                       _launch_stream(stream, who, dev, seqs.device, path, path_lens)))

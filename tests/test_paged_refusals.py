@@ -225,3 +225,21 @@ def test_wrappers_check_their_tensors():
         ops.cache_compact(c, s, n.view(1, 4), torch.zeros(3, dtype=torch.int32))
     with pytest.raises(ValueError, match="path_lens"):
         ops.cache_compact(c, s, torch.zeros(3, 4, dtype=torch.int32), n)
+
+
+def test_wrappers_refuse_rows_that_overlap():
+    """A broadcast row has stride 0: read at its width it would lead past the
+    tensor's memory."""
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="overlap"):
+        ops.make_seqs(i32(1, 4).expand(3, 4), i32(3), i32(4), 1)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.make_seqs(i32(3, 4), i32(3), i32(4), 5, tree=i32(1, 2).long().expand(9, 2))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.make_seqs(i32(9).as_strided((3, 4), (2, 1)), i32(3), i32(4), 1)
+    with pytest.raises(ValueError, match="max_new"):  # does not fit the handle
+        ops.make_seqs(i32(3, 4), i32(3), i32(4), (1 << 32) + 1)
+    c, s = cache(), seqs()
+    c.device = s.device = 0
+    with pytest.raises(ValueError, match="overlap"):
+        ops.cache_compact(c, s, i32(1, 4).expand(3, 4), i32(3))
