@@ -153,8 +153,11 @@ class PagedCache:
         self.handle = ops.make_cache(self.k, self.v)
 
     def _current(self):
-        """Before the tables change: the calls that follow must reach the pages."""
+        """Before the tables change: the calls that follow must reach the pages,
+        and now (a captured copy would only run with its graph)."""
         import torch
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("the tables cannot change while a graph is captured")
         if torch.cuda.current_device() != self.handle.device:
             raise ValueError("the cache is on device %d, the current device is %d" % (
                 self.handle.device, torch.cuda.current_device()))
@@ -167,7 +170,9 @@ class PagedCache:
         """The next launch's sequences: news[seq] new tokens of each, in order.
         Reserves their pages (copying shared ones). tree [rows, words] int64:
         ops.make_seqs; depths[seq]: each draft's depth below the sequence's last
-        token (None: 0, 1, 2, ..). Returns (handle, positions, slots)."""
+        token (None: 0, 1, 2, ..). Returns (handle, positions, slots), good until
+        one of the sequences ends, gets tokens or is in another batch, or the
+        pages are defragmented."""
         import torch
         self._current()
         if depths is not None and any(len(depths[s]) != n for s, n in news.items()):
@@ -186,10 +191,13 @@ class PagedCache:
                              self._ints([self.tables.tokens(s) for s in news], torch.int32),
                              self._ints(starts, torch.int32), max(news.values(), default=0), tree=tree)
         seqs.news = dict(news)
+        seqs.held = {s: (self.tables.tokens(s), i) for s, i in zip(news, ids)}
         return seqs, self._ints(positions, torch.int64), self._ints(slots, torch.int64)
 
     def commit(self, news):
         """All new tokens of the last batch are kept."""
+        for s, n in news.items():
+            self.tables.slots(s, n)  # all have room, or none is kept
         for s, n in news.items():
             self.tables.commit(s, n)
 
@@ -201,6 +209,9 @@ class PagedCache:
         self._current()
         if list(paths) != list(seqs.news):
             raise ValueError("paths must be of the batch's sequences, in its order")
+        for s, held in seqs.held.items():
+            if held != (self.tables.tokens(s), self.tables.pages_of(s)):
+                raise ValueError("the batch is out of date: sequence %r has other tokens or pages now" % (s,))
         for s, p in paths.items():
             if len(set(p)) != len(p) or any(not 0 <= i < seqs.news[s] for i in p):
                 raise ValueError("the path of sequence %r must name its drafts, each once" % (s,))

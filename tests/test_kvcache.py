@@ -3,9 +3,12 @@ accident, never lost, and copies are asked for exactly where a shared page
 would be written."""
 
 import random
+from types import SimpleNamespace
 
 import pytest
+import torch
 
+from kernrelay_amd import kvcache
 from kernrelay_amd.kvcache import PageTables
 
 
@@ -120,3 +123,82 @@ def test_refusals():
     t.free(a)
     with pytest.raises(KeyError):
         t.tokens(a)
+
+
+class Calls:
+    """Stands for the GPU calls: what would have been launched."""
+
+    def __init__(self, monkeypatch):
+        self.made = []
+        note = lambda name: lambda *a, **kw: self.made.append(name)  # noqa: E731
+        monkeypatch.setattr(kvcache.ops, "make_cache", lambda k, v: SimpleNamespace(device=0))
+        monkeypatch.setattr(kvcache.ops, "make_seqs", lambda *a, **kw: SimpleNamespace())
+        for name in ("cache_copy_pages", "cache_compact"):
+            monkeypatch.setattr(kvcache.ops, name, note(name))
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+@pytest.mark.parametrize("between", ["defragment", "free", "accept", "batch", "commit"])
+def test_accept_refuses_a_batch_whose_pages_moved(monkeypatch, between):
+    """Its page table is the batch's: rows would move on pages that are not the
+    sequences' any more."""
+    calls = Calls(monkeypatch)
+    cache = kvcache.PagedCache(1, 16, 4, 1, 64, device="cpu")
+    hole, a, b = (cache.tables.add() for _ in range(3))
+    for s in (hole, a, b):
+        cache.batch({s: 5})
+        cache.commit({s: 5})
+    seqs, _, _ = cache.batch({a: 6, b: 2})
+    if between == "defragment":
+        cache.free(hole)
+        cache.defragment()
+    elif between == "free":
+        cache.free(b)
+    elif between == "accept":
+        cache.accept(seqs, {a: [1, 3], b: [0]})
+    elif between == "batch":
+        cache.batch({a: 9})
+    else:
+        cache.commit({a: 1, b: 2})
+    made, held = list(calls.made), {s: cache.tables.tokens(s) for s in (a,)}
+    with pytest.raises((ValueError, KeyError)):
+        cache.accept(seqs, {a: [1, 3], b: [0]})
+    assert calls.made == made and cache.tables.tokens(a) == held[a]
+
+
+def test_accept_after_a_fork(monkeypatch):
+    """A fork in between shares the tokens that were; the drafts stay their own."""
+    Calls(monkeypatch)
+    cache = kvcache.PagedCache(1, 16, 4, 1, 64, device="cpu")
+    a = cache.tables.add()
+    cache.batch({a: 5})
+    cache.commit({a: 5})
+    seqs, _, _ = cache.batch({a: 3})
+    b = cache.fork(a)
+    cache.accept(seqs, {a: [0, 2]})
+    assert (cache.tables.tokens(a), cache.tables.tokens(b)) == (7, 5)
+
+
+def test_commit_is_all_or_nothing(monkeypatch):
+    Calls(monkeypatch)
+    cache = kvcache.PagedCache(1, 16, 4, 1, 64, device="cpu")
+    a, b = cache.tables.add(), cache.tables.add()
+    cache.batch({a: 3, b: 3})
+    with pytest.raises(ValueError, match="no room"):
+        cache.commit({a: 3, b: 30})
+    assert cache.tables.tokens(a) == 0
+
+
+def test_tables_stay_as_they_are_while_a_graph_is_captured(monkeypatch):
+    """The copies that a reservation needs would only run with the graph."""
+    Calls(monkeypatch)
+    cache = kvcache.PagedCache(1, 16, 4, 1, 64, device="cpu")
+    a = cache.tables.add()
+    seqs, _, _ = cache.batch({a: 3})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    free = cache.tables.free_pages()
+    for call in (lambda: cache.batch({a: 9}), lambda: cache.accept(seqs, {a: [1]}), cache.defragment):
+        with pytest.raises(ValueError, match="captured"):
+            call()
+    assert cache.tables.free_pages() == free and cache.tables.tokens(a) == 0
