@@ -333,7 +333,7 @@ int kr_op_qk_norm_rope_cache(const kr_rope *rope, const kr_cache *cache, int lay
                              const int64_t *positions, const int64_t *slots, int rows, int HQ, void *stream);
 
 /* Attention of a launch's new tokens over the pages: out [rows, HQ, D] (rows
- * of no sequence are left alone), query head h reads key head h / (HQ /
+ * of no sequence are left alone; out overlaps neither q nor the cache), query head h reads key head h / (HQ /
  * heads), scores scaled by `scale` (> 0). A row that sees no key gives zeros.
  * What a row does not see has no part in its result, NaN and infinities
  * included. ws / counters: caller-owned device memory of at least the sizes

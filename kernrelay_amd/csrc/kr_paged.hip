@@ -9,7 +9,10 @@
 // What bounds it: every visible key and value is read once, 4 D bytes a
 // position and key head, against 4 D flops for each of the rows that share
 // the head (new tokens x G query heads): HBM up to about a hundred rows, the
-// matrix cores and the softmax's VALU work above.
+// matrix cores and the softmax's VALU work above. Measured (head size 128): 64
+// single tokens over 2000 to 4000, 4 key heads, 394 MB in 87 us; one over
+// 120001, 8 key heads, 492 MB in 100; 2048 tokens of a prompt over 8000, 28 query
+// heads, 265 GFLOP in 296 (0.9 PFLOP/s).
 //
 // A unit of work is one key head of one sequence and RT = 32 QW packed rows
 // (row r = new token r / G, query head r % G of the key head's G), so the

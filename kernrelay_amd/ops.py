@@ -527,7 +527,8 @@ def attention_paged_workspace(cache, seqs, HQ):
 
 def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
     """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
-    cache; their own keys and values are in the cache already. ws (uint8) and
+    cache; their own keys and values are in the cache already, and out is none
+    of the inputs' memory. ws (uint8) and
     counters (int32, zero before the first call): of attention_paged_workspace's
     sizes, for one stream at a time; None: no sequence is cut into pieces."""
     who = "attention_paged"

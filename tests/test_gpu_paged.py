@@ -85,7 +85,7 @@ def test_qk_norm_rope(gpu, rows, HQ, HKV, D, dt, tdt, norm):
     check_rope(k2, k, gains[1], c[:rows], s[:rows], 1e-5)
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("dt", [BF, HF])
 def test_chain_has_the_separate_calls_bits(gpu, D, dt):
     announce("qk_norm_rope chain %d %s" % (D, dt))
@@ -473,6 +473,24 @@ def test_device_arrays_that_lead_outside(gpu):
     out = b.run()
     b.dev[1].copy_(ints([0, 40]))
     assert torch.equal(out[:4], b.run()[:4]) and bool(out[:4].isfinite().all())
+
+
+@pytest.mark.parametrize("news,most", [([3, 2], 1), ([40, 20], 17)])
+def test_new_tokens_past_max_new_are_not_worked(gpu, news, most):
+    """The first max_new tokens of a sequence are as in a launch of theirs, and
+    the rows behind them as they were."""
+    announce("attention_paged past max_new %s %d" % (news, most))
+    b = Batch(18, 8, 2, 128, HF, 16, [100, 30], news)
+    seqs, out = ops.make_seqs(*b.dev, most), torch.full_like(b.q, 9.0)
+    ops.attention_paged(b.cache, 1, seqs, b.q, out)
+    for s, n in enumerate(news):
+        lo, n = b.starts[s], min(n, most)
+        assert torch.all(out[lo + n:b.starts[s + 1]] == 9.0)
+        alone = torch.full_like(b.q, 9.0)
+        starts = ints([lo if i <= s else lo + n for i in range(3)])
+        ops.attention_paged(b.cache, 1, ops.make_seqs(b.dev[0], b.dev[1], starts, most), b.q, alone)
+        assert torch.equal(out[lo:lo + n], alone[lo:lo + n])
+        assert torch.all(alone[:lo] == 9.0) and torch.all(alone[lo + n:] == 9.0)
 
 
 def test_far_pages(gpu):
