@@ -29,7 +29,9 @@
 // row instead and seen by nobody.
 // The products are those of the prompt's kernel (kr_attn.hip): S^T = K Q^T,
 // softmax in base 2 with a lazily moved maximum, O^T += V^T P^T, fp32 state;
-// P is rounded to 16 bits for the matrix cores, its sum is of the unrounded.
+// P is rounded to 16 bits for the matrix cores, which moves a result by at most
+// half a step of sum p |v|, about what rounding the result does; its sum is of
+// the unrounded. fp16 weights carry a factor 2^7 through the sums.
 // A block in which some row does not see some key goes the careful way: the
 // scores are masked by 64 bits a row; value rows that are not there or hold a
 // number that is not finite are zeroed in LDS (0 x NaN would reach everybody),
@@ -591,6 +593,12 @@ PagedKernel(PagedParams p)
                 const float mnew = move ? mloc : m;
                 const float msub = mnew == -INFINITY ? 0.0f : mnew;
                 const float alpha = move ? __builtin_amdgcn_exp2f(m - msub) : 1.0f;
+                // fp16 holds its full precision down to 2^-14 only, and below
+                // 2^-25 nothing: many small weights beside one of 1 would be
+                // lost. So P is 2^7 2^(s - m): at most 2^15 with the lazy
+                // maximum's 2^8, and full down to 2^-21; O and l both have the
+                // factor, in every stream and piece, and lose it in O / l
+                const float sub = DT == kF16 ? 7.0f - msub : -msub;
                 uint4 pf[2 * KB];
                 float ls[4];
 #pragma unroll
@@ -599,7 +607,7 @@ PagedKernel(PagedParams p)
                     float pv[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kh][vb + e], p.scale_log2, -msub));
+                        pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kh][vb + e], p.scale_log2, sub));
                         ls[e & 3] = c == 0 && e < 4 ? pv[e] : ls[e & 3] + pv[e];
                     }
                     pf[c] = make_uint4(Pack2<DT>(pv[0], pv[1]), Pack2<DT>(pv[2], pv[3]), Pack2<DT>(pv[4], pv[5]),
