@@ -9,6 +9,7 @@ takes pages as its tokens come and gives them back when it ends.
 """
 
 import heapq
+import warnings
 
 from . import ops
 
@@ -170,11 +171,13 @@ class PagedCache:
         """The next launch's sequences: news[seq] new tokens of each, in order.
         Reserves their pages (copying shared ones). tree [rows, words] int64:
         ops.make_seqs; depths[seq]: each draft's depth below the sequence's last
-        token (None: 0, 1, 2, ..). Returns (handle, positions, slots), good until
-        one of the sequences ends, gets tokens or is in another batch, or the
-        pages are defragmented."""
+        token (needed with a tree; None: 0, 1, 2, ..). Returns (handle,
+        positions, slots), good until one of the sequences ends, gets tokens or
+        is in another batch, or the pages are defragmented."""
         import torch
         self._current()
+        if tree is not None and depths is None:
+            raise ValueError("a tree needs the depths of its drafts")
         if depths is not None and any(len(depths[s]) != n for s, n in news.items()):
             raise ValueError("depths must give one depth for each new token")
         src, dst = self.tables.reserve(news)
@@ -191,6 +194,7 @@ class PagedCache:
                              self._ints([self.tables.tokens(s) for s in news], torch.int32),
                              self._ints(starts, torch.int32), max(news.values(), default=0), tree=tree)
         seqs.news = dict(news)
+        seqs.depths = None if depths is None else {s: tuple(depths[s]) for s in news}
         seqs.held = {s: (self.tables.tokens(s), i) for s, i in zip(news, ids)}
         return seqs, self._ints(positions, torch.int64), self._ints(slots, torch.int64)
 
@@ -204,7 +208,10 @@ class PagedCache:
     def accept(self, seqs, paths):
         """Of the drafts of a batch (its handle), paths[seq] are kept, in this
         order: their rows move up behind the sequence's tokens. Every sequence
-        of the batch has a path, an empty one where none is kept."""
+        of the batch has a path, an empty one where none is kept. Keys stay
+        rotated for the positions that batch returned, so the draft kept i-th
+        must be one of depth i; a batch without depths cannot tell whether
+        others' positions were used, and warns where its own would be wrong."""
         import torch
         self._current()
         if list(paths) != list(seqs.news):
@@ -215,6 +222,12 @@ class PagedCache:
         for s, p in paths.items():
             if len(set(p)) != len(p) or any(not 0 <= i < seqs.news[s] for i in p):
                 raise ValueError("the path of sequence %r must name its drafts, each once" % (s,))
+            if seqs.depths is not None and any(seqs.depths[s][d] != i for i, d in enumerate(p)):
+                raise ValueError("the path of sequence %r must go down draft by draft, from depth 0" % (s,))
+        for s, p in paths.items():
+            if seqs.depths is None and list(p) != list(range(len(p))):
+                warnings.warn("the path of sequence %r skips drafts of a chain: keys written at the batch's positions "
+                              "keep those of their old places" % (s,), RuntimeWarning, stacklevel=2)
         width = max([1] + [len(p) for p in paths.values()])
         path = self._ints([list(p) + [-1] * (width - len(p)) for p in paths.values()], torch.int32).view(-1, width)
         ops.cache_compact(self.handle, seqs, path, self._ints([len(p) for p in paths.values()], torch.int32))
