@@ -528,9 +528,10 @@ def attention_paged_workspace(cache, seqs, HQ):
 def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
     """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
     cache; their own keys and values are in the cache already, and out is none
-    of the inputs' memory. ws (uint8) and
-    counters (int32, zero before the first call): of attention_paged_workspace's
-    sizes, for one stream at a time; None: no sequence is cut into pieces."""
+    of the inputs' memory. ws (uint8) and counters (int32, zero before the
+    first call): of attention_paged_workspace's sizes for these handles at
+    least (a wider table or more sequences may need more), for one stream at a
+    time; None: no sequence is cut into pieces."""
     who = "attention_paged"
     _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
     shape, dt, dev = q.shape, cache.torch_dtype, cache.device
@@ -542,7 +543,9 @@ def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=No
     if ws is not None:
         _need(counters is not None and counters.dtype == _ints()[0] and counters.dim() == 1 and counters.is_contiguous()
               and ws.is_contiguous(), who, "ws and counters (an int32 vector) must be contiguous")
-        wp, cp, nbytes, ncnt = ws.data_ptr(), counters.data_ptr(), ws.nbytes, counters.shape[0]
+        # (an empty tensor's address is 0, which would say that there is none; at
+        # 0 bytes no address is used, and too few are refused)
+        wp, cp, nbytes, ncnt = ws.data_ptr() or 16, counters.data_ptr(), ws.nbytes, counters.shape[0]
     _check(_lib().kr_op_attention_paged(cache, layer, seqs, qp, ldq, op, ldo, shape[0], shape[1],
                                         cache.head_dim ** -0.5 if scale is None else scale, wp, nbytes, cp, ncnt,
                                         _launch_stream(stream, who, dev, seqs.device, q, out, ws, counters)))

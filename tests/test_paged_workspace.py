@@ -1,0 +1,46 @@
+"""Workspaces of attention_paged that a batch has outgrown are refused before
+anything reaches a GPU, empty ones too."""
+
+import pytest
+import torch
+
+from kernrelay_amd import ops
+from tests.test_paged_refusals import cache, seqs
+
+
+def handles(table_pages, n):
+    c = cache()
+    s = seqs(seqs=n, max_new=1, table_pages=table_pages, ld_table=table_pages)
+    c.torch_dtype, c.device, s.device, s.rows = torch.bfloat16, 0, 0, None
+    return c, s
+
+
+def space(nbytes, ncnt):
+    return dict(ws=torch.empty(nbytes, dtype=torch.uint8), counters=torch.zeros(ncnt, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("first,then,n", [(2, 4000, 1), (2, 4000, 64), (30, 4000, 64), (4000, 4000, 64)])
+def test_a_sequence_that_grows_on_its_first_workspace(monkeypatch, first, then, n):
+    monkeypatch.setattr(ops, "_launch_stream", lambda *a: None)
+    q = torch.zeros(n, 8, 128, dtype=torch.bfloat16)
+    one = handles(first, 1)
+    need = ops.attention_paged_workspace(*one, 8)
+    c, s = handles(then, n)
+    assert (need == (0, 0)) == (first == 2)
+    more = ops.attention_paged_workspace(c, s, 8)
+    assert more[0] > need[0] or more[1] > need[1]
+    with pytest.raises(RuntimeError, match="workspace is too small"):
+        ops.attention_paged(c, 0, s, q, torch.empty_like(q), **space(*need))
+    if more[1]:  # enough memory, no counters
+        with pytest.raises(RuntimeError, match="workspace is too small"):
+            ops.attention_paged(c, 0, s, q, torch.empty_like(q), **space(more[0], 0))
+
+
+def test_workspaces_grow_with_the_batch():
+    """What a larger batch of the same rows needs is enough for a smaller one."""
+    for n in (1, 3, 40, 200):
+        last = 0
+        for pages in (1, 5, 40, 1000, 8000):
+            nbytes, _ = ops.attention_paged_workspace(*handles(pages, n), 8)
+            assert nbytes >= last
+            last = nbytes
