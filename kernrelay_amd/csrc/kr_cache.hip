@@ -46,7 +46,8 @@ kr_cache CheckCache(const kr_cache *c, const char *who)
 
 void CheckSeqs(const kr_seqs *s, const char *who)
 {
-    if (s == nullptr || s->table == nullptr || s->lens == nullptr || s->starts == nullptr)
+    // (arrays of no sequence may have no address)
+    if (s == nullptr || (s->seqs > 0 && (s->table == nullptr || s->lens == nullptr || s->starts == nullptr)))
         Refuse(who, "needs a page table, lengths and starts");
     if (s->seqs < 0 || s->max_new < 0 || s->table_pages < 1) Refuse(who, "a negative or empty size");
     if (s->seqs > 1 && s->ld_table < s->table_pages) Refuse(who, "page table rows overlap");

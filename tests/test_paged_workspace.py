@@ -44,3 +44,13 @@ def test_workspaces_grow_with_the_batch():
             nbytes, _ = ops.attention_paged_workspace(*handles(pages, n), 8)
             assert nbytes >= last
             last = nbytes
+
+
+def test_no_sequences():
+    """Arrays of no sequence have no address in torch."""
+    c, none = cache(), seqs(seqs=0, table=None, lens=None, starts=None)
+    assert ops.attention_paged_workspace(c, none, 8) == (0, 0)
+    L, A = ops._lib(), 1 << 20
+    assert L.kr_op_attention_paged(c, 0, none, A, 0, A, 0, 4, 8, 0.1, None, 0, None, 0, None) == 0
+    assert L.kr_op_attention_paged(c, 0, none, None, 0, None, 0, 0, 8, 0.1, None, 0, None, 0, None) == 0
+    assert L.kr_op_cache_compact(c, none, None, 1, 1, None, None) == 0
