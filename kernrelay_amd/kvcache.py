@@ -176,19 +176,24 @@ class PagedCache:
         is in another batch, or the pages are defragmented."""
         import torch
         self._current()
-        if tree is not None and depths is None:
-            raise ValueError("a tree needs the depths of its drafts")
+        if tree is not None:
+            if depths is None:
+                raise ValueError("a tree needs the depths of its drafts")
+            ops.check_tree(tree, max(news.values(), default=0), "batch")
+            if tree.shape[0] < sum(news.values()) or tree.device != self.k.device:
+                raise ValueError("the tree must have a row for each new token, on the cache's device")
         if depths is not None and any(len(depths[s]) != n for s, n in news.items()):
             raise ValueError("depths must give one depth for each new token")
+        # (all that can be refused is, before the tables change)
+        positions = self._ints([self.tables.tokens(s) + (i if depths is None else depths[s][i])
+                                for s, n in news.items() for i in range(n)], torch.int64)
         src, dst = self.tables.reserve(news)
         ops.cache_copy_pages(self.handle, src, dst)
         ids = [self.tables.pages_of(s) for s in news]
         width = max([1] + [len(i) for i in ids])
-        starts, positions, slots = [0], [], []
+        starts, slots = [0], []
         for s, n in news.items():
-            at = self.tables.tokens(s)
             starts.append(starts[-1] + n)
-            positions += [at + (i if depths is None else depths[s][i]) for i in range(n)]
             slots += self.tables.slots(s, n)
         seqs = ops.make_seqs(self._ints([i + [-1] * (width - len(i)) for i in ids], torch.int32).view(-1, width),
                              self._ints([self.tables.tokens(s) for s in news], torch.int32),
@@ -196,7 +201,7 @@ class PagedCache:
         seqs.news = dict(news)
         seqs.depths = None if depths is None else {s: tuple(depths[s]) for s in news}
         seqs.held = {s: (self.tables.tokens(s), i) for s, i in zip(news, ids)}
-        return seqs, self._ints(positions, torch.int64), self._ints(slots, torch.int64)
+        return seqs, positions, self._ints(slots, torch.int64)
 
     def commit(self, news):
         """All new tokens of the last batch are kept."""

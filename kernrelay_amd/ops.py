@@ -422,6 +422,15 @@ def make_cache(k, v):
     return c
 
 
+def check_tree(tree, max_new, who):
+    """Words and row stride of make_seqs' tree; refuses one that is none."""
+    _need(tree.dtype == _ints()[1] and tree.dim() == 2 and (tree.shape[1] <= 1 or tree.stride(1) == 1), who,
+          "tree must be int64 [rows, words] with contiguous rows")
+    words, ld = tree.shape[1], _pitch(tree, who, "tree")
+    _need(max_new <= 64 * words, who, "the tree has too few words for max_new")
+    return words, ld
+
+
 def make_seqs(table, lens, starts, max_new, tree=None):
     """Handle of a launch's sequences: table [seqs, pages] and lens [seqs]
     int32, starts [seqs + 1] int32 (rows starts[b] .. starts[b + 1] - 1 are
@@ -439,12 +448,7 @@ def make_seqs(table, lens, starts, max_new, tree=None):
               "%s must be a contiguous int32 vector of %d" % (name, size))
     _need(0 <= max_new < 1 << 31, who, "max_new must not be negative, nor past 32 bits")
     ld_table = _pitch(table, who, "table")
-    words = ld = 0
-    if tree is not None:
-        _need(tree.dtype == torch.int64 and tree.dim() == 2 and (tree.shape[1] <= 1 or tree.stride(1) == 1), who,
-              "tree must be int64 [rows, words] with contiguous rows")
-        words, ld = tree.shape[1], _pitch(tree, who, "tree")
-        _need(max_new <= 64 * words, who, "the tree has too few words for max_new")
+    words, ld = (0, 0) if tree is None else check_tree(tree, max_new, who)
     tensors = [t for t in (table, lens, starts, tree) if t is not None]
     _need(len({t.device for t in tensors}) == 1, who, "the tensors must be on one device")
     s = KrSeqs(_ptr(table), ld_table, _ptr(lens), _ptr(starts), _ptr(tree), ld,

@@ -1,5 +1,6 @@
 """Accepted paths of PagedCache against the positions that their drafts' keys
-were rotated for (no GPU: the launches are stood in for)."""
+were rotated for, and batches that are refused (no GPU: the launches are stood
+in for)."""
 
 import warnings
 
@@ -62,3 +63,24 @@ def test_a_chain_that_is_not_kept_from_its_start_warns(cache):
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         cache.accept(seqs, {cache.seq: [0, 1, 2]})
+
+
+@pytest.mark.parametrize("tree,depths,error", [
+    (TREE.int(), DEPTHS, ValueError), (TREE[:, 0], DEPTHS, ValueError), (TREE[:4], DEPTHS, ValueError),
+    (torch.zeros(9, 0, dtype=torch.int64), DEPTHS, ValueError),
+    (torch.zeros(1, 1, dtype=torch.int64).expand(5, 1), DEPTHS, ValueError),
+    (torch.zeros(5, 1, dtype=torch.int64, device="meta"), DEPTHS, ValueError),
+    (TREE, DEPTHS[:4], ValueError), (TREE, ["a"] * 5, TypeError), (TREE, [None] * 5, TypeError)])
+def test_a_refused_batch_changes_nothing(cache, tree, depths, error):
+    """Not the tables, nor the pages that a fork shares."""
+    twin = cache.fork(cache.seq)
+    held = cache.tables.free_pages(), cache.tables.pages_of(cache.seq), list(cache.calls.made)
+    with pytest.raises(error):
+        cache.batch({cache.seq: 5}, tree=tree, depths={cache.seq: depths})
+    with pytest.raises(KeyError):
+        cache.batch({cache.seq: 5, twin + 9: 1})
+    with pytest.raises(ValueError):
+        cache.batch({cache.seq: 5, twin: -1})
+    assert (cache.tables.free_pages(), cache.tables.pages_of(cache.seq), cache.calls.made) == held
+    cache.batch({cache.seq: 5}, tree=TREE, depths={cache.seq: DEPTHS})
+    assert len(cache.calls.made) == len(held[2]) + 1 and cache.tables.pages_of(cache.seq) != held[1]
