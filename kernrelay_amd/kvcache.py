@@ -152,6 +152,11 @@ class PagedCache:
         shape = (layers, pages, page_size, heads, head_dim)
         self.k, self.v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         self.handle = ops.make_cache(self.k, self.v)
+        self._batches, self._last = 0, {}  # how many there were; the last one with new tokens of a sequence
+
+    def _state(self, seq):
+        """What a batch's rows of a sequence depend on."""
+        return self._last.get(seq), self.tables.tokens(seq), self.tables.pages_of(seq)
 
     def _current(self):
         """Before the tables change: the calls that follow must reach the pages,
@@ -173,7 +178,7 @@ class PagedCache:
         ops.make_seqs; depths[seq]: each draft's depth below the sequence's last
         token (needed with a tree; None: 0, 1, 2, ..). Returns (handle,
         positions, slots), good until one of the sequences ends, gets tokens or
-        is in another batch, or the pages are defragmented."""
+        is in another batch with new tokens, or the pages are defragmented."""
         import torch
         self._current()
         if tree is not None:
@@ -200,7 +205,9 @@ class PagedCache:
                              self._ints(starts, torch.int32), max(news.values(), default=0), tree=tree)
         seqs.news = dict(news)
         seqs.depths = None if depths is None else {s: tuple(depths[s]) for s in news}
-        seqs.held = {s: (self.tables.tokens(s), i) for s, i in zip(news, ids)}
+        self._batches += 1
+        self._last.update((s, self._batches) for s, n in news.items() if n > 0)
+        seqs.held = {s: self._state(s) for s in news}
         return seqs, positions, self._ints(slots, torch.int64)
 
     def commit(self, news):
@@ -222,8 +229,8 @@ class PagedCache:
         if list(paths) != list(seqs.news):
             raise ValueError("paths must be of the batch's sequences, in its order")
         for s, held in seqs.held.items():
-            if held != (self.tables.tokens(s), self.tables.pages_of(s)):
-                raise ValueError("the batch is out of date: sequence %r has other tokens or pages now" % (s,))
+            if held != self._state(s):
+                raise ValueError("the batch is out of date: sequence %r has other tokens, drafts or pages now" % (s,))
         for s, p in paths.items():
             if len(set(p)) != len(p) or any(not 0 <= i < seqs.news[s] for i in p):
                 raise ValueError("the path of sequence %r must name its drafts, each once" % (s,))
@@ -243,6 +250,7 @@ class PagedCache:
 
     def free(self, seq):
         self.tables.free(seq)
+        self._last.pop(seq, None)
 
     def defragment(self):
         self._current()

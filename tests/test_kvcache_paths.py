@@ -84,3 +84,20 @@ def test_a_refused_batch_changes_nothing(cache, tree, depths, error):
     assert (cache.tables.free_pages(), cache.tables.pages_of(cache.seq), cache.calls.made) == held
     cache.batch({cache.seq: 5}, tree=TREE, depths={cache.seq: DEPTHS})
     assert len(cache.calls.made) == len(held[2]) + 1 and cache.tables.pages_of(cache.seq) != held[1]
+
+
+def test_drafts_that_a_later_batch_wrote_over(cache):
+    """Two batches on the same page: the rows are the second's."""
+    first, _, _ = cache.batch({cache.seq: 2}, tree=TREE, depths={cache.seq: [0, 1]})
+    second, _, slots = cache.batch({cache.seq: 2}, tree=TREE, depths={cache.seq: [0, 0]})
+    made = list(cache.calls.made)
+    with pytest.raises(ValueError, match="out of date"):
+        cache.accept(first, {cache.seq: [0, 1]})
+    assert cache.calls.made == made and cache.tables.tokens(cache.seq) == 5
+    other = cache.tables.add()
+    cache.batch({other: 3, cache.seq: 0})  # no new tokens of the sequence
+    cache.accept(second, {cache.seq: [1]})
+    assert cache.tables.tokens(cache.seq) == 6
+    cache.free(cache.seq)
+    with pytest.raises(KeyError):
+        cache.accept(second, {cache.seq: []})
