@@ -318,22 +318,25 @@ typedef struct kr_rope {
 /* Per-head RMSNorm (with gammas) and rotate-half RoPE of q [rows, HQ, D] and
  * k [rows, HKV, D] in one pass (D 64, 128 or 256; ld* = row strides, 0 =
  * packed). Row r stands at positions[r] (NULL: r); a position outside the
- * tables gives zero rows. An output may be its own input. Same role as
- * kr_op_rowop's rmsnorm and kr_op_rope in sequence (reference EmitQkNorm,
- * exec/qwen_main.cpp:1346-1357, and Rope, :567-582). */
+ * tables gives zero rows. An output may be its own input (the same rows);
+ * one that overlaps an input or the other output otherwise is refused. Same
+ * role as kr_op_rowop's rmsnorm and kr_op_rope in sequence (reference
+ * EmitQkNorm, exec/qwen_main.cpp:1346-1357, and Rope, :567-582). */
 int kr_op_qk_norm_rope(int dtype, const kr_rope *rope, const void *q, int64_t ldq, const void *k, int64_t ldk,
                        void *q_out, int64_t ldqo, void *k_out, int64_t ldko, const int64_t *positions, int rows,
                        int HQ, int HKV, void *stream);
 
 /* The same with k and v [rows, heads, D] written to their cache slots
  * (slots[r] = page * page_size + row in the page; outside the cache, -1 say:
- * not written). No two rows may share a slot: it would hold a mixture. */
+ * not written). No two rows may share a slot: it would hold a mixture. q_out
+ * overlaps neither k, v nor the layer (refused), and q only as its own input. */
 int kr_op_qk_norm_rope_cache(const kr_rope *rope, const kr_cache *cache, int layer, const void *q, int64_t ldq,
                              const void *k, int64_t ldk, const void *v, int64_t ldv, void *q_out, int64_t ldqo,
                              const int64_t *positions, const int64_t *slots, int rows, int HQ, void *stream);
 
 /* Attention of a launch's new tokens over the pages: out [rows, HQ, D] (rows
- * of no sequence are left alone; out overlaps neither q nor the cache), query head h reads key head h / (HQ /
+ * of no sequence are left alone; refused where out overlaps q or the layer, the
+ * gaps between its rows included), query head h reads key head h / (HQ /
  * heads), scores scaled by `scale` (> 0). A row that sees no key gives zeros.
  * What a row does not see has no part in its result, NaN and infinities
  * included. ws / counters: caller-owned device memory of at least the sizes

@@ -22,6 +22,38 @@ bool Misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) !=
 
 }  // namespace
 
+bool Overlap(const RowSpan &a, const RowSpan &b)
+{
+    if (a.rows < 1 || b.rows < 1) return false;
+    const int64_t pa = int64_t(reinterpret_cast<uintptr_t>(a.p) / 2), pb = int64_t(reinterpret_cast<uintptr_t>(b.p) / 2);
+    if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return false;
+    if (a.ld == b.ld && a.ld > 0) {
+        // row i of a and i + t of b: -b.width < d + t ld < a.width
+        const int64_t d = pb - pa, ld = a.ld;
+        const auto floor_div = [](int64_t n, int64_t by) { return n / by - (n % by < 0); };
+        const int64_t lo = std::max(-floor_div(d + b.width - 1, ld), 1 - a.rows);
+        const int64_t hi = std::min(floor_div(a.width - 1 - d, ld), b.rows - 1);
+        return lo <= hi;
+    }
+    for (int64_t i = 0, j = 0; i < a.rows && j < b.rows;) {
+        const int64_t x = pa + i * a.ld, y = pb + j * b.ld;
+        if (x + a.width <= y) ++i;
+        else if (y + b.width <= x) ++j;
+        else return true;
+    }
+    return false;
+}
+
+RowSpan LayerSpan(const kr_cache &c, const void *base, int layer)
+{
+    RowSpan s;
+    s.p = static_cast<const uint16_t *>(base) + layer * c.layer_stride;
+    s.rows = 1;
+    s.width = (c.pages - 1) * c.page_stride + (c.page_size - 1) * c.token_stride + (c.heads - 1) * c.head_stride +
+              c.head_dim;
+    return s;
+}
+
 kr_cache CheckCache(const kr_cache *c, const char *who)
 {
     if (c == nullptr || c->k == nullptr || c->v == nullptr) Refuse(who, "needs a cache");
@@ -272,6 +304,19 @@ void QkRopeLaunch(const QkRopeDesc &d, hipStream_t stream)
     if (((p.ldq | p.ldk | p.ldv | p.ldqo | p.ldko) % 8) != 0) Refuse(who, "row strides must be multiples of 8");
     const int64_t total = int64_t(d.rows) * p.heads;
     if (total * (d.D / 16) > (int64_t(1) << 31) - 256) Refuse(who, "too many rows for one launch");
+    // an output is its own input or no input at all
+    const RowSpan q{d.q, p.ldq, d.rows, int64_t(d.HQ) * d.D}, k{d.k, p.ldk, d.rows, int64_t(d.HKV) * d.D};
+    const RowSpan qo{d.q_out, p.ldqo, d.rows, q.width}, ko{d.k_out, p.ldko, d.rows, k.width};
+    const auto same = [&](const RowSpan &a, const RowSpan &b) { return a.p == b.p && (d.rows == 1 || a.ld == b.ld); };
+    if ((Overlap(qo, q) && !same(qo, q)) || Overlap(qo, k)) Refuse(who, "q_out overlaps an input");
+    if (d.cache != nullptr) {
+        if (Overlap(qo, RowSpan{d.v, p.ldv, d.rows, k.width})) Refuse(who, "q_out overlaps an input");
+        const kr_cache c = CheckCache(d.cache, who);
+        if (Overlap(qo, LayerSpan(c, c.k, d.layer)) || Overlap(qo, LayerSpan(c, c.v, d.layer)))
+            Refuse(who, "q_out overlaps the cache");
+    } else if ((Overlap(ko, k) && !same(ko, k)) || Overlap(ko, q) || Overlap(ko, qo)) {
+        Refuse(who, "k_out overlaps an input or q_out");
+    }
     p.total = int(total);
     const bool t32 = d.rope.table_dtype == kF32, chain = d.rope.chain != 0, bf = d.dtype == kBF16;
     const auto go = [&](auto bf16, auto f16) { bf ? bf16(p, t32, chain, stream) : f16(p, t32, chain, stream); };

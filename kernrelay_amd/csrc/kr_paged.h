@@ -40,6 +40,19 @@ __device__ __forceinline__ int PageOf(const PageDiv &d, int n)
 // counts its threads in 32 bits).
 constexpr int64_t kMaxGrid = int64_t(1) << 23;
 
+// Rows of 16-bit values: `width` of them every `ld` elements.
+struct RowSpan {
+    const void *p = nullptr;
+    int64_t ld = 0, rows = 0, width = 0;
+};
+
+// Do two of them share memory (rows lying between the other's, the columns of
+// one projection, do not)?
+bool Overlap(const RowSpan &a, const RowSpan &b);
+
+// Keys (or values) of a layer, the gaps between its rows included.
+RowSpan LayerSpan(const kr_cache &c, const void *base, int layer);
+
 // Throws unless the cache handle describes memory that the kernels can walk:
 // known type, head size 64 or 128, 16-byte aligned rows, strides in range.
 // Strides of dimensions of one element are not looked at (and set to 0).

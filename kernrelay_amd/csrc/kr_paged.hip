@@ -1023,6 +1023,11 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     p.max_units = int(units);
     const int64_t wg = std::max<int64_t>(units, p.slots);
     if (wg >= kMaxGrid) refuse("too many rows for one launch");
+    const int64_t width = int64_t(d.HQ) * c.head_dim;
+    const RowSpan out{d.out, p.ldo, d.rows, width};
+    if (Overlap(out, RowSpan{d.q, p.ldq, d.rows, width})) refuse("out overlaps q");
+    if (Overlap(out, LayerSpan(c, c.k, d.layer)) || Overlap(out, LayerSpan(c, c.v, d.layer)))
+        refuse("out overlaps the cache");
     void *args[] = {&p};
     const dim3 threads(f.qw == 1 && !f.wide ? 128 : 256);
     Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw, f.wide), dim3(unsigned(wg)), threads, args, 0, stream),

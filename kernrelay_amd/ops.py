@@ -482,7 +482,7 @@ def qk_norm_rope(rope, q, k, q_out, k_out, positions=None, stream=None):
     """q_out, k_out = per-head RMSNorm (if the handle has gains) and rotation
     of q [rows, HQ, D] and k [rows, HKV, D] in one pass. Row r stands at
     positions[r] (int64; None: r); outside the tables: zeros. Outputs may be
-    the inputs themselves."""
+    the inputs themselves; other overlaps are refused."""
     who = "qk_norm_rope"
     _need(q.dim() == 3 and k.dim() == 3, who, "q and k are [rows, heads, head_dim]")
     qs, ks, dt, dev = q.shape, k.shape, q.dtype, rope.device
@@ -531,8 +531,8 @@ def attention_paged_workspace(cache, seqs, HQ):
 
 def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
     """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
-    cache; their own keys and values are in the cache already, and out is none
-    of the inputs' memory. ws (uint8) and counters (int32, zero before the
+    cache; their own keys and values are in the cache already, and out
+    overlaps neither q nor the layer. ws (uint8) and counters (int32, zero before the
     first call): of attention_paged_workspace's sizes for these handles at
     least (a wider table or more sequences may need more), for one stream at a
     time; None: no sequence is cut into pieces."""
