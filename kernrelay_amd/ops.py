@@ -401,6 +401,9 @@ def _launch_stream(stream, who, dev, other, *tensors):
     if dev != other or _RAW[0]() != dev:
         raise ValueError("%s: the handles' tensors are on devices %d and %d, the current device is %d" % (
             who, dev, other, _RAW[0]()))
+    if stream is not None and getattr(stream, "device_index", dev) != dev:
+        raise ValueError("%s: the stream is on device %d, the handles' tensors are on device %d" % (
+            who, stream.device_index, dev))
     return _stream(stream)
 
 

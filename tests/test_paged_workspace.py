@@ -1,5 +1,7 @@
 """Workspaces of attention_paged that a batch has outgrown are refused before
-anything reaches a GPU, empty ones too."""
+anything reaches a GPU, empty ones too; so are streams of another device."""
+
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -54,3 +56,16 @@ def test_no_sequences():
     assert L.kr_op_attention_paged(c, 0, none, A, 0, A, 0, 4, 8, 0.1, None, 0, None, 0, None) == 0
     assert L.kr_op_attention_paged(c, 0, none, None, 0, None, 0, 0, 8, 0.1, None, 0, None, 0, None) == 0
     assert L.kr_op_cache_compact(c, none, None, 1, 1, None, None) == 0
+
+
+def test_streams_of_another_device(monkeypatch):
+    """A launch there would reach for memory that its device may not have."""
+    monkeypatch.setattr(ops, "_RAW", (lambda: 0, lambda dev: 77))
+    on = lambda **kw: SimpleNamespace(cuda_stream=5, **kw)  # noqa: E731
+    with pytest.raises(ValueError, match="stream is on device 1"):
+        ops._launch_stream(on(device_index=1), "cache_copy_pages", 0, 0)
+    with pytest.raises(ValueError, match="current device is 0"):
+        ops._launch_stream(on(device_index=1), "cache_copy_pages", 1, 1)
+    assert ops._launch_stream(on(device_index=0), "cache_copy_pages", 0, 0) == 5
+    assert ops._launch_stream(on(), "cache_copy_pages", 0, 0) == 5  # a QueueStream
+    assert ops._launch_stream(None, "cache_copy_pages", 0, 0) == 77
