@@ -29,9 +29,17 @@
 // row instead and seen by nobody.
 // The products are those of the prompt's kernel (kr_attn.hip): S^T = K Q^T,
 // softmax in base 2 with a lazily moved maximum, O^T += V^T P^T, fp32 state;
-// P is rounded to 16 bits for the matrix cores, which moves a result by at most
-// half a step of sum p |v|, about what rounding the result does; its sum is of
-// the unrounded. fp16 weights carry a factor 2^7 through the sums.
+// P goes to the matrix cores in 16 bits, its sum is of the unrounded. Up to 32
+// rows, where they have time to spare, it goes in two parts, the second what
+// the first left over: a result is rounded once, at its store. Above, in one,
+// which moves a result by at most half a step of sum p |v|, about what its own
+// rounding does. Measured, one part / two, in us: 64 single tokens over 2000 to
+// 4000, head size 128, 4 key heads, 86.7 / 87.1; one over 120001, 8 key heads,
+// 103.4 / 103.7; head size 64, 2 key heads: 64 over 2000 to 4000 29.2 / 30.4, 64
+// over 250 to 500 13.7 / 14.7; but two row blocks (8 trees of 16 over 2900, 8
+// key heads) 33.6 / 35.4, and four (2048 rows of a prompt over 8000, 4 heads of
+// 7) 317 / 405.
+// fp16 weights carry a factor 2^7 through the sums.
 // A block in which some row does not see some key goes the careful way: the
 // scores are masked by 64 bits a row; value rows that are not there or hold a
 // number that is not finite are zeroed in LDS (0 x NaN would reach everybody),
@@ -125,6 +133,24 @@ __device__ __forceinline__ uint2 LoadU64Dev(const void *base, int off)
         __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), short(0), 0x7fffffff, 0x00020000);
     const U32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 16 /* sc1 */);
     return make_uint2(v.x, v.y);
+}
+
+// A weight in two parts: the first its leading bits, the second what they left
+// over and a little more (2^-23 of it; fp16: 2^-24, the smallest there is, as
+// weights go to 2^7 and more), so that neither part of a weight that is not 0
+// is 0 or negative: an infinite value times them is itself, and no NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t Pack2Down(float lo, float hi)
+{
+    if constexpr (DT == kBF16) return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+}
+
+template <int DT>
+__device__ __forceinline__ float PartLeft(float p, float first)
+{
+    if constexpr (DT == kBF16) return __builtin_fmaf(p, 1.0f + 0x1p-23f, -first);
+    else return (p - first) + fminf(p, 0x1p-24f);
 }
 
 // Any 16-bit value of the eight that is an infinity or a NaN.
@@ -254,6 +280,7 @@ PagedKernel(PagedParams p)
     constexpr int RPD = 64 / DCH;           // rows per 1 KB DMA block
     constexpr int DPW = BLK / RPD / QW;     // DMA blocks per wave, operand and stage
     constexpr int VAH = 4;                  // V fragments read ahead
+    constexpr bool FINE = QW == 1;          // P in two parts (see the top)
     constexpr int VM = 2 * DPW + 1;         // DMA instructions of a wave's stage
     static_assert((NS - 1) * VM < 64, "vmcnt");
     static_assert(SB >= 64, "the host bounds the line by stages of 64 keys");
@@ -599,7 +626,7 @@ PagedKernel(PagedParams p)
                 // maximum's 2^8, and full down to 2^-21; O and l both have the
                 // factor, in every stream and piece, and lose it in O / l
                 const float sub = DT == kF16 ? 7.0f - msub : -msub;
-                uint4 pf[2 * KB];
+                uint4 pf[2 * KB], pl[FINE ? 2 * KB : 1];
                 float ls[4];
 #pragma unroll
                 for (int c = 0; c < 2 * KB; ++c) {
@@ -610,8 +637,20 @@ PagedKernel(PagedParams p)
                         pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kh][vb + e], p.scale_log2, sub));
                         ls[e & 3] = c == 0 && e < 4 ? pv[e] : ls[e & 3] + pv[e];
                     }
-                    pf[c] = make_uint4(Pack2<DT>(pv[0], pv[1]), Pack2<DT>(pv[2], pv[3]), Pack2<DT>(pv[4], pv[5]),
-                                       Pack2<DT>(pv[6], pv[7]));
+                    if constexpr (FINE) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            hi[e] = Pack2Down<DT>(pv[2 * e], pv[2 * e + 1]);
+                            lo[e] = Pack2<DT>(PartLeft<DT>(pv[2 * e], Elem<DT>::Load(uint16_t(hi[e]))),
+                                              PartLeft<DT>(pv[2 * e + 1], Elem<DT>::Load(uint16_t(hi[e] >> 16))));
+                        }
+                        pf[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        pl[c] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    } else {
+                        pf[c] = make_uint4(Pack2<DT>(pv[0], pv[1]), Pack2<DT>(pv[2], pv[3]), Pack2<DT>(pv[4], pv[5]),
+                                           Pack2<DT>(pv[6], pv[7]));
+                    }
                 }
                 l = l * alpha + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
                 m = mnew;
@@ -641,14 +680,20 @@ PagedKernel(PagedParams p)
                     for (int i = 0; i < NP; ++i) {
                         oacc[i % DBLK] = Mfma<DT>(vf[i], pf[i / DBLK], oacc[i % DBLK]);
                         if (i + VAH < NP) vf[i + VAH] = rd(i + VAH);
+                        if (FINE && i % DBLK == DBLK - 1) {
+#pragma unroll
+                            for (int d = 0; d < DBLK; ++d)
+                                oacc[d] = Mfma<DT>(vf[i - DBLK + 1 + d], pl[FINE ? i / DBLK : 0], oacc[d]);
+                        }
                     }
+                    constexpr int PER = FINE ? 2 : 1;  // products of a fragment
                     __builtin_amdgcn_sched_group_barrier(0x100, 2 * VAH, 0);
 #pragma unroll
                     for (int i = 0; i < NP - VAH; ++i) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
                         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                     }
-                    __builtin_amdgcn_sched_group_barrier(0x008, VAH, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, PER * VAH, 0);
                 }
                 // keys whose values are not all finite (zeroed in the ring):
                 // added to the rows that see them, and to no others
@@ -657,16 +702,20 @@ PagedKernel(PagedParams p)
                     bad &= bad - 1;
                     // key 16 c + 8 e2 + 4 half + e: half word e % 2 of word 4 c + 2 e2 + e / 2 in that half's lanes
                     const int at = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);
-                    uint32_t w = 0;
+                    const auto weight = [&](const auto &pw) {
+                        uint32_t w = 0;
 #pragma unroll
-                    for (int c = 0; c < 2 * KB; ++c) {
-                        w = at == 4 * c ? pf[c].x : w;
-                        w = at == 4 * c + 1 ? pf[c].y : w;
-                        w = at == 4 * c + 2 ? pf[c].z : w;
-                        w = at == 4 * c + 3 ? pf[c].w : w;
-                    }
-                    w = uint32_t(__shfl(int(w), (lane & 31) + 32 * ((key >> 2) & 1), 64));
-                    const float pk = Elem<DT>::Load(uint16_t(w >> (16 * (key & 1))));
+                        for (int c = 0; c < 2 * KB; ++c) {
+                            w = at == 4 * c ? pw[c].x : w;
+                            w = at == 4 * c + 1 ? pw[c].y : w;
+                            w = at == 4 * c + 2 ? pw[c].z : w;
+                            w = at == 4 * c + 3 ? pw[c].w : w;
+                        }
+                        w = uint32_t(__shfl(int(w), (lane & 31) + 32 * ((key >> 2) & 1), 64));
+                        return Elem<DT>::Load(uint16_t(w >> (16 * (key & 1))));
+                    };
+                    float pk = weight(pf);
+                    if constexpr (FINE) pk += weight(pl);
                     const bool here = ((sees >> key) & 1) != 0;
                     const int pos = key0(st) + key, pg = PageOf(p.div, pos);
                     const uint16_t *row = vh0 + int64_t(uint64_t(uint32_t(table[pg])) * p.page_stride +
