@@ -5,6 +5,7 @@ import torch
 
 from kernrelay_amd import kvcache, ops
 from tests.conftest import announce
+from tests.test_gpu_paged import Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,57 @@ def test_outputs_between_the_inputs(gpu, rows):
     if rows > 1:
         with pytest.raises(RuntimeError, match="out overlaps q"):
             ops.attention_paged(cache, 0, seqs, q, dense[1::2][:rows].view(rows, HQ, D))
+
+
+@pytest.mark.parametrize("form", ["step", "tree", "many"])
+def test_two_graphs_on_one_workspace(gpu, form):
+    """Captured calls that share a workspace, replayed one after the other in
+    changing order with eager calls between them: the bits of each alone."""
+    announce("attention_paged two graphs, one workspace, " + form)
+    if form == "many":  # hundreds of units, one long among them: tickets
+        lens = [20] * 100
+        lens[40] = 9000
+        a, b = (Batch(41 + i, 28, 4, 128, BF, 16, lens, [1] * 100) for i in range(2))
+    elif form == "step":
+        a, b = Batch(41, 28, 4, 128, BF, 16, [3000, 40], [1, 1]), Batch(42, 8, 2, 128, BF, 16, [900, 2500, 7], [1, 1, 1])
+    else:
+        a, b = Batch(41, 8, 2, 128, BF, 16, [3000, 40], [30, 9], "tree"), Batch(42, 8, 2, 128, BF, 16, [2000], [70], "tree")
+    want = [x.run() for x in (a, b)]
+    need = [ops.attention_paged_workspace(x.cache, x.seqs, x.HQ) for x in (a, b)]
+    ws = torch.full((max(n for n, _ in need),), 255, dtype=torch.uint8, device="cuda")
+    counters = torch.zeros(max(n for _, n in need), dtype=torch.int32, device="cuda")
+    assert ws.numel() > 0 and (counters.numel() > 0) == (form == "many")
+    outs, graphs = [torch.empty_like(x.q) for x in (a, b)], []
+    call = lambda x, o: ops.attention_paged(x.cache, 1, x.seqs, x.q, o, ws=ws, counters=counters)  # noqa: E731
+    for x, o in zip((a, b), outs):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(x, o)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1), (1, 0, 1)):
+        for o in outs:
+            o.fill_(9.0)
+        for i in order:
+            graphs[i].replay()
+            eager = torch.empty_like(outs[1 - i])
+            call((a, b)[1 - i], eager)
+            assert torch.equal(eager, want[1 - i])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert int(counters.abs().sum()) == 0
+
+
+def test_compact_one_row_to_many(gpu):
+    """A path that names a draft more than once: each place gets its row."""
+    announce("cache_compact, a draft named twice")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(2, 4, 8, 2, 64, device="cuda", generator=g).to(BF) for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    was = [c.clone() for c in (k, v)]
+    seqs = ops.make_seqs(ints([[2, 0]]), ints([5]), ints([0, 6]), 6)
+    ops.cache_compact(ops.make_cache(k, v), seqs, ints([[4, 0, 4, 1]]), ints([4]))
+    for now, old in zip((k, v), was):
+        rows, old_rows = (torch.cat((c[:, 2], c[:, 0]), 1) for c in (now, old))
+        for i, j in enumerate((4, 0, 4, 1)):
+            old_rows[:, 5 + i] = torch.cat((old[:, 2], old[:, 0]), 1)[:, 5 + j]
+        assert torch.equal(rows, old_rows) and torch.equal(now[:, [1, 3]], old[:, [1, 3]])
