@@ -103,7 +103,8 @@ void CheckSeqs(const kr_seqs *s, const char *who)
 // follow each other in one flat index: every lane has work whatever the head
 // counts. The sums and the rotation are fp32; without `chain` the only
 // rounding is the store. Measured: 4096 tokens of 32 + 8 heads of 128, 86 MB in
-// 17.6 us (4.9 TB/s, what a large copy reaches); 48 tokens of 28 + 2 x 4 heads 2.6 us.
+// 17.2 us (5.0 TB/s, what a large copy reaches), with `chain` 19.2 (the four
+// separate launches: 37.2); 48 tokens of 28 + 2 x 4 heads 3.4 us.
 namespace {
 
 struct QkRopeParams {
@@ -339,7 +340,7 @@ void QkRopeLaunch(const QkRopeDesc &d, hipStream_t stream)
 // flight. The pairs travel with the launch, so nothing is copied to the
 // device first and the host has seen every id. A page is (outer, mid, run): a
 // run of contiguous values, merged as far as the strides allow (both usual
-// layouts are one run). Measured: 239 MB in 48.3 us (4.9 TB/s), 14 MB in 3.4.
+// layouts are one run). Measured: 239 MB in 48.0 us (5.0 TB/s), 14 MB in 3.9.
 namespace {
 
 constexpr int kCopyPairs = 384;  // of one launch: 3 KB of kernel arguments

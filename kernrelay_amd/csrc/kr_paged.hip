@@ -12,7 +12,12 @@
 // matrix cores and the softmax's VALU work above. Measured (head size 128): 64
 // single tokens over 2000 to 4000, 4 key heads, 394 MB in 87 us; one over
 // 120001, 8 key heads, 492 MB in 100; 2048 tokens of a prompt over 8000, 28 query
-// heads, 265 GFLOP in 296 (0.9 PFLOP/s).
+// heads, 265 GFLOP in 295 to 317 (cards differ; 0.84 to 0.9 PFLOP/s). There the
+// matrix cores are 44% busy: every K and V fragment is read from LDS for one
+// MFMA, which at their full rate would take the whole of the LDS's (128 B a
+// cycle).
+// Each kernel spills 78 to 94 scalars into vector lanes, a dozen of which are
+// read back in a stage.
 //
 // A unit of work is one key head of one sequence and RT = 32 QW packed rows
 // (row r = new token r / G, query head r % G of the key head's G), so the
@@ -252,15 +257,24 @@ constexpr int kPagedSlots = 512;
 // When units are cut. Whole, the launch lasts as long as its longest unit
 // (`longest` stages of 64 keys; one workgroup alone on a CU has the CU's whole
 // bandwidth and issue); cut, every workgroup has the same share, but a piece's
-// rows are written and read once more (fp32), by a second launch of 5 to 11
-// us. So units are cut where the longest is more than a even shares and c
-// stages. Measured, cut against whole, in us (D 128):
-//   one row block: 1 sequence of 2000 tokens, 8 key heads: 13 / 42; 16 of up to
-//   4000: 50 / 76; 64 of up to 500, 4 heads: 24 / 18; 64 of up to 1800, 8
-//   heads: 89 / 81;
-//   two: 8 trees of 16 over 3000, 8 heads: 31 / 52; 32: 89 / 81;
-//   four: 8 trees of 61 over 2900, 8 heads: 57 / 72; 16: 78 / 74; 1000 rows of a
-//   prompt over 8000, 4 heads of 7: 166 / 184; 2048 rows: 321 / 300.
+// rows are written and read once more (fp32), by a second launch of 6 to 18 us.
+// So units are cut where the longest is more than a even shares and c stages.
+// Measured, cut against whole, in us, at head size 128:
+//   one row block: 1 sequence of 2000 tokens, 8 key heads: 14.5 / 46; 16 of up to
+//   4000: 51 / 85; 64 of up to 500, 4 heads: 28 / 19; 64 of up to 1800, 8 heads:
+//   86 / 79;
+//   two: 8 trees of 16 over 3000, 8 heads: 34 / 52; 32: 91 / 82; 32 of 8 over
+//   1000, 4 heads of 7: 30 / 24 (and cut, against the better);
+//   four: 8 trees of 61 over 2900, 8 heads: 55 / 73; 16: 93 / 78; 1000 rows of a
+//   prompt over 8000, 4 heads of 7: 169 / 185; 2048 rows: 330 / 309;
+// and at 64, with 2 key heads of 7, where the shares are those of 128 though
+// four workgroups would fit a CU:
+//   one: 1 of 700: 14.4 / 15.2; 16 of up to 500: 14.4 / 12.7 (cut, against the
+//   better); 1000: 14.8 / 19; 64 of up to 500: 14.8 / 13.2 (cut); 1800: 22 / 30;
+//   128 of up to 4000: 53 / 48;
+//   two: 8 trees of 9 over 800: 17 / 16 (cut); 3000: 19 / 40; 64: 30 / 40;
+//   four: 8 trees of 61 over 1500: 25 / 31; 32 over 2900: 57 / 53 (cut); 2048
+//   rows over 8000: 120 / 152; 2 of 1500 over 4000: 82 / 110 (whole).
 template <int QW> struct CutRule {
     static constexpr float a = QW == 4 ? 2.0f : 2.6f;
     static constexpr int c = QW == 1 ? 6 : QW == 2 ? 8 : 16;
@@ -869,8 +883,11 @@ PagedKernel(PagedParams p)
 
 // The second launch: sums the pieces of the cut units, in the line's order.
 // Workgroup (x, y) takes 256 / SP chunks of 4 columns of unit x, SP threads to
-// a chunk with a share of its pieces each, UN of them in flight: units of few
-// rows come in up to 64 pieces, those of many in a few.
+// a chunk with a share of its pieces each, UN of them in flight. A unit of
+// few rows may come in nearly as many pieces as there are workgroups, one of many
+// rows in a few. One sequence of 120001 tokens, head size 128, 8, 4, 2 and 1 key
+// heads: 63, 126, 235 and 469 pieces a unit, 6, 7, 12 and 18 us beside 93, 52, 30
+// and 18 of the first launch (head size 64, 2 heads: 10 beside 19).
 template <int QW> struct JoinShape {
     static constexpr int SP = 4 / QW, UN = QW == 4 ? 4 : 8, CH = 256 / SP;
 };
@@ -935,18 +952,24 @@ const void *PagedFor(int dtype, int D, int qw, bool wide)
 
 // Units from which the pieces of a cut one are summed by the last of them
 // (tickets) instead of a second launch. That many units are cut only where
-// their lengths differ a lot, and the launch costs 2 to 4 us all the same (64
-// sequences of up to 500 tokens, 4 key heads: 20 with it, 18 us without); where
-// cutting is the rule it is the faster (4 sequences of up to 2000, 2 key heads:
-// 13 us against 15).
+// their lengths differ a lot, and the launch costs 2 us all the same (64
+// sequences of up to 500 tokens, 4 key heads, whole: 21.1 with it, 19.4 us
+// without; of up to 1800, 8 heads: 81.3, 79.1); where cutting is the rule it is
+// the faster (4 sequences of up to 2000, 2 key heads of 64: 14.3 us against 15.5).
 constexpr int kTicketUnits = 192;
+// A launch with notes has a workgroup for each unit, so that each writes its
+// note whatever `starts` holds.
+static_assert(kTicketUnits <= kPagedSlots, "units with notes");
 
-// Up to that many units of one row block (and from kTicketUnits) a workgroup
-// has its CU to itself for the most part: it takes four key streams. 64
-// sequences of up to 4000 tokens, 4 key heads: 94 us with two, 89 with four; 128
-// units are better cut for two streams (16 sequences of up to 4000, 8 heads: 50
-// us, four streams 61), and more than 256 better off two to a CU (200 of up to
-// 500, 4 heads: 50, four streams 73).
+// Units of one row block from which, and up to which, a workgroup has its CU to
+// itself for the most part: it takes four key streams. Measured with two streams
+// (the better of cut and whole) / with four, in us, head size 128, 4 key heads,
+// lengths of up to 4000: 128 units 54 / 62, 160 68 / 68, 192 77 / 74, 256 93 / 87,
+// 288 124 / 119; up to 500: 192 19.0 / 18.1, 256 19.3 / 19.3, 288 22 / 32 (more
+// than one to a CU, and two do not fit). Head size 64, 2 heads, up to 4000: 160 38
+// / 38, 192 41 / 40, 256 59 / 48, 288 75 / 66; up to 500: 256 14.9 / 13.7, 288 17.9
+// / 16.8 (two fit: there four streams would go on being the better).
+constexpr int kWideFrom = 192;
 constexpr int kWideUnits = 256;
 
 struct PagedShape {
@@ -974,7 +997,7 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     const int64_t most_stages = (int64_t(s.table_pages) * c.page_size + 63) / 64;
     const int at_least = r.qw == 1 ? CutRule<1>::c : r.qw == 2 ? CutRule<2>::c : CutRule<4>::c;
     const bool cuts = r.units > 0 && most_stages > at_least && r.units * most_stages < (int64_t(1) << 30);
-    r.wide = r.qw == 1 && r.units >= kTicketUnits && r.units <= kWideUnits;
+    r.wide = r.qw == 1 && r.units >= kWideFrom && r.units <= kWideUnits;
     // a ticket, or a note for the second launch, per unit
     r.tickets = cuts && r.units >= kTicketUnits;
     r.part_bytes = cuts ? size_t(kPagedSlots) * 2 * 32 * r.qw * (c.head_dim + 2) * 4 : 0;
