@@ -352,6 +352,125 @@ int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs,
                           void *out, int64_t ldo, int rows, int HQ, float scale, void *ws, size_t ws_bytes,
                           int32_t *counters, int n_counters, void *stream);
 
+/* kr_op_attention_paged that also writes lse[r * ld_lse + head] = ln sum
+ * exp(scale q.k) over the keys that the row sees (-infinity where it sees
+ * none), fp32 [rows, HQ], ld_lse = 0 for packed rows: what
+ * kr_op_attention_paged_weigh takes. The same results and workspace; lse
+ * overlaps no other tensor of the call (refused for q, out and the layer). */
+int kr_op_attention_paged_lse(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                              void *out, int64_t ldo, float *lse, int64_t ld_lse, int rows, int HQ, float scale,
+                              void *ws, size_t ws_bytes, int32_t *counters, int n_counters, void *stream);
+
+/* Attention weight that cached tokens got so far: fp32 [layers, entries,
+ * heads, width], the strides in elements (rows of width contiguous, no two
+ * overlapping). Sequence b of a launch has entry[b] (device [seqs]; NULL: b),
+ * token t of it column t. A sequence whose entry is outside 0..entries-1 has
+ * none: the calls below leave it alone. No two sequences of a launch may have
+ * the same entry. */
+typedef struct kr_weights {
+    float *w;
+    int64_t layer_stride;
+    int64_t entry_stride;
+    int64_t head_stride;
+    int32_t layers;
+    int32_t entries;
+    int32_t heads;
+    int32_t width;
+    const int32_t *entry;
+} kr_weights;
+
+/* Adds what the cached tokens get from a launch's new tokens to their weights
+ * of a layer: for key head h and column j of sequence b
+ *   sum over new tokens i that see j, query heads g of h: exp(scale q_ig.k_j - lse[i, g])
+ * is added to decay times the old value for a cached token (decay = 0: the old
+ * value is not read), and stands for itself for a new one. q, lse as of
+ * kr_op_attention_paged_lse for the same handles; a row whose lse is
+ * -infinity, and what a row does not see, count nothing, whatever is there.
+ * last > 0: only the last `last` new tokens of each sequence count. Columns
+ * past the width are left out, sequences without new tokens left alone.
+ * path != NULL: the drafts of seqs have been accepted and moved together
+ * (kr_op_cache_compact with this path and these handles); new token i of
+ * sequence b is row starts[b] + path[b][i], i < path_lens[b], and sees the
+ * cached ones and the path up to itself (the handle's tree is not looked at);
+ * entries of the path that name no row of the sequence count nothing. path:
+ * device [seqs, path_width], row stride ld_path. ws: caller-owned device
+ * memory of at least kr_op_attention_paged_weigh_workspace's size, for one
+ * stream at a time (it may hold anything). The same bits at every call. */
+int kr_op_attention_paged_weigh_workspace(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_bytes);
+int kr_op_attention_paged_weigh(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                                const float *lse, int64_t ld_lse, int rows, int HQ, float scale,
+                                const kr_weights *weights, int last, float decay, const int32_t *path,
+                                int64_t ld_path, int path_width, const int32_t *path_lens, void *ws, size_t ws_bytes,
+                                void *stream);
+
+/* Sequences with more than `budget` tokens (lens of the handle, its starts and
+ * tree are not looked at) come down to that many, layer by layer and key head
+ * by key head: the first `sinks` and the last `recent` tokens stay, and of the
+ * others the budget - sinks - recent with the largest weights, of equal ones
+ * the first (a NaN is below everything). Afterwards token i of the sequence is
+ * the one that was token keep[layer, b, head, i]: what stays and stands at
+ * sinks..budget-recent-1 is not moved, the others among the largest take the
+ * free places there, first to first, and the recent ones follow in their
+ * order; keys, values and weights move alike, columns and rows from budget on
+ * keep what they hold. (Attention does not depend on the order of cached
+ * tokens: their keys carry their positions.) A sequence with fewer tokens has
+ * 0, 1, .. in keep, then -1; so has one without weights or with more tokens than
+ * columns, but for the weights and rows, which stay. keep: int32 device
+ * [layers, seqs, heads, budget], packed. Rows of pages that are none stay.
+ * Sequences must not share pages below position budget. 0 <= sinks, recent;
+ * sinks + recent <= budget. */
+int kr_op_cache_evict(const kr_cache *cache, const kr_seqs *seqs, const kr_weights *weights, int budget, int sinks,
+                      int recent, int32_t *keep, void *stream);
+
+/* Drafted tokens and what the target model says to them. Row r of a launch
+ * (rows starts[b].. of sequence b, as in kr_seqs) is a token; logits
+ * [rows, vocab] (row stride ld_logits; KR_BF16, KR_F16 or KR_F32) are the
+ * target's after it. The first row of a sequence is its last token, decided
+ * before; the others are drafts: row i of the sequence is tokens[r], drawn to
+ * follow row parents[r] of the sequence (an earlier one; otherwise it follows
+ * nothing). parents == NULL: each row follows the one before it. draft
+ * [rows, vocab] (row stride ld_draft, draft_dtype): the probabilities from
+ * which the tokens that follow row r were drawn, each on its own; NULL: the
+ * drafts were not drawn. A negative or NaN probability is 0, a NaN logit -infinity. Any
+ * vocab and strides >= vocab; rows that are not 16-byte aligned are read more slowly. */
+typedef struct kr_drafts {
+    const void *logits;
+    int64_t ld_logits;
+    const void *draft;
+    int64_t ld_draft;
+    const int64_t *tokens;    /* device [rows] */
+    const int32_t *parents;   /* device [rows], or NULL */
+    const float *u;           /* device [rows]: uniform in [0, 1), one for each draft */
+    const float *u_next;      /* device [seqs]: one for the token that follows */
+    const float *temperature; /* device [seqs], or NULL: 1; <= 0 or NaN: the first of the largest logits has it all */
+    int32_t dtype;
+    int32_t draft_dtype;
+    int32_t vocab;
+    int32_t rows;
+} kr_drafts;
+
+/* Rejection sampling down the drafts of each sequence. At a row with
+ * probabilities p = softmax(logits / temperature) its drafts are tried in
+ * order: token x is accepted if u q(x) < p(x) (q = 1 where the drafts were
+ * not drawn), and the walk goes on there; if not, p becomes max(p - q, 0)
+ * over its sum (without q: p without x over its sum; where nothing is left, p
+ * stays). Where none is accepted, the token that follows is the first v with
+ * p(0) + .. + p(v) > u_next (p(0) + .. + p(vocab - 1)), or the last with p > 0.
+ * The kept tokens are then distributed as the target's own. All of it in 64
+ * bits. Out: path[b][..] int32 [seqs, width], row stride ld_path: the accepted
+ * rows of the sequence from 0 on, then -1 (kr_op_cache_compact takes it; a
+ * walk ends after `width` rows, with the p of the last one); path_lens
+ * [seqs]; next [seqs]: -1 where a row has no logit above -infinity, or the
+ * sequence no rows. max_new <= 1024; of kr_seqs starts and max_new are looked
+ * at. ws: caller-owned device memory of at least the sizes that
+ * kr_op_verify_drafts_workspace reports (functions of host fields alone);
+ * counters zero before the first call and left zero; calls sharing them must
+ * be ordered. */
+int kr_op_verify_drafts_workspace(const kr_drafts *drafts, const kr_seqs *seqs, size_t *ws_bytes, int *counters);
+int kr_op_verify_drafts(const kr_drafts *drafts, const kr_seqs *seqs, int32_t *path, int64_t ld_path, int width,
+                        int32_t *path_lens, int64_t *next, void *ws, size_t ws_bytes, int32_t *counters,
+                        int n_counters, void *stream);
+
 /* Page dst[i] becomes a copy of page src[i], keys and values of every layer.
  * src and dst are HOST arrays, read during the call. Refused: ids outside the
  * cache, a page named twice in dst, a page in both src and dst. */

@@ -489,6 +489,101 @@ int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs,
     });
 }
 
+int kr_op_attention_paged_lse(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                              void *out, int64_t ldo, float *lse, int64_t ld_lse, int rows, int HQ, float scale,
+                              void *ws, size_t ws_bytes, int32_t *counters, int n_counters, void *stream)
+{
+    return Guard([&] {
+        kr::PagedAttnDesc d;
+        d.cache = cache;
+        d.seqs = seqs;
+        d.layer = layer;
+        d.q = q;
+        d.out = out;
+        d.ldq = ldq;
+        d.ldo = ldo;
+        d.rows = rows;
+        d.HQ = HQ;
+        d.scale = scale;
+        d.ws = ws;
+        d.ws_bytes = ws_bytes;
+        d.cnt = counters;
+        d.cnt_len = n_counters;
+        d.with_lse = true;
+        d.lse = lse;
+        d.ld_lse = ld_lse;
+        kr::PagedAttnLaunch(d, S(stream));
+    });
+}
+
+int kr_op_attention_paged_weigh_workspace(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_bytes)
+{
+    return Guard([&] {
+        if (ws_bytes == nullptr) throw std::runtime_error("null output pointer");
+        kr::WeighNeeds(cache, seqs, HQ, ws_bytes);
+    });
+}
+
+int kr_op_attention_paged_weigh(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+                                const float *lse, int64_t ld_lse, int rows, int HQ, float scale,
+                                const kr_weights *weights, int last, float decay, const int32_t *path,
+                                int64_t ld_path, int path_width, const int32_t *path_lens, void *ws, size_t ws_bytes,
+                                void *stream)
+{
+    return Guard([&] {
+        kr::WeighDesc d;
+        d.cache = cache;
+        d.seqs = seqs;
+        d.weights = weights;
+        d.layer = layer;
+        d.q = q;
+        d.ldq = ldq;
+        d.lse = lse;
+        d.ld_lse = ld_lse;
+        d.rows = rows;
+        d.HQ = HQ;
+        d.scale = scale;
+        d.last = last;
+        d.decay = decay;
+        d.path = path;
+        d.ld_path = ld_path;
+        d.path_width = path_width;
+        d.path_lens = path_lens;
+        d.ws = ws;
+        d.ws_bytes = ws_bytes;
+        kr::WeighLaunch(d, S(stream));
+    });
+}
+
+int kr_op_cache_evict(const kr_cache *cache, const kr_seqs *seqs, const kr_weights *weights, int budget, int sinks,
+                      int recent, int32_t *keep, void *stream)
+{
+    return Guard([&] { kr::EvictLaunch(cache, seqs, weights, budget, sinks, recent, keep, S(stream)); });
+}
+
+int kr_op_verify_drafts_workspace(const kr_drafts *drafts, const kr_seqs *seqs, size_t *ws_bytes, int *counters)
+{
+    return Guard([&] {
+        if (ws_bytes == nullptr || counters == nullptr) throw std::runtime_error("null output pointer");
+        kr::VerifyNeeds(drafts, seqs, ws_bytes, counters);
+    });
+}
+
+int kr_op_verify_drafts(const kr_drafts *drafts, const kr_seqs *seqs, int32_t *path, int64_t ld_path, int width,
+                        int32_t *path_lens, int64_t *next, void *ws, size_t ws_bytes, int32_t *counters,
+                        int n_counters, void *stream)
+{
+    return Guard([&] {
+        kr::VerifyOut o;
+        o.path = path;
+        o.ld_path = ld_path;
+        o.width = width;
+        o.path_lens = path_lens;
+        o.next = next;
+        kr::VerifyLaunch(drafts, seqs, o, ws, ws_bytes, counters, n_counters, S(stream));
+    });
+}
+
 int kr_op_cache_copy_pages(const kr_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream)
 {
     return Guard([&] { kr::CopyPagesLaunch(cache, src, dst, n, S(stream)); });

@@ -1,7 +1,9 @@
 // Host interface of the paged key/value cache's kernels: q/k norm + RoPE into
 // plain tensors or cache slots, page copies and draft compaction
-// (kr_cache.hip), attention over the pages (kr_paged.hip). The handles are
-// the C ABI's own (include/kr_ops.h).
+// (kr_cache.hip), attention over the pages (kr_paged.hip), the weight it gives
+// each cached token (kr_weigh.hip) and the tokens that go by it (kr_evict.hip),
+// drafts against the target's logits (kr_verify.hip). The handles are the C
+// ABI's own (include/kr_ops.h).
 #pragma once
 
 #include "../../include/kr_ops.h"
@@ -95,7 +97,79 @@ struct PagedAttnDesc {
     size_t ws_bytes = 0;
     int32_t *cnt = nullptr;
     int cnt_len = 0;
+    bool with_lse = false;  // the logarithms of the rows' sums too
+    float *lse = nullptr;
+    int64_t ld_lse = 0;
 };
 void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream);
+
+// Memory from p on, as far as a launch may touch it.
+struct MemSpan {
+    const void *p = nullptr;
+    int64_t bytes = 0;
+};
+inline bool Meets(const MemSpan &a, const MemSpan &b)
+{
+    if (a.p == nullptr || b.p == nullptr || a.bytes < 1 || b.bytes < 1) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x < y + uintptr_t(b.bytes) && y < x + uintptr_t(a.bytes);
+}
+// Rows of `width` values of `size` bytes, every `ld` values.
+inline MemSpan RowsSpan(const void *p, int64_t rows, int64_t ld, int64_t width, int64_t size)
+{
+    return MemSpan{p, rows < 1 ? 0 : ((rows - 1) * ld + width) * size};
+}
+
+// Throws unless the weights' rows are apart; strides of dimensions of one element become 0.
+kr_weights CheckWeights(const kr_weights *w, const kr_cache &c, const char *who);
+MemSpan WeightsSpan(const kr_weights &w);
+
+// Attention weight per cached token (kr_weigh.hip).
+void WeighNeeds(const kr_cache *c, const kr_seqs *s, int HQ, size_t *ws_bytes);
+struct WeighDesc {
+    const kr_cache *cache = nullptr;
+    const kr_seqs *seqs = nullptr;
+    const kr_weights *weights = nullptr;
+    int layer = 0;
+    const void *q = nullptr;
+    const float *lse = nullptr;
+    int64_t ldq = 0, ld_lse = 0;
+    int rows = 0, HQ = 0, last = 0;
+    float scale = 1.0f, decay = 1.0f;
+    const int32_t *path = nullptr, *path_lens = nullptr;
+    int64_t ld_path = 0;
+    int path_width = 0;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+};
+void WeighLaunch(const WeighDesc &d, hipStream_t stream);
+
+// Tokens that got least go (kr_evict.hip).
+void EvictLaunch(const kr_cache *c, const kr_seqs *s, const kr_weights *w, int budget, int sinks, int recent,
+                 int32_t *keep, hipStream_t stream);
+
+// Drafts against the target's logits (kr_verify.hip).
+void VerifyNeeds(const kr_drafts *d, const kr_seqs *s, size_t *ws_bytes, int *counters);
+struct VerifyOut {
+    int32_t *path = nullptr, *path_lens = nullptr;
+    int64_t ld_path = 0;
+    int width = 0;
+    int64_t *next = nullptr;
+};
+void VerifyLaunch(const kr_drafts *d, const kr_seqs *s, const VerifyOut &o, void *ws, size_t ws_bytes, int32_t *cnt,
+                  int cnt_len, hipStream_t stream);
+
+// A value that is the same in every lane, as the scalar it is.
+__device__ __forceinline__ int Uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ int WaveScan(int v, int lane)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
 
 }  // namespace kr

@@ -87,6 +87,8 @@ struct PagedParams {
     int max_units;
     int min_piece;     // stages of a piece, unless the units are shorter
     int slots;         // workgroups of the cut schedule; 0: whole units only
+    float *lse;        // the rows' logarithms of sums [rows, HQ] (the kernels with LSE)
+    int64_t ld_lse;
 };
 
 typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
@@ -107,19 +109,6 @@ __device__ __forceinline__ PagedSeq LoadSeq(const PagedParams &p, int b)
     s.len = min(s.len, p.cap);
     return s;
 }
-
-__device__ __forceinline__ int WaveScan(int v, int lane)
-{
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
-
-// A value that is the same in every lane, as the scalar it is.
-__device__ __forceinline__ int Uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A wave's own LDS writes before its other lanes' reads of them.
 __device__ __forceinline__ void WaveLdsOrder()
@@ -236,6 +225,15 @@ __device__ __forceinline__ PieceSum SumPieces(const float *ws, int part, int lo,
     return s;
 }
 
+// ln sum exp of a row from its base-2 maximum m and sum l.
+template <int DT>
+__device__ __forceinline__ float LseOf(float m, float l)
+{
+    // (fp16 weights carry 2^7: see the kernel)
+    const float log2_sum = __builtin_amdgcn_logf(l) - (DT == kF16 ? 7.0f : 0.0f);
+    return l == 0.0f ? -INFINITY : (m + log2_sum) * 0.6931471805599453f;
+}
+
 // A chunk's result to its row: row r of the unit's packed rows is new token
 // r / G, query head `head` + r % G.
 template <int DT>
@@ -248,6 +246,13 @@ __device__ __forceinline__ void StoreSum(const PieceSum &s, uint16_t *o, int64_t
     w.x = Pack2<DT>(s.acc[0] * inv, s.acc[1] * inv);
     w.y = Pack2<DT>(s.acc[2] * inv, s.acc[3] * inv);
     *reinterpret_cast<uint2 *>(o + int64_t(first + tok) * ldo + int64_t(head + r - tok * G) * D + cc * 4) = w;
+}
+
+template <int DT>
+__device__ __forceinline__ void StoreLse(const PieceSum &s, float *lse, int64_t ld, int first, int r, int head, int G)
+{
+    const int tok = r / G;
+    lse[int64_t(first + tok) * ld + head + r - tok * G] = LseOf<DT>(s.m, s.l);
 }
 
 // Workgroups of the cut schedule: two on each of 256 CUs (their rings fill 128
@@ -280,7 +285,7 @@ template <int QW> struct CutRule {
     static constexpr int c = QW == 1 ? 6 : QW == 2 ? 8 : 16;
 };
 
-template <int DT, int D, int QW, int KW, int KB, int NS>
+template <int DT, int D, int QW, int KW, int KB, int NS, bool LSE>
 __global__ void __attribute__((amdgpu_flat_work_group_size(64 * QW * KW, 64 * QW * KW), amdgpu_waves_per_eu(2)))
 PagedKernel(PagedParams p)
 {
@@ -802,6 +807,9 @@ PagedKernel(PagedParams p)
         const bool out_row = live && ks == 0 && r0 + wq * 32 + (lane & 31) < R;
         if (pieces == 1) {
             if (out_row) {
+                if constexpr (LSE) {
+                    if (hf == 0) p.lse[int64_t(sq.first + tok) * p.ld_lse + h * p.G + r - tok * p.G] = LseOf<DT>(m, l);
+                }
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 uint16_t *orow = p.o + int64_t(sq.first + tok) * p.ldo + int64_t(h * p.G + r - tok * p.G) * D;
 #pragma unroll
@@ -853,6 +861,9 @@ PagedKernel(PagedParams p)
                         const PieceChunk<D> c(ch, nrow);
                         const PieceSum s = SumPieces<D, QW, 8, true>(p.ws, first, 0, pieces, c);
                         StoreSum<DT>(s, p.o, p.ldo, sq.first, r0 + c.row, h * p.G, p.G, D, c.cc);
+                        if constexpr (LSE) {
+                            if (c.cc == 0) StoreLse<DT>(s, p.lse, p.ld_lse, sq.first, r0 + c.row, h * p.G, p.G);
+                        }
                     }
                 }
             }
@@ -892,9 +903,9 @@ template <int QW> struct JoinShape {
     static constexpr int SP = 4 / QW, UN = QW == 4 ? 4 : 8, CH = 256 / SP;
 };
 
-template <int DT, int D, int QW>
+template <int DT, int D, int QW, bool LSE>
 __global__ void __launch_bounds__(256)
-PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ldo, int G)
+PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ldo, int G, float *lse, int64_t ld_lse)
 {
     constexpr int SP = JoinShape<QW>::SP, CH = JoinShape<QW>::CH;
     __shared__ float part_sum[SP > 1 ? SP - 1 : 1][6][CH];
@@ -926,7 +937,11 @@ PagedJoinKernel(const float *ws, const PagedJoin *joins, uint16_t *o, int64_t ld
             s.m = mn;
         }
     }
-    if (ch < chunks) StoreSum<DT>(s, o, ldo, j.first, j.r0 + c.row, j.head, G, D, c.cc);
+    if (ch >= chunks) return;
+    StoreSum<DT>(s, o, ldo, j.first, j.r0 + c.row, j.head, G, D, c.cc);
+    if constexpr (LSE) {
+        if (c.cc == 0) StoreLse<DT>(s, lse, ld_lse, j.first, j.r0 + c.row, j.head, G);
+    }
 }
 
 // Rows a unit holds for this many rows of a sequence and key head.
@@ -935,19 +950,20 @@ int UnitWaves(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 // The kernels: one row block with two key streams, or with four (the whole
 // CU's rings in one workgroup); two with two streams; four with one, 64 keys a
 // stage.
-template <int DT, int D>
+template <int DT, int D, bool LSE>
 const void *PagedFor(int qw, bool wide)
 {
-    if (qw == 1 && wide) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 4, 1, 2>);
-    if (qw == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1, 2>);
-    if (qw == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1, 2>);
-    return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2, 2>);
+    if (qw == 1 && wide) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 4, 1, 2, LSE>);
+    if (qw == 1) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 1, 2, 1, 2, LSE>);
+    if (qw == 2) return reinterpret_cast<const void *>(&PagedKernel<DT, D, 2, 2, 1, 2, LSE>);
+    return reinterpret_cast<const void *>(&PagedKernel<DT, D, 4, 1, 2, 2, LSE>);
 }
 
+template <bool LSE>
 const void *PagedFor(int dtype, int D, int qw, bool wide)
 {
-    if (D == 64) return dtype == kBF16 ? PagedFor<kBF16, 64>(qw, wide) : PagedFor<kF16, 64>(qw, wide);
-    return dtype == kBF16 ? PagedFor<kBF16, 128>(qw, wide) : PagedFor<kF16, 128>(qw, wide);
+    if (D == 64) return dtype == kBF16 ? PagedFor<kBF16, 64, LSE>(qw, wide) : PagedFor<kF16, 64, LSE>(qw, wide);
+    return dtype == kBF16 ? PagedFor<kBF16, 128, LSE>(qw, wide) : PagedFor<kF16, 128, LSE>(qw, wide);
 }
 
 // Units from which the pieces of a cut one are summed by the last of them
@@ -1006,18 +1022,18 @@ PagedShape ShapeOf(const kr_cache &c, const kr_seqs &s, int HQ)
     return r;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool LSE>
 void JoinGo(int qw, const PagedParams &p, hipStream_t stream)
 {
     const int64_t rows = std::min(int64_t(p.max_new) * p.G, int64_t(32 * qw));
     const int64_t per = qw == 1 ? JoinShape<1>::CH : qw == 2 ? JoinShape<2>::CH : JoinShape<4>::CH;
     const dim3 grid(unsigned(p.max_units), unsigned((rows * (D / 4) + per - 1) / per));
     const auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p.ws, p.joins, p.o, p.ldo, p.G);
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p.ws, p.joins, p.o, p.ldo, p.G, p.lse, p.ld_lse);
     };
-    if (qw == 1) go(PagedJoinKernel<DT, D, 1>);
-    else if (qw == 2) go(PagedJoinKernel<DT, D, 2>);
-    else go(PagedJoinKernel<DT, D, 4>);
+    if (qw == 1) go(PagedJoinKernel<DT, D, 1, LSE>);
+    else if (qw == 2) go(PagedJoinKernel<DT, D, 2, LSE>);
+    else go(PagedJoinKernel<DT, D, 4, LSE>);
 }
 
 }  // namespace
@@ -1100,14 +1116,32 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
     if (Overlap(out, RowSpan{d.q, p.ldq, d.rows, width})) refuse("out overlaps q");
     if (Overlap(out, LayerSpan(c, c.k, d.layer)) || Overlap(out, LayerSpan(c, c.v, d.layer)))
         refuse("out overlaps the cache");
+    if (d.with_lse) {
+        p.lse = d.lse;
+        p.ld_lse = d.ld_lse > 0 ? d.ld_lse : d.HQ;
+        if (p.lse == nullptr || (reinterpret_cast<uintptr_t>(p.lse) & 3) != 0) refuse("lse is missing or misaligned");
+        if (d.rows > 1 && p.ld_lse < d.HQ) refuse("lse rows overlap");
+        const MemSpan lse = RowsSpan(p.lse, d.rows, p.ld_lse, d.HQ, 4);
+        const RowSpan k = LayerSpan(c, c.k, d.layer), v = LayerSpan(c, c.v, d.layer);
+        if (Meets(lse, RowsSpan(d.q, d.rows, p.ldq, width, 2)) || Meets(lse, RowsSpan(d.out, d.rows, p.ldo, width, 2)) ||
+            Meets(lse, MemSpan{k.p, k.width * 2}) || Meets(lse, MemSpan{v.p, v.width * 2}) ||
+            Meets(lse, MemSpan{p.ws, int64_t(f.ws_bytes)}))
+            refuse("lse overlaps another tensor of the call");
+    }
     void *args[] = {&p};
     const dim3 threads(f.qw == 1 && !f.wide ? 128 : 256);
-    Check(hipLaunchKernel(PagedFor(c.dtype, c.head_dim, f.qw, f.wide), dim3(unsigned(wg)), threads, args, 0, stream),
-          "attention_paged launch");
+    const void *kern = d.with_lse ? PagedFor<true>(c.dtype, c.head_dim, f.qw, f.wide)
+                                  : PagedFor<false>(c.dtype, c.head_dim, f.qw, f.wide);
+    Check(hipLaunchKernel(kern, dim3(unsigned(wg)), threads, args, 0, stream), "attention_paged launch");
     if (p.joins != nullptr) {
-        const bool bf = c.dtype == kBF16;
-        if (c.head_dim == 64) bf ? JoinGo<kBF16, 64>(f.qw, p, stream) : JoinGo<kF16, 64>(f.qw, p, stream);
-        else bf ? JoinGo<kBF16, 128>(f.qw, p, stream) : JoinGo<kF16, 128>(f.qw, p, stream);
+        const auto join = [&](auto bf16, auto f16) { c.dtype == kBF16 ? bf16(f.qw, p, stream) : f16(f.qw, p, stream); };
+        if (c.head_dim == 64) {
+            if (d.with_lse) join(JoinGo<kBF16, 64, true>, JoinGo<kF16, 64, true>);
+            else join(JoinGo<kBF16, 64, false>, JoinGo<kF16, 64, false>);
+        } else {
+            if (d.with_lse) join(JoinGo<kBF16, 128, true>, JoinGo<kF16, 128, true>);
+            else join(JoinGo<kBF16, 128, false>, JoinGo<kF16, 128, false>);
+        }
     }
     Check(hipGetLastError(), "attention_paged launch");
 }

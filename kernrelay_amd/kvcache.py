@@ -1,7 +1,7 @@
 """A paged key/value cache: whose page is whose (PageTables, plain host
 bookkeeping) and the pages themselves on the GPU (PagedCache), with the calls
 that write, read and move them (ops.qk_norm_rope_cache, ops.attention_paged,
-ops.cache_copy_pages, ops.cache_compact).
+ops.cache_copy_pages, ops.cache_compact, ops.cache_evict).
 
 No counterpart in the reference, which stops at the prompt's last row. Pages
 are shared by forked sequences and copied when one of them writes; a sequence
@@ -25,6 +25,7 @@ class PageTables:
         self._free = list(range(pages))  # a heap
         self._refs = [0] * pages
         self._seqs = {}                  # id -> [tokens, page ids]
+        self._gone = {}                  # id -> tokens evicted so far, where there are any
         self._next = 0
 
     def _seq(self, seq):
@@ -38,6 +39,10 @@ class PageTables:
 
     def tokens(self, seq):
         return self._seq(seq)[0]
+
+    def position(self, seq):
+        """Of the sequence's next token: its tokens and those evicted."""
+        return self._seq(seq)[0] + self._gone.get(seq, 0)
 
     def pages_of(self, seq):
         return list(self._seq(seq)[1])
@@ -54,6 +59,8 @@ class PageTables:
         keep = ids[:-(-tokens // self.page_size)]
         new = self.add()
         self._seqs[new] = [tokens, keep]
+        if seq in self._gone:
+            self._gone[new] = self._gone[seq]
         for p in keep:
             self._refs[p] += 1
         return new
@@ -68,6 +75,7 @@ class PageTables:
         """Ends a sequence; pages that no other one shares are free again."""
         self._drop(self._seq(seq)[1])
         del self._seqs[seq]
+        self._gone.pop(seq, None)
 
     def reserve(self, wants):
         """Room for wants[seq] more tokens of each sequence: new pages, and own
@@ -127,6 +135,42 @@ class PageTables:
         self._drop(s[1][keep:])
         del s[1][keep:]
 
+    def own(self, counts):
+        """Own copies of the shared pages that hold the first counts[seq] tokens of
+        each sequence. Returns the pages to copy as (sources, copies).
+        MemoryError if the pages do not suffice."""
+        plan = []
+        left = {}  # shared page -> holders that keep it
+        for seq, n in counts.items():
+            ids = self._seq(seq)[1]
+            for at in range(min(-(-n // self.page_size), len(ids))):
+                holders = left.setdefault(ids[at], self._refs[ids[at]])
+                if holders > 1:
+                    plan.append((ids, at))
+                    left[ids[at]] = holders - 1
+        if len(plan) > len(self._free):
+            raise MemoryError("needs %d pages, %d of %d are free" % (len(plan), len(self._free), self.pages))
+        src, dst = [], []
+        for ids, at in plan:
+            new = self._take()
+            src.append(ids[at])
+            dst.append(new)
+            self._refs[ids[at]] -= 1
+            ids[at] = new
+        return src, dst
+
+    def evict(self, seq, budget):
+        """The sequence has `budget` tokens if it had more; pages behind them are given back."""
+        s = self._seq(seq)
+        if budget < 1:
+            raise ValueError("a budget holds at least one token")
+        if s[0] > budget:
+            self._gone[seq] = self._gone.get(seq, 0) + s[0] - budget
+            s[0] = budget
+            keep = -(-budget // self.page_size)
+            self._drop(s[1][keep:])
+            del s[1][keep:]
+
     def defragment(self):
         """Moves the pages in use to the lowest ids; returns (sources, copies)."""
         used = self.pages - len(self._free)
@@ -153,6 +197,7 @@ class PagedCache:
         self.k, self.v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         self.handle = ops.make_cache(self.k, self.v)
         self._batches, self._last = 0, {}  # how many there were; the last one with new tokens of a sequence
+        self._evicted = set()              # sequences that lost tokens after their last batch
 
     def _state(self, seq):
         """What a batch's rows of a sequence depend on."""
@@ -190,7 +235,7 @@ class PagedCache:
         if depths is not None and any(len(depths[s]) != n for s, n in news.items()):
             raise ValueError("depths must give one depth for each new token")
         # (all that can be refused is, before the tables change)
-        positions = self._ints([self.tables.tokens(s) + (i if depths is None else depths[s][i])
+        positions = self._ints([self.tables.position(s) + (i if depths is None else depths[s][i])
                                 for s, n in news.items() for i in range(n)], torch.int64)
         src, dst = self.tables.reserve(news)
         ops.cache_copy_pages(self.handle, src, dst)
@@ -207,12 +252,15 @@ class PagedCache:
         seqs.depths = None if depths is None else {s: tuple(depths[s]) for s in news}
         self._batches += 1
         self._last.update((s, self._batches) for s, n in news.items() if n > 0)
+        self._evicted.difference_update(s for s, n in news.items() if n > 0)
         seqs.held = {s: self._state(s) for s in news}
         return seqs, positions, self._ints(slots, torch.int64)
 
     def commit(self, news):
         """All new tokens of the last batch are kept."""
         for s, n in news.items():
+            if n > 0 and s in self._evicted:
+                raise ValueError("the batch is out of date: sequence %r lost tokens since" % (s,))
             self.tables.slots(s, n)  # all have room, or none is kept
         for s, n in news.items():
             self.tables.commit(s, n)
@@ -251,6 +299,45 @@ class PagedCache:
     def free(self, seq):
         self.tables.free(seq)
         self._last.pop(seq, None)
+        self._evicted.discard(seq)
+
+    def evict(self, seqs, weights, budget, sinks=0, recent=0):
+        """Of each of the sequences (ids, each once) that has more than `budget`
+        tokens the first `sinks`, the last `recent` and those with the largest
+        weights stay (ops.cache_evict, of every layer and head by itself); the
+        pages behind them are free again. weights: a handle (ops.make_weights)
+        whose entries are these sequences', in this order. Positions of later
+        tokens go on as if nothing had gone. Batches of the sequences are out of
+        date afterwards. Returns keep [layers, seqs, heads, budget]."""
+        import torch
+        self._current()
+        seqs = list(seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError("sinks and recent must fit a budget of at least one token")
+        tokens = [self.tables.tokens(s) for s in seqs]
+        layers, heads = self.k.shape[0], self.k.shape[3]
+        if (weights.layers, weights.heads, weights.device) != (layers, heads, self.handle.device):
+            raise ValueError("the weights must be of the cache's layers and heads, on its device")
+        if weights.entries < len(seqs) if weights.seqs is None else weights.seqs != len(seqs):
+            raise ValueError("the weights must have an entry for each sequence")
+        if any(n > budget and n > weights.width for n in tokens):
+            raise ValueError("a sequence has more tokens than the weights have columns")
+        # (all that can be refused is, before the tables change)
+        src, dst = self.tables.own({s: budget for s, n in zip(seqs, tokens) if n > budget})
+        ops.cache_copy_pages(self.handle, src, dst)
+        ids = [self.tables.pages_of(s) for s in seqs]
+        width = max([1] + [len(i) for i in ids])
+        handle = ops.make_seqs(self._ints([i + [-1] * (width - len(i)) for i in ids], torch.int32).view(-1, width),
+                               self._ints(tokens, torch.int32), self._ints([0] * (len(seqs) + 1), torch.int32), 0)
+        keep = torch.empty(layers, len(seqs), heads, budget, dtype=torch.int32, device=self.k.device)
+        ops.cache_evict(self.handle, handle, weights, keep, sinks=sinks, recent=recent)
+        for s, n in zip(seqs, tokens):
+            if n > budget:
+                self.tables.evict(s, budget)
+                self._evicted.add(s)
+        return keep
 
     def defragment(self):
         self._current()

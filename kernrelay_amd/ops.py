@@ -44,6 +44,22 @@ class KrSeqs(ctypes.Structure):
                 ("max_new", ctypes.c_int32), ("tree_words", ctypes.c_int32)]
 
 
+class KrWeights(ctypes.Structure):
+    """Attention weight per cached token (kr_weights); make_weights fills it."""
+    _fields_ = [("w", ctypes.c_void_p), ("layer_stride", ctypes.c_int64), ("entry_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("layers", ctypes.c_int32), ("entries", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("width", ctypes.c_int32), ("entry", ctypes.c_void_p)]
+
+
+class KrDrafts(ctypes.Structure):
+    """Drafts and the target's logits (kr_drafts)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ld_logits", ctypes.c_int64), ("draft", ctypes.c_void_p),
+                ("ld_draft", ctypes.c_int64), ("tokens", ctypes.c_void_p), ("parents", ctypes.c_void_p),
+                ("u", ctypes.c_void_p), ("u_next", ctypes.c_void_p), ("temperature", ctypes.c_void_p),
+                ("dtype", ctypes.c_int32), ("draft_dtype", ctypes.c_int32), ("vocab", ctypes.c_int32),
+                ("rows", ctypes.c_int32)]
+
+
 class KrRope(ctypes.Structure):
     """Rotation tables and the gains of the per-head norms (kr_rope); make_rope fills it."""
     _fields_ = [("cos_t", ctypes.c_void_p), ("sin_t", ctypes.c_void_p), ("q_gamma", ctypes.c_void_p),
@@ -96,6 +112,14 @@ def _lib():
                                             i32, vp]
         L.kr_op_cache_copy_pages.argtypes = [p(KrCache), vp, vp, i32, vp]
         L.kr_op_cache_compact.argtypes = [p(KrCache), p(KrSeqs), vp, i64, i32, vp, vp]
+        L.kr_op_attention_paged_lse.argtypes = [p(KrCache), i32, p(KrSeqs), vp, i64, vp, i64, vp, i64, i32, i32, f32,
+                                                vp, sz, vp, i32, vp]
+        L.kr_op_attention_paged_weigh_workspace.argtypes = [p(KrCache), p(KrSeqs), i32, p(sz)]
+        L.kr_op_attention_paged_weigh.argtypes = [p(KrCache), i32, p(KrSeqs), vp, i64, vp, i64, i32, i32, f32,
+                                                  p(KrWeights), i32, f32, vp, i64, i32, vp, vp, sz, vp]
+        L.kr_op_cache_evict.argtypes = [p(KrCache), p(KrSeqs), p(KrWeights), i32, i32, i32, vp, vp]
+        L.kr_op_verify_drafts_workspace.argtypes = [p(KrDrafts), p(KrSeqs), p(sz), p(ctypes.c_int)]
+        L.kr_op_verify_drafts.argtypes = [p(KrDrafts), p(KrSeqs), vp, i64, i32, vp, vp, vp, sz, vp, i32, vp]
         L.kr_op_stream_create.argtypes = []
         L.kr_op_stream_create.restype = vp
         L.kr_op_stream_destroy.argtypes = [vp]
@@ -106,7 +130,9 @@ def _lib():
                      "kr_op_embedding", "kr_op_rope", "kr_op_attention", "kr_op_attention_workspace",
                      "kr_op_attention_split", "kr_op_transpose", "kr_op_qk_norm_rope", "kr_op_qk_norm_rope_cache",
                      "kr_op_attention_paged_workspace", "kr_op_attention_paged", "kr_op_cache_copy_pages",
-                     "kr_op_cache_compact"):
+                     "kr_op_cache_compact", "kr_op_attention_paged_lse", "kr_op_attention_paged_weigh_workspace",
+                     "kr_op_attention_paged_weigh", "kr_op_cache_evict", "kr_op_verify_drafts_workspace",
+                     "kr_op_verify_drafts"):
             getattr(L, name).restype = ctypes.c_int
         _BOUND = True
     return L
@@ -532,13 +558,14 @@ def attention_paged_workspace(cache, seqs, HQ):
     return b.value, c.value
 
 
-def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None):
+def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=None, stream=None, lse=None):
     """Attention of a launch's new tokens q [rows, HQ, D] over a layer of the
     cache; their own keys and values are in the cache already, and out
     overlaps neither q nor the layer. ws (uint8) and counters (int32, zero before the
     first call): of attention_paged_workspace's sizes for these handles at
     least (a wider table or more sequences may need more), for one stream at a
-    time; None: no sequence is cut into pieces."""
+    time; None: no sequence is cut into pieces. lse [rows, HQ] float32: gets
+    the logarithms of the rows' sums, for attention_paged_weigh."""
     who = "attention_paged"
     _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
     shape, dt, dev = q.shape, cache.torch_dtype, cache.device
@@ -553,9 +580,34 @@ def attention_paged(cache, layer, seqs, q, out, scale=None, ws=None, counters=No
         # (an empty tensor's address is 0, which would say that there is none; at
         # 0 bytes no address is used, and too few are refused)
         wp, cp, nbytes, ncnt = ws.data_ptr() or 16, counters.data_ptr(), ws.nbytes, counters.shape[0]
-    _check(_lib().kr_op_attention_paged(cache, layer, seqs, qp, ldq, op, ldo, shape[0], shape[1],
-                                        cache.head_dim ** -0.5 if scale is None else scale, wp, nbytes, cp, ncnt,
-                                        _launch_stream(stream, who, dev, seqs.device, q, out, ws, counters)))
+    scale = cache.head_dim ** -0.5 if scale is None else scale
+    if lse is not None:
+        lp, ld_lse = _rows32(lse, shape, who, "lse")
+        _check(_lib().kr_op_attention_paged_lse(cache, layer, seqs, qp, ldq, op, ldo, lp, ld_lse, shape[0], shape[1],
+                                                scale, wp, nbytes, cp, ncnt,
+                                                _launch_stream(stream, who, dev, seqs.device, q, out, ws, counters,
+                                                               lse)))
+        return
+    _check(_lib().kr_op_attention_paged(cache, layer, seqs, qp, ldq, op, ldo, shape[0], shape[1], scale, wp, nbytes,
+                                        cp, ncnt, _launch_stream(stream, who, dev, seqs.device, q, out, ws, counters)))
+
+
+def _rows32(t, shape, who, name):
+    """Address and row stride of a float32 [rows, heads] tensor, as q's shape has them."""
+    if t.dtype == _f32() and t.shape == shape[:2] and (shape[1] == 1 or t.stride(1) == 1):
+        return t.data_ptr(), _pitch(t, who, name)
+    raise ValueError("%s: %s must be float32 %s with contiguous rows" % (who, name, tuple(shape[:2])))
+
+
+_F32 = None
+
+
+def _f32():
+    global _F32
+    if _F32 is None:
+        import torch
+        _F32 = torch.float32
+    return _F32
 
 
 def cache_copy_pages(cache, src, dst, stream=None):
@@ -581,3 +633,159 @@ def cache_compact(cache, seqs, path, path_lens, stream=None):
     width = path.shape[1]
     _check(_lib().kr_op_cache_compact(cache, seqs, path.data_ptr(), _pitch(path, who, "path"), width, lens,
                                       _launch_stream(stream, who, dev, seqs.device, path, path_lens)))
+
+
+# ------------------------------------------------- after a step over the cache
+def make_weights(w, entry=None):
+    """Handle of the attention weight that cached tokens got: w float32
+    [layers, entries, heads, width] (or without layers), rows of width
+    contiguous and none overlapping. entry [seqs] int32, read on the device at
+    each call: where in w a launch's sequence b stands (None: at b; outside w:
+    nowhere, and the calls leave it alone). No two sequences of a launch may
+    have the same entry."""
+    who = "make_weights"
+    _need(w.dim() in (3, 4) and w.dtype == _f32(), who, "w must be float32 [layers, entries, heads, width]")
+    _need(w.shape[-1] <= 1 or w.stride(-1) == 1, who, "rows must be contiguous")
+    _need(all(0 < n < 1 << 31 for n in w.shape), who, "w is empty, or too large")
+    shape, stride = list(w.shape), list(w.stride())
+    if len(shape) == 3:
+        shape, stride = [1] + shape, [0] + stride
+    if entry is not None:
+        _need(entry.dtype == _ints()[0] and entry.dim() == 1 and (entry.shape[0] <= 1 or entry.stride(0) == 1), who,
+              "entry must be a contiguous int32 vector")
+        _need(entry.device == w.device, who, "w and entry must be on one device")
+    h = KrWeights(_ptr(w), *stride[:3], *shape, _ptr(entry))
+    h.keep, h.device, h.seqs = (w, entry), w.get_device(), None if entry is None else entry.shape[0]
+    return h
+
+
+def _of_weights(weights, cache, seqs, who):
+    _need(weights.device == cache.device, who, "the weights are on another device than the cache")
+    if weights.seqs is None:
+        _need(weights.entries >= seqs.seqs, who, "the weights have fewer entries than there are sequences")
+    else:
+        _need(weights.seqs == seqs.seqs, who, "entry must name one entry for each sequence")
+
+
+def attention_paged_weigh_workspace(cache, seqs, HQ):
+    """Bytes of workspace that attention_paged_weigh needs for these handles."""
+    b = ctypes.c_size_t(0)
+    _check(_lib().kr_op_attention_paged_weigh_workspace(cache, seqs, HQ, ctypes.byref(b)))
+    return b.value
+
+
+def attention_paged_weigh(cache, layer, seqs, q, lse, weights, ws, scale=None, last=0, decay=1.0, path=None,
+                          path_lens=None, stream=None):
+    """Adds the attention weight that each cached token gets from a launch's new
+    tokens q [rows, HQ, D] to its weight (make_weights) times `decay`, key head
+    by key head; a new token's weight becomes what it gets. lse [rows, HQ]: of
+    attention_paged for the same handles and scale. last > 0: only the last
+    `last` new tokens of each sequence count. path [seqs, width], path_lens
+    [seqs] int32: the drafts have been accepted and moved together by
+    cache_compact with these; only their rows count. ws: uint8 of
+    attention_paged_weigh_workspace's size, for one stream at a time."""
+    who = "attention_paged_weigh"
+    _need(q.dim() == 3, who, "q is [rows, heads, head_dim]")
+    shape, dev, i32 = q.shape, cache.device, _ints()[0]
+    _need(shape[2] == cache.head_dim, who, "q has another head_dim than the cache")
+    _need(seqs.rows is None or path is not None or seqs.rows >= shape[0], who, "the tree has too few rows")
+    _of_weights(weights, cache, seqs, who)
+    qp, ldq = _heads(q, shape, cache.torch_dtype, who, "q")
+    lp, ld_lse = _rows32(lse, shape, who, "lse")
+    _need((path is None) == (path_lens is None), who, "a path needs its lengths")
+    pp, ld_path, width, pl = None, 0, 0, None
+    if path is not None:
+        _need(path.dim() == 2 and path.dtype == i32 and path.shape[0] == seqs.seqs
+              and (path.shape[1] <= 1 or path.stride(1) == 1), who, "path must be int32 [seqs, width] with contiguous rows")
+        _need(path.shape[1] > 0 or seqs.seqs == 0, who, "path rows are empty")
+        pl = _vector(path_lens, i32, seqs.seqs, who, "path_lens")
+        pp, ld_path, width = path.data_ptr(), _pitch(path, who, "path"), path.shape[1]
+    _need(ws.is_contiguous(), who, "ws must be contiguous")
+    _check(_lib().kr_op_attention_paged_weigh(cache, layer, seqs, qp, ldq, lp, ld_lse, shape[0], shape[1],
+                                              cache.head_dim ** -0.5 if scale is None else scale, weights, last, decay,
+                                              pp, ld_path, width, pl, ws.data_ptr(), ws.nbytes,
+                                              _launch_stream(stream, who, dev, seqs.device, q, lse, ws, path,
+                                                             path_lens)))
+
+
+def cache_evict(cache, seqs, weights, keep, sinks=0, recent=0, stream=None):
+    """Sequences of more than budget = keep.shape[3] tokens come down to that
+    many, layer by layer and key head by key head: the first `sinks`, the last
+    `recent` and of the others those with the largest weights stay. keep [layers,
+    seqs, heads, budget] int32 (packed) gets which token the one at each place
+    was (-1 behind the last). What stands where it may stay is not moved, the
+    others take the free places, the recent ones follow in their order; keys,
+    values and weights move alike. Sequences must not share the pages of their
+    first `budget` tokens."""
+    who = "cache_evict"
+    shape = (cache.layers, seqs.seqs, cache.heads)
+    _need(keep.dim() == 4 and keep.shape[:3] == shape and keep.dtype == _ints()[0] and keep.is_contiguous(), who,
+          "keep must be contiguous int32 %s + [budget]" % (shape,))
+    _of_weights(weights, cache, seqs, who)
+    _check(_lib().kr_op_cache_evict(cache, seqs, weights, keep.shape[3], sinks, recent, keep.data_ptr(),
+                                    _launch_stream(stream, who, cache.device, seqs.device, keep)))
+
+
+def _vocab_rows(t, who, name):
+    """Row stride of a [rows, vocab] tensor with contiguous rows."""
+    _need(t.dim() == 2 and t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1), who,
+          "%s must be [rows, vocab] with contiguous rows" % name)
+    return _pitch(t, who, name)
+
+
+def _drafts(seqs, logits, draft, who):
+    ld = _vocab_rows(logits, who, "logits")
+    _need(logits.shape[0] < 1 << 31 and logits.shape[1] < 1 << 31, who, "logits are too large")
+    ld_draft = 0
+    if draft is not None:
+        _need(draft.shape == logits.shape, who, "draft must have the logits' shape")
+        ld_draft = _vocab_rows(draft, who, "draft")
+    return KrDrafts(None, ld, None, ld_draft, None, None, None, None, None, _dt(logits),
+                    0 if draft is None else _dt(draft), logits.shape[1], logits.shape[0])
+
+
+def verify_drafts_workspace(seqs, logits, draft=None):
+    """(workspace bytes, counters) that verify_drafts needs for these shapes."""
+    b, c = ctypes.c_size_t(0), ctypes.c_int(0)
+    _check(_lib().kr_op_verify_drafts_workspace(_drafts(seqs, logits, draft, "verify_drafts_workspace"), seqs,
+                                                ctypes.byref(b), ctypes.byref(c)))
+    return b.value, c.value
+
+
+def verify_drafts(seqs, logits, tokens, u, u_next, path, path_lens, next_tokens, ws, counters, parents=None, draft=None,
+                  temperature=None, stream=None):
+    """Holds drafted tokens against the target's logits [rows, vocab] (bf16,
+    f16 or f32; row r's are for the token after row r) by rejection sampling.
+    The first row of each sequence is its last token, the others are drafts:
+    tokens [rows] int64, each following row parents[row] of its sequence (int32
+    [rows], an earlier one; None: the row before). draft [rows, vocab]: the
+    probabilities from which the drafts after row r were drawn; None: they were
+    not drawn. u [rows] and u_next [seqs] float32: uniform numbers in [0, 1).
+    temperature [seqs] float32 (None: 1; 0: the first of the largest logits).
+    Out: path [seqs, width] int32 (accepted rows from 0 on, then -1: what
+    cache_compact takes; `width` rows at most), path_lens [seqs] int32,
+    next_tokens [seqs] int64 (the token after the last accepted row; -1: none).
+    ws (uint8) and counters (int32, zero before the first call): of
+    verify_drafts_workspace's sizes, for one stream at a time."""
+    who = "verify_drafts"
+    d = _drafts(seqs, logits, draft, who)
+    rows, n, (i32, i64), f32 = d.rows, seqs.seqs, _ints(), _f32()
+    d.logits, d.draft = logits.data_ptr(), None if draft is None else draft.data_ptr()
+    d.tokens, d.u = _vector(tokens, i64, rows, who, "tokens"), _vector(u, f32, rows, who, "u")
+    d.u_next = _vector(u_next, f32, n, who, "u_next")
+    if parents is not None:
+        # (an empty tensor's address is 0, which would say that there is none)
+        d.parents = _vector(parents, i32, rows, who, "parents") or 16
+    if temperature is not None:
+        d.temperature = _vector(temperature, f32, n, who, "temperature")
+    _need(path.dim() == 2 and path.dtype == i32 and path.shape[0] == n and path.shape[1] > 0
+          and (path.shape[1] == 1 or path.stride(1) == 1), who, "path must be int32 [seqs, width] with contiguous rows")
+    _need(counters.dtype == i32 and counters.dim() == 1 and counters.is_contiguous() and ws.is_contiguous(), who,
+          "ws and counters (an int32 vector) must be contiguous")
+    _check(_lib().kr_op_verify_drafts(d, seqs, path.data_ptr(), _pitch(path, who, "path"), path.shape[1],
+                                      _vector(path_lens, i32, n, who, "path_lens"),
+                                      _vector(next_tokens, i64, n, who, "next_tokens"), ws.data_ptr(), ws.nbytes,
+                                      counters.data_ptr(), counters.shape[0],
+                                      _launch_stream(stream, who, seqs.device, seqs.device, logits, draft, tokens,
+                                                     parents, u, u_next, temperature, path, path_lens, next_tokens, ws,
+                                                     counters)))
