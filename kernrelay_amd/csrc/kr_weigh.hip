@@ -16,6 +16,7 @@
 #include <cmath>
 
 #include "kr_attncore.h"
+#include "kr_dma.h"
 #include "kr_paged.h"
 
 namespace kr {
@@ -64,8 +65,11 @@ struct WeighParams {
     int cap, pages, table_pages, seqs, rows, max_new, tree_words, HQ, HKV, G;
     int entries, width, path_width, last;
     float scale_log2, decay;
-    PageDiv div;
+    PageDiv div, group;  // by page_size, by G
+    float *parts;        // [kWeighParts, 2, kWeighKeys]
 };
+
+constexpr float kLog2E = 1.4426950408889634f;
 
 // A sequence as the launch has it, every number within its bounds whatever
 // the device arrays hold.
@@ -92,138 +96,340 @@ __device__ __forceinline__ WeighSeq LoadSeq(const WeighParams &p, int b)
     return s;
 }
 
-constexpr int kWeighKeys = 128;  // of a workgroup's tile: 32 a wave
-constexpr int kWeighGroups = 2048;
+constexpr int kWeighKeys = 256;   // of a workgroup's tile: 64 a wave
+constexpr int kWeighParts = 768;  // workgroups that share the line: three on each of 256 CUs
+constexpr int kWeighStages = 3;   // row tiles in LDS
 
-template <int DT, int D>
-__global__ void __launch_bounds__(256) WeighKernel(WeighParams p)
+// Where in the line a workgroup stands: row tiles of the key tiles of all
+// sequences, key head by key head. A key tile of new tokens begins with the
+// first row tile that sees any of it: each of the `more` last ones has 8 G row
+// tiles (its 256 tokens) less than the one before it.
+struct WeighLine {
+    int rt;           // row tiles of the sequence
+    int full, more;   // key tiles of a key head with all row tiles, and the others
+    int first, step;  // row tiles that the first of the others leaves out, and each after it more
+    __device__ __forceinline__ WeighLine(const WeighParams &p, const WeighSeq &s)
+    {
+        const int tiles = (s.cols + kWeighKeys - 1) / kWeighKeys;
+        rt = ((s.n - s.skip) * p.G + 31) / 32;
+        full = tiles;
+        if (p.tree == nullptr || p.path != nullptr) full = min(tiles, (s.len + s.skip) / kWeighKeys + 1);
+        more = tiles - full;
+        first = more > 0 ? (full * kWeighKeys - s.len - s.skip) * p.G / 32 : 0;
+        step = 8 * p.G;
+    }
+    __device__ __forceinline__ int Head() const  // of a key head
+    {
+        return full * rt + more * (rt - first) - step * (more * (more - 1) / 2);
+    }
+};
+
+// A piece of a key tile: row tiles r_lo .. r_hi - 1.
+struct WeighPiece {
+    int b, h, t;
+    int start, rows;  // of the tile: where in the line it begins, and its row tiles
+    int skip;         // row tiles that it leaves out
+};
+
+// Position x of the line, in a sequence that begins at `base` of it.
+__device__ __forceinline__ WeighPiece PieceAt(const WeighParams &p, const WeighLine &l, int b, int base, int x)
 {
-    const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
-    const int hf = lane >> 5;
-    // tiles of all sequences in one line: key head by key head, 128 keys each
-    const auto tiles_of = [&](const WeighSeq &s) { return p.HKV * ((s.cols + kWeighKeys - 1) / kWeighKeys); };
-    int tiles = 0;
+    WeighPiece w;
+    const int head = l.Head();
+    w.b = b;
+    w.h = Uni((x - base) / head);
+    int y = x - base - w.h * head;
+    const int at = base + w.h * head;
+    if (y < l.full * l.rt) {
+        w.t = Uni(y / l.rt);
+        w.start = at + w.t * l.rt;
+        w.rows = l.rt;
+        w.skip = 0;
+    } else {
+        w.start = at + l.full * l.rt;
+        w.t = l.full;
+        w.skip = l.first;
+        while (x >= w.start + (l.rt - w.skip)) {
+            w.start += l.rt - w.skip;
+            w.skip += l.step;
+            ++w.t;
+        }
+        w.rows = l.rt - w.skip;
+    }
+    return w;
+}
+
+// The line's length.
+__device__ __forceinline__ int WeighTotal(const WeighParams &p, int lane)
+{
+    int total = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int u = b0 + lane < p.seqs ? tiles_of(LoadSeq(p, b0 + lane)) : 0;
+        int u = 0;
+        if (b0 + lane < p.seqs) {
+            const WeighSeq s = LoadSeq(p, b0 + lane);
+            if (s.cols > 0) u = p.HKV * WeighLine(p, s).Head();
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
-        tiles += Uni(u);
+        total += Uni(u);
     }
-    const int share = (tiles + int(gridDim.x) - 1) / int(gridDim.x);
-    int x = int(blockIdx.x) * share;
-    const int x_end = min(x + share, tiles);
-    if (x >= x_end) return;
-    int b = 0, base = 0;
+    return total;
+}
+
+// The sequence that holds position x of the line, which is inside it; `base`: where it begins.
+__device__ __forceinline__ int WeighFind(const WeighParams &p, int lane, int x, int &base)
+{
+    base = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        const int u = b0 + lane < p.seqs ? tiles_of(LoadSeq(p, b0 + lane)) : 0;
+        int u = 0;
+        if (b0 + lane < p.seqs) {
+            const WeighSeq s = LoadSeq(p, b0 + lane);
+            if (s.cols > 0) u = p.HKV * WeighLine(p, s).Head();
+        }
         const int incl = WaveScan(u, lane) + base;
         const uint64_t above = __ballot(incl > x);
         const int at = above != 0 ? __builtin_ctzll(above) : 63;
         base = Uni(__shfl(incl - (above != 0 ? u : 0), at, 64));
-        if (above != 0) {
-            b = b0 + at;
-            break;
-        }
+        if (above != 0) return b0 + at;
     }
+    return 0;
+}
+
+// A key's sum to its column.
+__device__ __forceinline__ void PutWeight(const WeighParams &p, const WeighSeq &s, int h, int key, float got)
+{
+    float *w = p.w + int64_t(s.entry) * p.w_entry + int64_t(h) * p.w_head + key;
+    float old = 0.0f;
+    if (key < s.len && p.decay != 0.0f) old = p.decay * *w;
+    *w = old + got;
+}
+
+// PLAIN: causal, no path.
+template <int DT, int D, bool PLAIN>
+__global__ void __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2)))
+WeighKernel(WeighParams p)
+{
+    constexpr int KB = 2;                 // 32-key blocks of a wave
+    constexpr int NS = kWeighStages;
+    constexpr int DCH = D / 8;            // 16-byte chunks per row
+    constexpr int RPD = 64 / DCH;         // rows per 1 KB DMA block
+    constexpr int DPW = 32 / RPD / 4;     // DMA blocks per wave and row tile
+    __shared__ __attribute__((aligned(1024))) uint16_t qring[NS][32 * D];
+    __shared__ __attribute__((aligned(256))) float lring[4][NS][64];  // a wave's own: lse of the tile's rows, twice
+    const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
+    const int hf = lane >> 5;
+    const int total = WeighTotal(p, lane);
+    const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+    int x = int(blockIdx.x) * share;
+    const int x_end = min(x + share, total);
+    if (x >= x_end) return;
+    int base;
+    int b = WeighFind(p, lane, x, base);
     WeighSeq sq = LoadSeq(p, b);
-    for (; x < x_end; ++x) {
-        while (x >= base + tiles_of(sq)) {
-            base += tiles_of(sq);
+    WeighLine line(p, sq);
+    const bool causal = PLAIN || p.tree == nullptr || p.path != nullptr;
+    const int qaddr = (lane & 31) * D + KSlot<D>(lane & 31, hf) * 8;  // step dc: XOR 16 dc
+    // 32 packed rows on: so many tokens and query heads
+    const int step_tok = 32 / p.G, step_g = 32 - step_tok * p.G;
+    while (x < x_end) {
+        while (sq.cols == 0 || x >= base + p.HKV * line.Head()) {
+            if (sq.cols > 0) base += p.HKV * line.Head();
             sq = LoadSeq(p, ++b);
+            line = WeighLine(p, sq);
         }
-        const int per = (sq.cols + kWeighKeys - 1) / kWeighKeys;
-        const int h = Uni((x - base) / per), t = x - base - h * per;
-        const int j0 = Uni(t * kWeighKeys + wave * 32);
-        if (j0 >= sq.cols) continue;
-        // this wave's keys: lane l holds key l % 32's chunks of 8, every second one
-        const int pos = j0 + (lane & 31);
-        const int pg = PageOf(p.div, min(pos, sq.total - 1));
-        const int id = p.table[b * p.ld_table + pg];
-        const bool ok = pos < sq.total && uint32_t(id) < uint32_t(p.pages);
-        const int64_t off = ok ? int64_t(uint64_t(uint32_t(id)) * p.page_stride +
-                                         uint64_t(uint32_t(pos - pg * p.div.size)) * p.token_stride)
-                               : 0;
-        const uint16_t *kr = p.k + h * p.head_stride + off + hf * 8;
-        uint4 kf[D / 16];
-#pragma unroll
-        for (int dc = 0; dc < D / 16; ++dc) kf[dc] = *reinterpret_cast<const uint4 *>(kr + dc * 16);
-        const uint32_t there = uint32_t(__ballot(ok));
-        float sum[16];
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sum[v] = 0.0f;
+        const WeighPiece pc = PieceAt(p, line, b, base, x);
+        const int h = pc.h;
+        const int rt_lo = Uni(pc.skip + x - pc.start);
+        const int rt_hi = Uni(min(pc.skip + pc.rows, rt_lo + (x_end - x)));
         const int R = (sq.n - sq.skip) * p.G;
-        // rows whose token comes before the wave's first key see none of it
-        int r0 = 0;
-        if ((p.tree == nullptr || p.path != nullptr) && j0 - sq.len > sq.skip)
-            r0 = (j0 - sq.len - sq.skip) * p.G / 32 * 32;
-        for (; r0 < R; r0 += 32) {
-            const int r = min(r0 + (lane & 31), R - 1);
-            const int i = sq.skip + r / p.G;  // the new token
-            const int g = r % p.G;
-            int tok = i;                      // its row of the sequence
-            if (p.path != nullptr) tok = p.path[b * p.ld_path + i];
-            const bool live = r0 + (lane & 31) < R && tok >= 0 && tok < sq.rows;
-            const int64_t row = sq.first + (live ? tok : 0);
-            const uint16_t *qr = p.q + row * p.ldq + int64_t(h * p.G + g) * D + hf * 8;
-            uint4 qf[D / 16];
+        const int j0 = Uni(pc.t * kWeighKeys + wave * (32 * KB));
+        // ---- this wave's keys: lane l holds key l % 32 of each block, chunks of 8, every second one
+        const uint16_t *kr[KB];
+        uint32_t there = 0;  // bit kb: this lane's key is there
+        bool all = true;     // so are all of the wave's
 #pragma unroll
-            for (int dc = 0; dc < D / 16; ++dc) qf[dc] = *reinterpret_cast<const uint4 *>(qr + dc * 16);
-            const float lse = p.lse[row * p.ld_lse + h * p.G + g];
-            const float nl = lse * -1.4426950408889634f;
-            f32x16 s;
+        for (int kb = 0; kb < KB; ++kb) {
+            const int pos = j0 + kb * 32 + (lane & 31);
+            const int pg = PageOf(p.div, min(pos, sq.total - 1));
+            const int id = p.table[b * p.ld_table + pg];
+            const bool ok = pos < sq.total && uint32_t(id) < uint32_t(p.pages);
+            const int64_t off = ok ? int64_t(uint64_t(uint32_t(id)) * p.page_stride +
+                                             uint64_t(uint32_t(pos - pg * p.div.size)) * p.token_stride)
+                                   : 0;
+            kr[kb] = p.k + h * p.head_stride + off + hf * 8;
+            there |= ok ? 1u << kb : 0u;
+            all = all && __ballot(!ok) == 0;
+        }
+        // packed row r: its row of the launch and query head of the key head
+        const auto row_of = [&](int r, int &g) {
+            const int i = PageOf(p.group, r);
+            g = r - i * p.G;
+            int tok = sq.skip + i;
+            if (!PLAIN && p.path != nullptr) {
+                tok = p.path[b * p.ld_path + tok];
+                if (tok < 0 || tok >= sq.rows) tok = 0;  // (counts nothing, see below)
+            }
+            return int64_t(sq.first + tok);
+        };
+        // this lane's chunks of a row tile's rows, and their lse: from tile to
+        // tile the addresses go on by as many tokens and heads
+        const uint16_t *qp[DPW];
+        const float *lp;
+        int qg[DPW], lg;
+        const auto point = [&](int r0) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+            for (int j = 0; j < DPW; ++j) {
+                const int r = (wave * DPW + j) * RPD + lane / DCH;
+                const int64_t row = row_of(min(r0 + r, R - 1), qg[j]);
+                qp[j] = p.q + row * p.ldq + int64_t(h * p.G + qg[j]) * D + KSlot<D>(r, lane % DCH) * 8;
+            }
+            const int64_t row = row_of(min(r0 + (lane & 31), R - 1), lg);
+            lp = p.lse + row * p.ld_lse + h * p.G + lg;
+        };
+        const auto fetch = [&](int st) {
+            const int r0 = (rt_lo + st) * 32;
+            if (!PLAIN || st == 0 || r0 + 32 > R) {
+                point(r0);
+            } else {
 #pragma unroll
-            for (int dc = 0; dc < D / 16; ++dc) s = Mfma<DT>(kf[dc], qf[dc], s);
-            uint32_t sees = live && lse != -INFINITY ? there : 0u;
-            const int nj = j0 - sq.len;  // the first key as a new token
-            if (p.tree != nullptr && p.path == nullptr) {
-                if (nj + 31 >= 0) {
-                    const uint64_t *tree = p.tree + row * p.ld_tree;
-                    const auto word = [&](int w) { return w < p.tree_words ? tree[w] : 0ull; };
-                    uint64_t w;
-                    if (nj >= 0) {
-                        w = word(nj >> 6) >> (nj & 63);
-                        if ((nj & 63) != 0) w |= word((nj >> 6) + 1) << (64 - (nj & 63));
-                    } else {
-                        w = ((1ull << -nj) - 1) | (word(0) << -nj);
+                for (int j = 0; j < DPW; ++j) {
+                    qg[j] += step_g;
+                    const bool wrap = qg[j] >= p.G;
+                    qg[j] -= wrap ? p.G : 0;
+                    qp[j] += step_tok * p.ldq + step_g * D + (wrap ? p.ldq - p.G * D : 0);
+                }
+                lg += step_g;
+                const bool wrap = lg >= p.G;
+                lg -= wrap ? p.G : 0;
+                lp += step_tok * p.ld_lse + step_g + (wrap ? p.ld_lse - p.G : 0);
+            }
+            const uint32_t dst = LdsAddr(&qring[st % NS][0]) + uint32_t(wave * DPW) * 1024u;
+#pragma unroll
+            for (int j = 0; j < DPW; ++j) DmaLoad16(qp[j], dst + uint32_t(j) * 1024u);
+            DmaTouch4(lp, LdsAddr(&lring[wave][st % NS][0]));
+        };
+        const int ns = rt_hi - rt_lo;
+        __syncthreads();  // (the rings are free)
+        fetch(0);
+        if (ns > 1) fetch(1);
+        uint4 kf[KB][D / 16];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) kf[kb][dc] = *reinterpret_cast<const uint4 *>(kr[kb] + dc * 16);
+        float sum[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sum[kb] = 0.0f;
+        const int nj = j0 - sq.len;  // the first key as a new token
+        for (int st = 0; st < ns; ++st) {
+            if (st + 1 < ns) KR_WAIT_VM(DPW + 1);
+            else KR_WAIT_VM(0);
+            __syncthreads();
+            if (st + 2 < ns) fetch(st + 2);
+            const int r0 = (rt_lo + st) * 32;
+            const uint16_t *Q = &qring[st % NS][0];
+            const float *ls = &lring[wave][st % NS][0];
+            // rows that see nothing of the wave's keys, or all of them
+            const int tok_lo = sq.skip + Uni(PageOf(p.group, r0));
+            const int tok_hi = sq.skip + Uni(PageOf(p.group, min(r0 + 31, R - 1)));
+            if (j0 >= sq.cols || (causal && nj > tok_hi)) continue;
+            const bool dead = __ballot(ls[lane & 31] == -INFINITY) != 0;
+            const bool whole = all && !dead && (PLAIN || p.path == nullptr) && r0 + 32 <= R &&
+                               nj + 32 * KB <= (causal ? tok_lo + 1 : 0);
+            f32x16 s[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[kb][v] = 0.0f;
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) {
+                const uint4 qf = *reinterpret_cast<const uint4 *>(Q + (qaddr ^ (dc * 16)));
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) s[kb] = Mfma<DT>(qf, kf[kb][dc], s[kb]);
+            }
+            // register v: row 8 (v / 4) + 4 hf + v % 4
+            if (whole) {
+#pragma unroll
+                for (int v4 = 0; v4 < 4; ++v4) {
+                    const float4 l4 = *reinterpret_cast<const float4 *>(ls + 8 * v4 + 4 * hf);
+                    const float nl[4] = {l4.x * -kLog2E, l4.y * -kLog2E, l4.z * -kLog2E, l4.w * -kLog2E};
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        float e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][4 * v4 + i], p.scale_log2, nl[i]));
+                        sum[kb] += (e[0] + e[1]) + (e[2] + e[3]);
                     }
-                    sees &= uint32_t(w);
                 }
             } else {
-                const int nb = i - nj + 1;
-                sees &= nb >= 32 ? ~0u : nb <= 0 ? 0u : (1u << nb) - 1;
-            }
-            const uint32_t bits = sees >> (4 * hf);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], p.scale_log2, nl));
-                sum[v] += ((bits >> (8 * (v >> 2) + (v & 3))) & 1) != 0 ? e : 0.0f;
+                for (int v = 0; v < 16; ++v) {
+                    const int r = 8 * (v >> 2) + 4 * hf + (v & 3);
+                    const float lse = ls[r];
+                    const int tok = sq.skip + PageOf(p.group, min(r0 + r, R - 1));
+                    bool live = r0 + r < R && lse != -INFINITY;
+                    if (!PLAIN && p.path != nullptr) {
+                        const int at = p.path[b * p.ld_path + tok];
+                        live = live && at >= 0 && at < sq.rows;
+                    }
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        const int k = nj + kb * 32 + (lane & 31);  // the key as a new token
+                        bool sees = live && ((there >> kb) & 1) != 0;
+                        if (causal) {
+                            sees = sees && k <= tok;
+                        } else if (sees && k >= 0) {
+                            const uint64_t w = (k >> 6) < p.tree_words
+                                                   ? p.tree[int64_t(sq.first + tok) * p.ld_tree + (k >> 6)]
+                                                   : 0ull;
+                            sees = ((w >> (k & 63)) & 1) != 0;
+                        }
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][v], p.scale_log2, lse * -kLog2E));
+                        sum[kb] += sees ? e : 0.0f;
+                    }
+                }
             }
         }
-        // over the 32 lanes of a half: each step halves the registers, a lane
-        // keeps the half that its bit names
+        // ---- the two halves of a key's rows, and where its sum goes
+        const bool cut = x > pc.start || x + ns < pc.start + pc.rows;
 #pragma unroll
-        for (int m = 8, o = 16; m > 0; m >>= 1, o >>= 1) {
-            const bool up = (lane & o) != 0;
-#pragma unroll
-            for (int v = 0; v < m; ++v) {
-                const float give = up ? sum[v] : sum[v + m], own = up ? sum[v + m] : sum[v];
-                sum[v] = own + __shfl_xor(give, o, 64);
-            }
+        for (int kb = 0; kb < KB; ++kb) {
+            const float got = sum[kb] + __shfl_xor(sum[kb], 32, 64);
+            const int key = j0 + kb * 32 + (lane & 31);
+            if (hf != 0) continue;
+            if (cut) p.parts[(2 * int(blockIdx.x) + (x > pc.start ? 0 : 1)) * kWeighKeys + wave * 32 * KB + kb * 32 + lane] = got;
+            else if (key < sq.cols) PutWeight(p, sq, h, key, got);
         }
-        const float got = sum[0] + __shfl_xor(sum[0], 1, 64);
-        const int v = (lane >> 1) & 15;
-        // bit 16 of the lane chose the registers' bit 3, 8 bit 2, 4 bit 1, 2 bit 0
-        const int key = j0 + 8 * (v >> 2) + 4 * hf + (v & 3);
-        if ((lane & 1) == 0 && key < sq.cols) {
-            float *w = p.w + int64_t(sq.entry) * p.w_entry + int64_t(h) * p.w_head + key;
-            float old = 0.0f;
-            if (key < sq.len && p.decay != 0.0f) old = p.decay * *w;
-            *w = old + got;
-        }
+        x += ns;
     }
 }
+
+// Tiles that came in pieces: workgroup i has the one that begins in part i and
+// ends in a later one, slot 1 of that part and slot 0 of the next.
+__global__ void __launch_bounds__(kWeighKeys) WeighJoinKernel(WeighParams p)
+{
+    const int lane = int(threadIdx.x) & 63;
+    const int total = WeighTotal(p, lane);
+    const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+    const int x0 = int(blockIdx.x) * share, x1 = x0 + share;
+    if (x1 >= total) return;
+    int base;
+    const int b = WeighFind(p, lane, x1 - 1, base);
+    const WeighSeq sq = LoadSeq(p, b);
+    const WeighPiece pc = PieceAt(p, WeighLine(p, sq), b, base, x1 - 1);
+    const int end = pc.start + pc.rows;
+    if (pc.start < x0 || end <= x1) return;
+    const int key = pc.t * kWeighKeys + int(threadIdx.x);
+    if (key >= sq.cols) return;
+    float got = p.parts[(2 * int(blockIdx.x) + 1) * kWeighKeys + int(threadIdx.x)];
+    const int last = (end - 1) / share;
+    for (int i = int(blockIdx.x) + 1; i <= last; ++i) got += p.parts[2 * i * kWeighKeys + int(threadIdx.x)];
+    PutWeight(p, sq, pc.h, key, got);
+}
+
+// Is every tile one row tile, so that none is cut?
+bool OneRowTile(int64_t tokens, int G) { return tokens * G <= 32; }
 
 }  // namespace
 
@@ -233,7 +439,7 @@ void WeighNeeds(const kr_cache *cache, const kr_seqs *seqs, int HQ, size_t *ws_b
     const kr_cache c = CheckCache(cache, who);
     CheckSeqs(seqs, who);
     if (HQ < 1 || HQ % c.heads != 0) throw std::runtime_error(std::string(who) + ": HQ must be a multiple of the cache's heads");
-    *ws_bytes = 0;
+    *ws_bytes = OneRowTile(seqs->max_new, HQ / c.heads) ? 0 : size_t(kWeighParts) * 2 * kWeighKeys * sizeof(float);
 }
 
 void WeighLaunch(const WeighDesc &d, hipStream_t stream)
@@ -303,18 +509,33 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     p.scale_log2 = d.scale * 1.4426950408889634f;
     p.decay = d.decay;
     p.div = MakePageDiv(c.page_size);
-    const int64_t most = (std::min<int64_t>(cap, w.width) + kWeighKeys - 1) / kWeighKeys * c.heads * s.seqs;
-    if (most >= (int64_t(1) << 31)) refuse("too many keys for one launch");
+    p.group = MakePageDiv(p.G);
+    p.parts = static_cast<float *>(d.ws);
+    // the line: at most so many row tiles
+    int64_t tokens = s.max_new;
+    if (d.path != nullptr) tokens = std::min<int64_t>(tokens, d.path_width);
+    if (d.last > 0) tokens = std::min<int64_t>(tokens, d.last);
+    const int64_t tiles = (std::min<int64_t>(cap, w.width) + kWeighKeys - 1) / kWeighKeys;
+    const int64_t most = tiles * c.heads * s.seqs, row_tiles = (tokens * p.G + 31) / 32;
+    if (most >= (int64_t(1) << 31) / row_tiles) refuse("too many rows and keys for one launch");
     const MemSpan out = WeightsSpan(w);
     const RowSpan k = LayerSpan(c, c.k, d.layer);
     if (Meets(out, RowsSpan(d.q, d.rows, p.ldq, int64_t(d.HQ) * c.head_dim, 2)) ||
         Meets(out, RowsSpan(d.lse, d.rows, p.ld_lse, d.HQ, 4)) || Meets(out, MemSpan{k.p, k.width * 2}) ||
         Meets(out, MemSpan{d.ws, int64_t(need)}))
         refuse("the weights overlap another tensor of the call");
-    const dim3 grid(unsigned(std::min<int64_t>(most, kWeighGroups)));
+    const bool one = OneRowTile(tokens, p.G);
+    const dim3 grid(unsigned(one ? std::min<int64_t>(most, kWeighParts) : kWeighParts));
     const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p); };
-    if (c.head_dim == 64) c.dtype == kBF16 ? go(WeighKernel<kBF16, 64>) : go(WeighKernel<kF16, 64>);
-    else c.dtype == kBF16 ? go(WeighKernel<kBF16, 128>) : go(WeighKernel<kF16, 128>);
+    const bool bf = c.dtype == kBF16;
+    if (s.tree == nullptr && d.path == nullptr) {
+        if (c.head_dim == 64) bf ? go(WeighKernel<kBF16, 64, true>) : go(WeighKernel<kF16, 64, true>);
+        else bf ? go(WeighKernel<kBF16, 128, true>) : go(WeighKernel<kF16, 128, true>);
+    } else {
+        if (c.head_dim == 64) bf ? go(WeighKernel<kBF16, 64, false>) : go(WeighKernel<kF16, 64, false>);
+        else bf ? go(WeighKernel<kBF16, 128, false>) : go(WeighKernel<kF16, 128, false>);
+    }
+    if (!one) hipLaunchKernelGGL(WeighJoinKernel, grid, dim3(kWeighKeys), 0, stream, p);
     Check(hipGetLastError(), "attention_paged_weigh launch");
 }
 
