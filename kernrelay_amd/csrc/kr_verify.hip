@@ -11,9 +11,13 @@
 // token's share of the cumulated sum is often below the 2^-24 that 32 bits
 // leave of it.
 //
-// Launches: the largest logit and the sum of each row, in pieces of 8192
-// values; a workgroup for each sequence walks down its drafts; sums of what is
-// left at the row where the walk ended, in the same pieces; and the token.
+// Two launches. The first takes the largest logit and the sum of every row, in
+// pieces of 8192 values; the last workgroup of a sequence to arrive walks down
+// its drafts. In the second a workgroup adds up what is left of 2048 values of a
+// sequence's last row, and the last of them to arrive finds the token: its
+// piece, its thread's eight values, its place. Only where several drafts were
+// drawn after one row does the walk need sums over the vocabulary on its way: it
+// is a launch of its own then, a workgroup a sequence.
 #include <algorithm>
 
 #include "kr_paged.h"
@@ -22,22 +26,24 @@ namespace kr {
 
 namespace {
 
-constexpr int kPiece = 8192;    // values of a piece: 32 a thread
+constexpr int kPiece = 8192;    // values of a piece of a row: 32 a thread
+constexpr int kEndPiece = 2048; // of a sequence's last row: 8 a thread
 constexpr int kMostNew = 1024;  // tokens of a sequence
+// Counters of a sequence, the first of them used: arrivals at one line of memory
+// wait for each other (15 ns each, 32 sequences on a line: 90 us for 53).
+constexpr int kCounters = 32;
+constexpr int kNone = -1;       // the type of draft probabilities that are not there
 
 struct RowPart {
-    float top;  // largest logit of the piece
-    int at;     // its first place
-    double sum; // of exp((x - top) / t)
+    float top;   // largest logit
+    int at;      // its first place
+    double sum;  // of exp((x - top) / t)
 };
 struct SeqEnd {
-    int row;      // where the walk ended: a row of the launch, -1: the sequence has none
+    int row;      // where the walk ended: a row of the sequence
     int refused;  // drafts that were refused there
+    RowPart stats;
 };
-struct LeftPart {
-    double left, was;  // sums of p after and before the last refusal
-};
-
 struct VerifyParams {
     const void *logits, *draft;
     const int64_t *tokens;
@@ -46,13 +52,14 @@ struct VerifyParams {
     int32_t *path, *path_lens;
     int64_t *next;
     int64_t ld_logits, ld_draft, ld_path;
-    int dtype, draft_dtype, vocab, rows, seqs, max_new, width, pieces;
-    bool wide, draft_wide;  // rows are 16-byte aligned
+    int vocab, rows, seqs, max_new, width, pieces, end_pieces;
     RowPart *parts;         // [rows, pieces]
-    RowPart *stats;         // [rows]
     double *totals;         // [rows]: of a sequence's end row, the sums after its refusals
+    int32_t *refused;       // [rows]: the tokens refused there
     SeqEnd *ends;           // [seqs]
-    LeftPart *lefts;        // [seqs, pieces]
+    double *sums;           // [seqs, end_pieces]: of what is left at the end row
+    double *sums8;          // [seqs, end_pieces, 256]: of 8 values each
+    int32_t *cnt;           // [seqs, kCounters]: arrivals, zero between launches
 };
 
 struct VerifySeq {
@@ -67,58 +74,113 @@ __device__ __forceinline__ VerifySeq LoadSeq(const VerifyParams &p, int b)
     return s;
 }
 
-// -1 for a temperature that picks the first of the largest.
-__device__ __forceinline__ double InvTemperature(const VerifyParams &p, int b)
+// log2(e) / t; -1 for a temperature that picks the first of the largest.
+__device__ __forceinline__ double Slope(float t) { return t > 0.0f ? 1.4426950408889634 / double(t) : -1.0; }
+__device__ __forceinline__ double SlopeOf(const VerifyParams &p, int b)
 {
-    if (p.temperature == nullptr) return 1.0;
-    const float t = p.temperature[b];
-    return t > 0.0f ? 1.0 / double(t) : -1.0;
+    return Slope(p.temperature != nullptr ? p.temperature[b] : 1.0f);
 }
 
-__device__ __forceinline__ float LoadAny(const void *base, int dtype, int64_t at)
+template <int DT> struct Val {
+    typedef uint16_t T;
+    static constexpr T kLow = DT == kBF16 ? 0xff80 : 0xfc00;  // -infinity
+    __device__ static float Load(T x) { return Elem<DT>::Load(x); }
+};
+template <> struct Val<kF32> {
+    typedef float T;
+    static constexpr T kLow = -INFINITY;
+    __device__ static float Load(T x) { return x; }
+};
+
+template <int DT>
+__device__ __forceinline__ float At(const void *base, int64_t at)
 {
-    if (dtype == kF32) return static_cast<const float *>(base)[at];
-    const uint16_t x = static_cast<const uint16_t *>(base)[at];
-    return dtype == kBF16 ? BF16ToF32(x) : F16ToF32(x);
+    typedef typename Val<DT>::T T;
+    return Val<DT>::Load(static_cast<const T *>(base)[at]);
 }
 
-// Values at .. at + 7 of a row of n; past its end `none`.
-__device__ __forceinline__ void Load8(const void *row, int dtype, bool wide, int at, int n, float none, float (&x)[8])
+// Eight values at `at` of a row of n, as they are; past its end `none`. A row may
+// begin anywhere: the loads are 16 bytes wide and as aligned as the values.
+template <int DT> struct Raw8 {
+    typename Val<DT>::T v[8];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> Load8(const void *base, int64_t row, int at, int n, typename Val<DT>::T none)
 {
-    if (wide && at + 8 <= n) {
-        if (dtype == kF32) {
-            const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(row) + at);
-            const float4 c = *reinterpret_cast<const float4 *>(static_cast<const float *>(row) + at + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-            x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-        } else {
-            const U16x8 v = LoadU16x8(static_cast<const uint16_t *>(row) + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = dtype == kBF16 ? BF16ToF32(v.v[e]) : F16ToF32(v.v[e]);
-        }
+    typedef typename Val<DT>::T T;
+    const T *p = static_cast<const T *>(base) + row + at;
+    Raw8<DT> r;
+    if (at + 8 <= n) {
+        __builtin_memcpy(&r, p, sizeof(r));
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = at + e < n ? LoadAny(row, dtype, at + e) : none;
+        for (int e = 0; e < 8; ++e) r.v[e] = at + e < n ? p[e] : none;
     }
-}
-
-__device__ __forceinline__ const void *RowOf(const void *base, int dtype, int64_t at)
-{
-    return static_cast<const char *>(base) + at * (dtype == kF32 ? 4 : 2);
+    return r;
 }
 
 __device__ __forceinline__ float Logit(float x) { return x != x ? -INFINITY : x; }
-__device__ __forceinline__ float Chance(float q) { return q > 0.0f ? q : 0.0f; }
+__device__ __forceinline__ double Chance(float q) { return q > 0.0f ? double(q) : 0.0; }
 
-// exp((x - top) / t), 1 at the top itself, also an infinite one; without a
-// temperature 1 at place `at` alone. (Differences of infinities and their
-// products with 1 / t = 0 are no numbers.)
-__device__ __forceinline__ double Weight(float x, int i, float top, int at, double inv_t)
+// 2^z for -1000 <= z <= 0, within 2^-44 of it: z = m / 64 + f with |f| <= 1/128,
+// m from the last bits of a sum with 1.5 2^52; 2^f by its series to f^4 (the
+// first term left out is below 2^-44), 2^(m % 64 / 64) from a table in LDS and
+// the rest by the exponent's bits. 17 operations at the full rate with the
+// difference and product that make z, where the series alone took 30, and the
+// library's exp three times that.
+constexpr int kTable = 64;
+struct Pow2 {
+    double of[kTable];
+    // all threads of the workgroup (at least 64); a barrier follows before its use
+    __device__ __forceinline__ void Fill()
+    {
+        if (threadIdx.x >= kTable) return;
+        // sqrt(2) exp(r), r = (j - 32) ln(2) / 64
+        const double r = double(int(threadIdx.x) - kTable / 2) * (0x1.62e42fefa39efp-1 / kTable);
+        double e = 1.0 / 479001600.0;
+        e = __builtin_fma(e, r, 1.0 / 39916800.0);
+        e = __builtin_fma(e, r, 1.0 / 3628800.0);
+        e = __builtin_fma(e, r, 1.0 / 362880.0);
+        e = __builtin_fma(e, r, 1.0 / 40320.0);
+        e = __builtin_fma(e, r, 1.0 / 5040.0);
+        e = __builtin_fma(e, r, 1.0 / 720.0);
+        e = __builtin_fma(e, r, 1.0 / 120.0);
+        e = __builtin_fma(e, r, 1.0 / 24.0);
+        e = __builtin_fma(e, r, 1.0 / 6.0);
+        e = __builtin_fma(e, r, 0.5);
+        e = __builtin_fma(e, r, 1.0);
+        e = __builtin_fma(e, r, 1.0);
+        of[threadIdx.x] = e * 1.4142135623730951;
+    }
+    __device__ __forceinline__ double operator()(double z) const
+    {
+        // (three-address sums, the constants in registers: the compiler would
+        // move each constant into the sum's own register first)
+        double t, s;
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(t) : "v"(z), "v"(double(kTable)), "v"(0x1.8p52));
+        const double f = __builtin_fma(t - 0x1.8p52, -1.0 / kTable, z);
+        const int m = __double2loint(t);
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(s) : "v"(f), "v"(0.009618129107628477),  // ln(2)^4 / 24
+            "v"(0.05550410866482158));                                                        // ln(2)^3 / 6
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(s) : "v"(s), "v"(f), "v"(0.2402265069591007));  // ln(2)^2 / 2
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(s) : "v"(s), "v"(f), "v"(0.6931471805599453));
+        const double b = of[m & (kTable - 1)];
+        const double w = __builtin_fma(b, s * f, b);
+        return __hiloint2double(__double2hiint(w) + ((m & -kTable) << 14), __double2loint(w));
+    }
+};
+
+constexpr double kFar = -1000.0;  // log2 of a weight that is 0
+
+// exp((x - top) / t), c = log2(e) / t: 1 at the top itself, also an infinite
+// one; without a temperature (c < 0) 1 at place `at` alone. (Differences of
+// infinities and their products with c = 0 are no numbers.)
+__device__ __forceinline__ double Weight(const Pow2 &pow2, float x, int i, float top, int at, double c)
 {
-    if (inv_t < 0.0) return i == at ? 1.0 : 0.0;
-    if (x == -INFINITY) return 0.0;
-    if (x == top) return 1.0;
-    return top == INFINITY ? 0.0 : exp((double(x) - double(top)) * inv_t);
+    if (c < 0.0) return i == at ? 1.0 : 0.0;
+    const double z = (double(x) - double(top)) * c;
+    const double w = pow2(fmax(z, kFar));
+    return x == top && x != -INFINITY ? 1.0 : x == -INFINITY || top == INFINITY || z < kFar ? 0.0 : w;
 }
 
 __device__ __forceinline__ double WaveSumD(double v)
@@ -128,76 +190,53 @@ __device__ __forceinline__ double WaveSumD(double v)
     return v;
 }
 
-// Sum over the 256 threads, in every one of them.
+// Sum over the NT threads, in every one of them.
+template <int NT>
 __device__ __forceinline__ double BlockSumD(double v, double *part)
 {
     v = WaveSumD(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (part[0] + part[1]) + (part[2] + part[3]);
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) s += part[i];
+    return s;
 }
 
-__global__ void __launch_bounds__(256) StatsKernel(VerifyParams p)
+// 8 bytes to and from other workgroups of the running launch.
+__device__ __forceinline__ void PutDev(double *p, double v)
 {
-    __shared__ float top_of[4];
-    __shared__ int at_of[4];
-    __shared__ double part[4];
-    const int piece = int(blockIdx.x) % p.pieces, row = int(blockIdx.x) / p.pieces;
-    const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
-    int b = -1;
-    for (int b0 = 0; b0 < p.seqs && b < 0; b0 += 64) {
-        bool mine = false;
-        if (b0 + lane < p.seqs) {
-            const VerifySeq s = LoadSeq(p, b0 + lane);
-            mine = row >= s.first && row < s.first + s.n;
-        }
-        const uint64_t hit = __ballot(mine);
-        if (hit != 0) b = b0 + __builtin_ctzll(hit);
-    }
-    if (b < 0) return;  // a row of no sequence
-    const double inv_t = InvTemperature(p, b);
-    const void *x_row = RowOf(p.logits, p.dtype, int64_t(row) * p.ld_logits);
-    float x[32];
-    const int i0 = piece * kPiece + int(threadIdx.x) * 8;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        float y[8];
-        Load8(x_row, p.dtype, p.wide, i0 + g * 2048, p.vocab, -INFINITY, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[g * 8 + e] = Logit(y[e]);
-    }
-    float top = x[0];
-#pragma unroll
-    for (int e = 1; e < 32; ++e) top = fmaxf(top, x[e]);
-    top = WaveMax(top);
-    if (lane == 0) top_of[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
-    int at = INT32_MAX;
-    double sum = 0.0;
-#pragma unroll
-    for (int g = 3; g >= 0; --g)
-#pragma unroll
-        for (int e = 7; e >= 0; --e) {
-            if (x[g * 8 + e] == top) at = i0 + g * 2048 + e;
-            if (inv_t >= 0.0) sum += Weight(x[g * 8 + e], 0, top, 0, inv_t);
-        }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
-    if (lane == 0) at_of[wave] = at;
-    sum = BlockSumD(sum, part);
-    if (threadIdx.x == 0) {
-        RowPart r;
-        r.top = top;
-        r.at = min(min(at_of[0], at_of[1]), min(at_of[2], at_of[3]));
-        r.sum = inv_t < 0.0 ? 1.0 : sum;
-        p.parts[int64_t(row) * p.pieces + piece] = r;
-    }
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double GetDev(const double *p)
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// What is left of value i's probability after `refused` refusals at a row with
-// draft probabilities q: `totals` are the sums after each, the last one not
+__device__ __forceinline__ void PutPart(RowPart *p, const RowPart &x)
+{
+    const uint64_t head = uint64_t(__float_as_uint(x.top)) | (uint64_t(uint32_t(x.at)) << 32);
+    PutDev(reinterpret_cast<double *>(p), __builtin_bit_cast(double, head));
+    PutDev(&p->sum, x.sum);
+}
+__device__ __forceinline__ RowPart GetPart(const RowPart *p)
+{
+    const uint64_t head = __builtin_bit_cast(uint64_t, GetDev(reinterpret_cast<const double *>(p)));
+    return RowPart{__uint_as_float(uint32_t(head)), int(head >> 32), GetDev(&p->sum)};
+}
+// One more of `all` arrivals, by one thread; is it the last? The counter is
+// zero again then.
+__device__ __forceinline__ bool Arrive(int32_t *cnt, int all)
+{
+    const bool last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+    if (last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return last;
+}
+
+// ---------------------------------------------------------------- the walk
+// What is left of a value's probability w after `refused` refusals at a row
+// with draft probability q: `totals` are the sums after each, the last one not
 // needed. was: before the last refusal.
 __device__ __forceinline__ double Left(double w, double q, const double *totals, int refused, double &was)
 {
@@ -214,127 +253,131 @@ __device__ __forceinline__ double Left(double w, double q, const double *totals,
     return r;
 }
 
-__global__ void __launch_bounds__(256) WalkKernel(VerifyParams p)
+// Of a sequence's rows, in LDS that the launch sizes by max_new.
+struct WalkLds {
+    RowPart *stats;
+    double *prob;    // of draft i at the row that it follows, before any refusal
+    double *totals;  // at the row where the walk is, after each refusal
+    float *chance, *u;
+    int *above, *token;
+    static constexpr int kBytes = sizeof(RowPart) + 2 * sizeof(double) + 4 * 4;
+    __device__ __forceinline__ WalkLds(char *lds, int n)
+    {
+        stats = reinterpret_cast<RowPart *>(lds);
+        prob = reinterpret_cast<double *>(stats + n);
+        totals = prob + n;
+        chance = reinterpret_cast<float *>(totals + n);
+        u = chance + n;
+        above = reinterpret_cast<int *>(u + n);
+        token = above + n;
+    }
+};
+
+// Down the drafts of sequence b, by NT threads that all take the same steps.
+// SUMS: several drafts after one row may have been drawn, so that a refusal's
+// sum over the vocabulary may be needed.
+template <int XT, int QT, int NT, bool SUMS>
+__device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifySeq &sq, double c, const Pow2 &pow2,
+                                       const WalkLds &l, double *part)
 {
-    __shared__ double prob[kMostNew];      // of draft i at the row that it follows, before any refusal
-    __shared__ double totals[kMostNew];
-    __shared__ RowPart stats[kMostNew];
-    __shared__ float chance[kMostNew], u[kMostNew];
-    __shared__ int above[kMostNew], token[kMostNew];
-    __shared__ double part[4];
-    const int b = int(blockIdx.x), tid = int(threadIdx.x), lane = tid & 63;
-    const VerifySeq sq = LoadSeq(p, b);
-    const double inv_t = InvTemperature(p, b);
-    for (int i = tid; i < p.width; i += 256) p.path[b * p.ld_path + i] = i == 0 && sq.n > 0 ? 0 : -1;
-    if (sq.n == 0) {
-        if (tid == 0) {
-            p.path_lens[b] = 0;
-            p.ends[b] = SeqEnd{-1, 0};
-        }
-        return;
-    }
-    // ---- rows: their pieces put together, eight lanes to a row
-    for (int r0 = 0; r0 < sq.n; r0 += 32) {
-        const int r = r0 + tid / 8, l8 = tid % 8;
-        const RowPart *parts = p.parts + int64_t(sq.first + min(r, sq.n - 1)) * p.pieces;
-        float top = -INFINITY;
-        for (int c = l8; c < p.pieces; c += 8) top = fmaxf(top, parts[c].top);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        int at = INT32_MAX;
-        double sum = 0.0;
-        for (int c = l8; c < p.pieces; c += 8) {
-            const RowPart x = parts[c];
-            if (x.top == top) at = min(at, x.at);
-            if (inv_t >= 0.0) sum += x.sum * Weight(x.top, 0, top, 0, inv_t);
-        }
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            at = min(at, __shfl_xor(at, o, 64));
-            sum += __shfl_xor(sum, o, 64);
-        }
-        if (l8 == 0 && r < sq.n) {
-            RowPart x;
-            x.top = top;
-            x.at = at;
-            x.sum = inv_t < 0.0 ? 1.0 : sum;
-            stats[r] = x;
-            p.stats[sq.first + r] = x;
-        }
-    }
-    // ---- drafts: what they follow and how likely they are there
-    for (int i = tid; i < sq.n; i += 256) {
+    const int tid = int(threadIdx.x), lane = tid & 63;
+    // ---- drafts: what they follow
+    for (int i = tid; i < sq.n; i += NT) {
         const int64_t tok = p.tokens[sq.first + i];
         const int par = p.parents != nullptr ? p.parents[sq.first + i] : i - 1;
-        above[i] = i > 0 && par >= 0 && par < i ? par : -1;
-        token[i] = tok >= 0 && tok < p.vocab ? int(tok) : -1;
-        u[i] = p.u[sq.first + i];
+        l.above[i] = i > 0 && par >= 0 && par < i ? par : -1;
+        l.token[i] = tok >= 0 && tok < p.vocab ? int(tok) : -1;
+        l.u[i] = p.u[sq.first + i];
+    }
+    // ---- rows: their pieces put together, eight lanes to a row
+    for (int r0 = 0; r0 < sq.n; r0 += NT / 8) {
+        const int r = r0 + tid / 8, l8 = tid % 8;
+        const RowPart *parts = p.parts + int64_t(sq.first + min(r, sq.n - 1)) * p.pieces;
+        RowPart x{-INFINITY, INT32_MAX, 0.0};
+        const auto add = [&](const RowPart &y) {
+            // (a part of no logits adds nothing; of two infinite tops both count)
+            const float top = fmaxf(x.top, y.top);
+            const int ax = x.top == top ? x.at : INT32_MAX, ay = y.top == top ? y.at : INT32_MAX;
+            if (c < 0.0) x.sum = 1.0;
+            else x.sum = x.sum * Weight(pow2, x.top, 0, top, 0, c) + y.sum * Weight(pow2, y.top, 0, top, 0, c);
+            x.top = top;
+            x.at = min(ax, ay);
+        };
+        for (int k = l8; k < p.pieces; k += 8) add(GetPart(parts + k));
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            RowPart y;
+            y.top = __shfl_xor(x.top, o, 64);
+            y.at = __shfl_xor(x.at, o, 64);
+            y.sum = __shfl_xor(x.sum, o, 64);
+            add(y);
+        }
+        if (l8 == 0 && r < sq.n) l.stats[r] = x;
     }
     __syncthreads();
-    for (int i = tid; i < sq.n; i += 256) {
-        const int par = above[i], tok = token[i];
+    // ---- and how likely they are there
+    for (int i = tid; i < sq.n; i += NT) {
+        const int par = l.above[i], tok = l.token[i];
         double w = 0.0;
         float q = 1.0f;
         if (par >= 0 && tok >= 0) {
-            const RowPart s = stats[par];
+            const RowPart s = l.stats[par];
             const int64_t row = sq.first + par;
-            const float x = Logit(LoadAny(p.logits, p.dtype, row * p.ld_logits + tok));
-            if (s.top != -INFINITY) w = Weight(x, tok, s.top, s.at, inv_t) / s.sum;
-            if (p.draft != nullptr) {
-                q = Chance(LoadAny(p.draft, p.draft_dtype, row * p.ld_draft + tok));
-            } else {
+            const float x = Logit(At<XT>(p.logits, row * p.ld_logits + tok));
+            if (QT != kNone) q = float(Chance(At<QT == kNone ? kF32 : QT>(p.draft, row * p.ld_draft + tok)));
+            if (s.top != -INFINITY) w = Weight(pow2, x, tok, s.top, s.at, c) / s.sum;
+            if (QT == kNone) {
                 // a token that was refused there already has nothing left
                 for (int j = par + 1; j < i; ++j)
-                    if (above[j] == par && token[j] == tok) w = 0.0;
+                    if (l.above[j] == par && l.token[j] == tok) w = 0.0;
             }
         }
-        prob[i] = w;
-        chance[i] = q;
+        l.prob[i] = w;
+        l.chance[i] = q;
     }
     __syncthreads();
-    // ---- down the drafts; every thread takes the same steps
     int cur = 0, len = 1, refused = 0;
     while (len < p.width) {
         refused = 0;
         double rest = 1.0;  // (drafts that were not drawn)
         int next = -1;
         for (int i0 = (cur + 1) / 64 * 64; i0 < sq.n && next < 0; i0 += 64) {
-            uint64_t hit = __ballot(i0 + lane < sq.n && i0 + lane > cur && above[min(i0 + lane, sq.n - 1)] == cur);
+            uint64_t hit = __ballot(i0 + lane < sq.n && i0 + lane > cur && l.above[min(i0 + lane, sq.n - 1)] == cur);
             while (hit != 0 && next < 0) {
                 const int i = Uni(i0 + __builtin_ctzll(hit));
                 hit &= hit - 1;
                 bool ok;
-                if (p.draft == nullptr) {
-                    ok = double(u[i]) * rest < prob[i];
-                    rest = fmax(rest - prob[i], 0.0);
+                if (QT == kNone) {
+                    ok = double(l.u[i]) * rest < l.prob[i];
+                    rest = fmax(rest - l.prob[i], 0.0);
                 } else {
-                    if (refused > 0) {
+                    if (SUMS && refused > 0) {
                         // the sum after the last refusal, over the vocabulary
-                        const RowPart s = stats[cur];
+                        const RowPart s = l.stats[cur];
                         const int64_t row = sq.first + cur;
-                        const void *xr = RowOf(p.logits, p.dtype, row * p.ld_logits);
-                        const void *qr = RowOf(p.draft, p.draft_dtype, row * p.ld_draft);
+                        const double inv = 1.0 / s.sum;
                         double sum = 0.0;
-                        for (int v = tid * 8; v < p.vocab; v += 2048) {
-                            float x[8], q[8];
-                            Load8(xr, p.dtype, p.wide, v, p.vocab, -INFINITY, x);
-                            Load8(qr, p.draft_dtype, p.draft_wide, v, p.vocab, 0.0f, q);
+                        for (int v = tid * 8; v < p.vocab; v += NT * 8) {
+                            const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
+                            const Raw8<QT == kNone ? kF32 : QT> q =
+                                Load8<QT == kNone ? kF32 : QT>(p.draft, row * p.ld_draft, v, p.vocab, 0);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
+                                if (s.top == -INFINITY) continue;
                                 double was;
-                                if (s.top != -INFINITY)
-                                    sum += Left(Weight(Logit(x[e]), v + e, s.top, s.at, inv_t) / s.sum, Chance(q[e]),
-                                                totals, refused, was);
+                                const double w =
+                                    Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, s.top, s.at, c) * inv;
+                                sum += Left(w, Chance(Val<QT == kNone ? kF32 : QT>::Load(q.v[e])), l.totals, refused, was);
                             }
                         }
-                        sum = BlockSumD(sum, part);
-                        if (tid == 0) totals[refused - 1] = sum;
+                        sum = BlockSumD<NT>(sum, part);
+                        if (tid == 0) l.totals[refused - 1] = sum;
                         __syncthreads();
                     }
-                    double r = prob[i];
-                    for (int k = 0; k < refused; ++k)
-                        r = totals[k] > 0.0 ? fmax(r - double(chance[i]), 0.0) / totals[k] : r;
-                    ok = double(u[i]) * double(chance[i]) < r;
+                    double r = l.prob[i];
+                    for (int k = 0; SUMS && k < refused; ++k)
+                        r = l.totals[k] > 0.0 ? fmax(r - double(l.chance[i]), 0.0) / l.totals[k] : r;
+                    ok = double(l.u[i]) * double(l.chance[i]) < r;
                 }
                 if (ok) next = i;
                 else ++refused;
@@ -347,183 +390,321 @@ __global__ void __launch_bounds__(256) WalkKernel(VerifyParams p)
         ++len;
     }
     if (tid == 0) {
+        p.path[b * p.ld_path] = 0;
         p.path_lens[b] = len;
-        p.ends[b] = SeqEnd{sq.first + cur, refused};
+        p.ends[b] = SeqEnd{cur, refused, l.stats[cur]};
     }
-    if (p.draft != nullptr)
-        for (int k = tid; k + 1 < refused; k += 256) p.totals[sq.first + k] = totals[k];
-}
-
-// What is left of the end row's values i .. i + 7 of a thread, before and after the last refusal.
-struct EndRow {
-    const void *x, *q;
-    RowPart s;
-    const double *totals;
-    double inv_t;
-    int refused, row;
-};
-
-__device__ __forceinline__ EndRow LoadEnd(const VerifyParams &p, int b, const SeqEnd &e)
-{
-    EndRow r;
-    r.row = e.row;
-    r.refused = e.refused;
-    r.s = p.stats[e.row];
-    r.inv_t = InvTemperature(p, b);
-    r.x = RowOf(p.logits, p.dtype, int64_t(e.row) * p.ld_logits);
-    r.q = p.draft != nullptr ? RowOf(p.draft, p.draft_dtype, int64_t(e.row) * p.ld_draft) : nullptr;
-    r.totals = p.totals + LoadSeq(p, b).first;
-    return r;
-}
-
-// Marks the tokens of a piece that were refused at the end row (drafts that were not drawn).
-__device__ __forceinline__ void MarkRefused(const VerifyParams &p, int b, const EndRow &r, int v0, uint32_t *marks)
-{
-    for (int i = int(threadIdx.x); i < kPiece / 32; i += 256) marks[i] = 0;
-    __syncthreads();
-    if (p.draft == nullptr && r.refused > 0) {
-        const VerifySeq sq = LoadSeq(p, b);
-        for (int i = int(threadIdx.x); i < sq.n; i += 256) {
-            const int par = p.parents != nullptr ? p.parents[sq.first + i] : i - 1;
-            const int64_t tok = p.tokens[sq.first + i] - v0;
-            if (i > 0 && par >= 0 && par < i && sq.first + par == r.row && tok >= 0 && tok < kPiece)
-                atomicOr(&marks[tok >> 5], 1u << (tok & 31));
-        }
-    }
-    __syncthreads();
-}
-
-__device__ __forceinline__ void Left8(const VerifyParams &p, const EndRow &r, int v, int v0, const uint32_t *marks,
-                                      double (&left)[8], double (&was)[8])
-{
-    float x[8], q[8];
-    Load8(r.x, p.dtype, p.wide, v, p.vocab, -INFINITY, x);
-    if (p.draft != nullptr && r.refused > 0) Load8(r.q, p.draft_dtype, p.draft_wide, v, p.vocab, 0.0f, q);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const double w = r.s.top == -INFINITY || v + e >= p.vocab ? 0.0 : Weight(Logit(x[e]), v + e, r.s.top, r.s.at, r.inv_t);
-        if (p.draft != nullptr) {
-            left[e] = Left(w / r.s.sum, r.refused > 0 ? double(Chance(q[e])) : 0.0, r.totals, r.refused, was[e]);
-        } else {
-            was[e] = w;
-            left[e] = ((marks[(v + e - v0) >> 5] >> ((v + e - v0) & 31)) & 1) != 0 ? 0.0 : w;
+    for (int i = len + tid; i < p.width; i += NT) p.path[b * p.ld_path + i] = -1;
+    if (QT != kNone) {
+        for (int k = tid; SUMS && k + 1 < refused; k += NT) p.totals[sq.first + k] = l.totals[k];
+    } else if (refused > 0 && tid < 64) {  // (all that follow it)
+        int at = 0;
+        for (int i0 = (cur + 1) / 64 * 64; i0 < sq.n; i0 += 64) {
+            const int i = min(i0 + lane, sq.n - 1);
+            const bool is = i0 + lane < sq.n && i0 + lane > cur && l.above[i] == cur;
+            const uint64_t hit = __ballot(is);
+            if (is) p.refused[sq.first + at + __popcll(hit & ((1ull << lane) - 1))] = l.token[i];
+            at += __popcll(hit);
         }
     }
 }
 
-__global__ void __launch_bounds__(256) LeftKernel(VerifyParams p)
+__device__ __forceinline__ void NoRows(const VerifyParams &p, int b, int nt)
 {
-    __shared__ uint32_t marks[kPiece / 32];
+    for (int i = int(threadIdx.x); i < p.width; i += nt) p.path[b * p.ld_path + i] = -1;
+    if (threadIdx.x == 0) {
+        p.path_lens[b] = 0;
+        p.next[b] = -1;
+    }
+}
+
+// Sampled trees: the walk by itself. 1024 threads, as the sums over the
+// vocabulary are made by one workgroup.
+template <int XT, int QT>
+__global__ void __launch_bounds__(1024) WalkKernel(VerifyParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ Pow2 pow2;
+    __shared__ double part[16];
+    const int b = int(blockIdx.x);
+    const VerifySeq sq = LoadSeq(p, b);
+    if (sq.n == 0) return;  // (the next launch says so)
+    const double c = SlopeOf(p, b);
+    pow2.Fill();
+    __syncthreads();
+    Walk<XT, QT, 1024, true>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
+}
+
+// ---------------------------------------------------------------- rows
+// WALK: the last workgroup of a sequence walks.
+template <int XT, int QT, bool WALK>
+__global__ void __launch_bounds__(256) StatsKernel(VerifyParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int last;
+    __shared__ Pow2 pow2;
+    __shared__ float top_of[4];
+    __shared__ int at_of[4];
     __shared__ double part[4];
-    const int piece = int(blockIdx.x) % p.pieces, b = int(blockIdx.x) / p.pieces;
-    const SeqEnd end = p.ends[b];
-    if (end.row < 0) return;
-    const EndRow r = LoadEnd(p, b, end);
-    const int v0 = piece * kPiece;
-    MarkRefused(p, b, r, v0, marks);
-    double left = 0.0, was = 0.0;
-#pragma unroll 1
-    for (int g = 0; g < 4; ++g) {
-        double l8[8], w8[8];
-        Left8(p, r, v0 + g * 2048 + int(threadIdx.x) * 8, v0, marks, l8, w8);
+    const int piece = int(blockIdx.x) % p.pieces, row = int(blockIdx.x) / p.pieces;
+    const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
+    const int i0 = piece * kPiece + int(threadIdx.x) * 8;
+    Raw8<XT> raw[4];  // (on their way while the row's sequence is looked up)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            left += l8[e];
-            was += w8[e];
+    for (int g = 0; g < 4; ++g) raw[g] = Load8<XT>(p.logits, int64_t(row) * p.ld_logits, i0 + g * 2048, p.vocab, Val<XT>::kLow);
+    pow2.Fill();
+    int b = -1;
+    VerifySeq sq{0, 0};
+    float t = 1.0f;
+    for (int b0 = 0; b0 < p.seqs && b < 0; b0 += 64) {
+        bool mine = false;
+        float tb = 1.0f;
+        VerifySeq s{0, 0};
+        if (b0 + lane < p.seqs) {
+            if (p.temperature != nullptr) tb = p.temperature[b0 + lane];
+            s = LoadSeq(p, b0 + lane);
+            mine = row >= s.first && row < s.first + s.n;
+        }
+        const uint64_t hit = __ballot(mine);
+        if (hit != 0) {
+            const int at = __builtin_ctzll(hit);
+            b = b0 + at;
+            t = __shfl(tb, at, 64);
+            sq.first = Uni(__shfl(s.first, at, 64));
+            sq.n = Uni(__shfl(s.n, at, 64));
         }
     }
-    left = BlockSumD(left, part);
-    was = BlockSumD(was, part);
-    if (threadIdx.x == 0) p.lefts[int64_t(b) * p.pieces + piece] = LeftPart{left, was};
+    if (b < 0) return;  // a row of no sequence
+    const double c = Slope(t);
+    float x[32];
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[g * 8 + e] = Val<XT>::Load(raw[g].v[e]);
+            top = fmaxf(top, x[g * 8 + e]);  // (passes a NaN by)
+        }
+    top = WaveMax(top);
+    if (lane == 0) top_of[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+    int at = INT32_MAX;
+    double sum = 1.0;
+    if (c < 0.0) {
+#pragma unroll
+        for (int g = 3; g >= 0; --g)
+#pragma unroll
+            for (int e = 7; e >= 0; --e)
+                if (x[g * 8 + e] == top) at = i0 + g * 2048 + e;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+        if (lane == 0) at_of[wave] = at;
+        __syncthreads();
+        at = min(min(at_of[0], at_of[1]), min(at_of[2], at_of[3]));
+    } else {
+        double s[2] = {0.0, 0.0};
+        if (top == INFINITY) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e & 1] += x[e] == top ? 1.0 : 0.0;
+        } else if (top != -INFINITY) {
+            // (weights below 2^-1000 count as that, nothing beside the top's 1;
+            // so do NaNs and -infinity times a slope of 0: fmax passes a NaN by)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e & 1] += pow2(fmax((double(x[e]) - double(top)) * c, kFar));
+        }
+        sum = BlockSumD<256>(s[0] + s[1], part);
+    }
+    if constexpr (!WALK) {
+        if (threadIdx.x == 0) p.parts[int64_t(row) * p.pieces + piece] = RowPart{top, at, sum};
+    } else {
+        if (threadIdx.x == 0) {
+            PutPart(&p.parts[int64_t(row) * p.pieces + piece], RowPart{top, at, sum});
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
+            last = Arrive(p.cnt + b * kCounters, sq.n * p.pieces);
+        }
+        __syncthreads();
+        if (!last) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        Walk<XT, QT, 256, false>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
+    }
 }
 
-__global__ void __launch_bounds__(256) NextKernel(VerifyParams p)
+// ---------------------------------------------------------------- the token
+// The first thread (of 256, in order) whose inclusive sum, from `base` on, is
+// over the bar, else the last one with anything; -1 if none has. `before`: the
+// sum ahead of it.
+struct Pick {
+    int at;
+    double before;
+    bool over;
+};
+__device__ __forceinline__ Pick PickThread(double v, double base, double bar, double *part, int *pick, double *ahead)
 {
-    __shared__ uint32_t marks[kPiece / 32];
-    __shared__ double wave_sum[4];
-    const int b = int(blockIdx.x), tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const SeqEnd end = p.ends[b];
-    if (end.row < 0) {
-        if (tid == 0) p.next[b] = -1;
-        return;
-    }
-    const EndRow r = LoadEnd(p, b, end);
-    // ---- the piece: every thread adds up the pieces in order
-    const LeftPart *lefts = p.lefts + int64_t(b) * p.pieces;
-    double left = 0.0, was = 0.0;
-    for (int c = 0; c < p.pieces; ++c) {
-        left += lefts[c].left;
-        was += lefts[c].was;
-    }
-    const bool stays = !(left > 0.0);  // nothing left: p as it was
-    const double total = stays ? was : left;
-    if (!(total > 0.0)) {
-        if (tid == 0) p.next[b] = -1;
-        return;
-    }
-    const double bar = double(p.u_next[b]) * total;
-    double base = 0.0, sum = 0.0;
-    int piece = -1;
-    for (int c = 0; c < p.pieces; ++c) {
-        const double x = stays ? lefts[c].was : lefts[c].left;
-        if (x > 0.0) {
-            piece = c;
-            base = sum;
-            if (sum + x > bar) break;
-        }
-        sum += x;
-    }
-    // ---- the value: thread t has 32 in a row
-    const int v0 = piece * kPiece, i0 = tid * 32;
-    MarkRefused(p, b, r, v0, marks);
-    double mine[32], own = 0.0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        double l8[8], w8[8];
-        Left8(p, r, v0 + i0 + g * 8, v0, marks, l8, w8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            mine[g * 8 + e] = stays ? w8[e] : l8[e];
-            own += mine[g * 8 + e];
-        }
-    }
-    double incl = own;
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    double incl = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const double x = __shfl_up(incl, o, 64);
         if (lane >= o) incl += x;
     }
-    if (lane == 63) wave_sum[wave] = incl;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) base += wave_sum[i];
-    double at = base + (incl - own);
-    int hit = INT32_MAX, tail = -1;
+    if (lane == 63) part[wave] = incl;
+    if (tid < 8) pick[tid] = -1;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) base += part[i];
+    const double excl = base + (incl - v);
+    const uint64_t over = __ballot(v > 0.0 && base + incl > bar), some = __ballot(v > 0.0);
+    // slots 0..3: a wave's first over the bar; 4..7: its last with anything
+    if (over != 0 && lane == __builtin_ctzll(over)) pick[wave] = tid, ahead[wave] = excl;
+    if (some != 0 && lane == 63 - __builtin_clzll(some)) pick[4 + wave] = tid, ahead[4 + wave] = excl;
+    __syncthreads();
+    Pick r{-1, 0.0, false};
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        at += mine[e];
-        if (mine[e] > 0.0) {
-            if (hit == INT32_MAX && at > bar) hit = v0 + i0 + e;
-            tail = v0 + i0 + e;
+    for (int i = 4; i < 8; ++i)
+        if (pick[i] >= 0) r = Pick{pick[i], ahead[i], false};
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+        if (pick[i] >= 0) r = Pick{pick[i], ahead[i], true};
+    return r;
+}
+
+template <int XT, int QT>
+__global__ void __launch_bounds__(256) NextKernel(VerifyParams p)
+{
+    __shared__ Pow2 pow2;
+    __shared__ uint32_t marks[kEndPiece / 32];  // refused tokens of a piece (drafts that were not drawn)
+    __shared__ double part[4], ahead[8];
+    __shared__ int pick[8];
+    __shared__ int last;
+    constexpr int QL = QT == kNone ? kF32 : QT;
+    const int b = int(blockIdx.x) / p.end_pieces, mine = int(blockIdx.x) - b * p.end_pieces;
+    const int tid = int(threadIdx.x), lane = tid & 63;
+    const VerifySeq sq = LoadSeq(p, b);
+    if (sq.n == 0) {
+        if (mine == 0) NoRows(p, b, 256);
+        return;
+    }
+    const double c = SlopeOf(p, b);
+    const SeqEnd end = p.ends[b];
+    pow2.Fill();
+    __syncthreads();
+    const int64_t row = sq.first + end.row;
+    const double inv = 1.0 / end.stats.sum;
+    const double *totals = p.totals + sq.first;
+    const auto mark = [&](int v0) {
+        if constexpr (QT == kNone) {
+            __syncthreads();
+            if (tid < kEndPiece / 32) marks[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < end.refused; i += 256) {
+                const int tok = p.refused[sq.first + i];
+                if (tok >= v0 && tok < v0 + kEndPiece) atomicOr(&marks[(tok - v0) >> 5], 1u << (tok & 31));
+            }
+            __syncthreads();
+        }
+    };
+    // what is left of value v, x its logit and q its draft probability; where
+    // nothing is left at all, p before the last refusal (`stays`)
+    const auto left_of = [&](int v, float x, float q, bool refused, bool stays) {
+        const double w = Weight(pow2, Logit(x), v, end.stats.top, end.stats.at, c);
+        if (QT == kNone) return refused && !stays ? 0.0 : w;
+        double was;
+        const double left = Left(w * inv, Chance(q), totals, end.refused, was);
+        return stays ? was : left;
+    };
+    // a piece's values, 8 in a row for each thread: their sum
+    const auto sum_of = [&](int piece, bool stays) {
+        const int v0 = piece * kEndPiece, v = v0 + tid * 8;
+        const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
+        Raw8<QL> q;
+        if (QT != kNone) q = Load8<QL>(p.draft, row * p.ld_draft, v, p.vocab, 0);
+        mark(v0);
+        const uint32_t refused = QT == kNone ? marks[tid >> 2] >> (8 * (tid & 3)) : 0;
+        double s = 0.0;
+        if (end.stats.top != -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                s += left_of(v + e, Val<XT>::Load(x.v[e]), QT != kNone ? Val<QL>::Load(q.v[e]) : 0.0f,
+                             ((refused >> e) & 1) != 0, stays);
+        }
+        return s;
+    };
+    double *sums = p.sums + int64_t(b) * p.end_pieces, *sums8 = p.sums8 + int64_t(b) * p.end_pieces * 256;
+    // ---- this workgroup's piece; the last one of the sequence goes on
+    {
+        const double s = sum_of(mine, false);
+        PutDev(sums8 + mine * 256 + tid, s);
+        const double all = BlockSumD<256>(s, part);
+        if (tid == 0) PutDev(sums + mine, all);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's sums are written
+        __syncthreads();
+        if (tid == 0) last = Arrive(p.cnt + b * kCounters, p.end_pieces);
+        __syncthreads();
+        if (!last) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    }
+    const auto total_of = [&] {
+        double s = 0.0;
+        for (int k = tid; k < p.end_pieces; k += 256) s += GetDev(sums + k);
+        return BlockSumD<256>(s, part);
+    };
+    double total = total_of();
+    const bool stays = !(total > 0.0);
+    if (stays) {  // nothing is left: all pieces again, by this workgroup
+        for (int k = 0; k < p.end_pieces; ++k) {
+            const double s = sum_of(k, true);
+            PutDev(sums8 + k * 256 + tid, s);
+            const double all = BlockSumD<256>(s, part);
+            if (tid == 0) PutDev(sums + k, all);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        __syncthreads();
+        total = total_of();
+        if (!(total > 0.0)) {
+            if (tid == 0) p.next[b] = -1;
+            return;
         }
     }
+    const double bar = double(p.u_next[b]) * total;
+    // its piece
+    int piece = 0;
+    double base = 0.0, before = 0.0;
+    for (int k0 = 0; k0 < p.end_pieces; k0 += 256) {
+        const double v = k0 + tid < p.end_pieces ? GetDev(sums + k0 + tid) : 0.0;
+        const Pick k = PickThread(v, before, bar, part, pick, ahead);
+        if (k.at >= 0) {
+            piece = k0 + k.at;
+            base = k.before;
+        }
+        if (k.over || k0 + 256 >= p.end_pieces) break;
+        before += BlockSumD<256>(v, part);
+    }
+    // its eight values
+    const Pick t = PickThread(GetDev(sums8 + piece * 256 + tid), base, bar, part, pick, ahead);
+    // its place: lanes 0 to 7
+    const int v0 = piece * kEndPiece, v = v0 + max(t.at, 0) * 8 + (lane & 7);
+    mark(v0);
+    if (tid >= 64) return;
+    double own = 0.0;
+    if (lane < 8 && v < p.vocab)
+        own = left_of(v, At<XT>(p.logits, row * p.ld_logits + v),
+                      QT != kNone ? At<QL>(p.draft, row * p.ld_draft + v) : 0.0f,
+                      QT == kNone && ((marks[(v - v0) >> 5] >> (v & 31)) & 1) != 0, stays);
+    double incl = own;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        hit = min(hit, __shfl_xor(hit, o, 64));
-        tail = max(tail, __shfl_xor(tail, o, 64));
+    for (int o = 1; o < 8; o <<= 1) {
+        const double x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
     }
-    __shared__ int hits[4], tails[4];
-    if (lane == 0) hits[wave] = hit, tails[wave] = tail;
-    __syncthreads();
-    if (tid == 0) {
-        hit = min(min(hits[0], hits[1]), min(hits[2], hits[3]));
-        tail = max(max(tails[0], tails[1]), max(tails[2], tails[3]));
-        p.next[b] = hit != INT32_MAX ? hit : tail;
-    }
+    const uint64_t over = __ballot(own > 0.0 && t.before + incl > bar), some = __ballot(own > 0.0);
+    if (lane == 0)
+        p.next[b] = v + (over != 0 ? __builtin_ctzll(over) : some != 0 ? 63 - __builtin_clzll(some) : 0);
 }
 
 struct VerifyShape {
-    int pieces;
-    size_t parts, stats, totals, ends, lefts, bytes;
+    int pieces, end_pieces;
+    size_t parts, totals, refused, ends, sums, sums8, bytes;
 };
 
 VerifyShape ShapeOf(const kr_drafts &d, const kr_seqs &s)
@@ -531,13 +712,46 @@ VerifyShape ShapeOf(const kr_drafts &d, const kr_seqs &s)
     VerifyShape f{};
     f.pieces = int((int64_t(d.vocab) + kPiece - 1) / kPiece);
     const size_t rows = size_t(d.rows), seqs = size_t(s.seqs);
-    f.parts = 0;
-    f.stats = f.parts + rows * f.pieces * sizeof(RowPart);
-    f.totals = f.stats + rows * sizeof(RowPart);
-    f.lefts = f.totals + (rows * sizeof(double) + 15) / 16 * 16;
-    f.ends = f.lefts + seqs * f.pieces * sizeof(LeftPart);
-    f.bytes = f.ends + (seqs * sizeof(SeqEnd) + 15) / 16 * 16;
+    f.end_pieces = int((int64_t(d.vocab) + kEndPiece - 1) / kEndPiece);
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t from = at;
+        at += (bytes + 15) / 16 * 16;
+        return from;
+    };
+    f.parts = take(rows * f.pieces * sizeof(RowPart));
+    f.totals = take(rows * sizeof(double));
+    f.refused = take(rows * sizeof(int32_t));
+    f.ends = take(seqs * sizeof(SeqEnd));
+    f.sums = take(seqs * f.end_pieces * sizeof(double));
+    f.sums8 = take(seqs * f.end_pieces * 256 * sizeof(double));
+    f.bytes = at;
     return f;
+}
+
+template <int XT, int QT>
+void VerifyGo(const VerifyParams &p, hipStream_t stream)
+{
+    const dim3 rows(unsigned(p.rows) * unsigned(p.pieces)), ends(unsigned(p.seqs) * unsigned(p.end_pieces));
+    const unsigned lds = unsigned(p.max_new) * WalkLds::kBytes;
+    if (p.rows > 0 && p.max_new > 0) {
+        if (QT != kNone && p.parents != nullptr) {
+            hipLaunchKernelGGL((StatsKernel<XT, kNone, false>), rows, dim3(256), 0, stream, p);
+            hipLaunchKernelGGL((WalkKernel<XT, QT>), dim3(unsigned(p.seqs)), dim3(1024), lds, stream, p);
+        } else {
+            hipLaunchKernelGGL((StatsKernel<XT, QT, true>), rows, dim3(256), lds, stream, p);
+        }
+    }
+    hipLaunchKernelGGL((NextKernel<XT, QT>), ends, dim3(256), 0, stream, p);
+}
+
+template <int XT>
+void VerifyGo(const VerifyParams &p, int qt, hipStream_t stream)
+{
+    if (qt == kNone) VerifyGo<XT, kNone>(p, stream);
+    else if (qt == kBF16) VerifyGo<XT, kBF16>(p, stream);
+    else if (qt == kF16) VerifyGo<XT, kF16>(p, stream);
+    else VerifyGo<XT, kF32>(p, stream);
 }
 
 kr_drafts CheckDrafts(const kr_drafts *d, const kr_seqs *s)
@@ -549,13 +763,15 @@ kr_drafts CheckDrafts(const kr_drafts *d, const kr_seqs *s)
     if (!known(d->dtype) || (d->draft != nullptr && !known(d->draft_dtype)))
         refuse("logits and draft must be bf16, f16 or f32");
     if (d->rows < 0 || d->vocab < 1) refuse("a negative or empty size");
+    if (s->seqs > (1 << 24)) refuse("too many sequences");
     if (s->max_new > kMostNew) refuse("a sequence has at most 1024 new tokens");
     if (d->rows > 1 && (d->ld_logits < d->vocab || (d->draft != nullptr && d->ld_draft < d->vocab)))
         refuse("rows of logits or draft overlap");
     if (d->ld_logits > (int64_t(1) << 40) || d->ld_draft > (int64_t(1) << 40)) refuse("a row stride is too large");
     if (d->vocab > (1 << 30)) refuse("the vocabulary is too large");
     const int64_t pieces = (int64_t(d->vocab) + kPiece - 1) / kPiece;
-    if (pieces * d->rows >= kMaxGrid || pieces * s->seqs >= kMaxGrid) refuse("too many rows for one launch");
+    const int64_t end_pieces = (int64_t(d->vocab) + kEndPiece - 1) / kEndPiece;
+    if (pieces * d->rows >= kMaxGrid || end_pieces * s->seqs >= kMaxGrid) refuse("too many rows for one launch");
     return *d;
 }
 
@@ -565,11 +781,11 @@ void VerifyNeeds(const kr_drafts *drafts, const kr_seqs *s, size_t *ws_bytes, in
 {
     const kr_drafts d = CheckDrafts(drafts, s);
     *ws_bytes = ShapeOf(d, *s).bytes;
-    *counters = 0;
+    *counters = s->seqs * kCounters;
 }
 
 void VerifyLaunch(const kr_drafts *drafts, const kr_seqs *s, const VerifyOut &o, void *ws, size_t ws_bytes,
-                  int32_t *, int, hipStream_t stream)
+                  int32_t *cnt, int cnt_len, hipStream_t stream)
 {
     const auto refuse = [](const char *what) { throw std::runtime_error(std::string("verify_drafts: ") + what); };
     const kr_drafts d = CheckDrafts(drafts, s);
@@ -585,16 +801,18 @@ void VerifyLaunch(const kr_drafts *drafts, const kr_seqs *s, const VerifyOut &o,
         off(d.parents, 4) || off(d.u, 4) || off(d.u_next, 4) || off(d.temperature, 4) || off(o.path, 4) || off(o.path_lens, 4))
         refuse("a pointer is misaligned");
     const VerifyShape f = ShapeOf(d, *s);
-    if (ws == nullptr || ws_bytes < f.bytes || off(ws, 16)) refuse("the workspace is too small or misaligned");
+    if (ws == nullptr || ws_bytes < f.bytes || off(ws, 16) || cnt == nullptr || cnt_len < s->seqs * kCounters || off(cnt, 4))
+        refuse("the workspace is too small or misaligned");
     const MemSpan outs[] = {RowsSpan(o.path, s->seqs, o.ld_path, o.width, 4), RowsSpan(o.path_lens, 1, 0, s->seqs, 4),
-                            RowsSpan(o.next, 1, 0, s->seqs, 8), MemSpan{ws, int64_t(f.bytes)}};
+                            RowsSpan(o.next, 1, 0, s->seqs, 8), MemSpan{ws, int64_t(f.bytes)},
+                            RowsSpan(cnt, 1, 0, s->seqs * kCounters, 4)};
     const MemSpan ins[] = {RowsSpan(d.logits, d.rows, d.ld_logits, d.vocab, size),
                            RowsSpan(d.draft, d.rows, d.ld_draft, d.vocab, dsize), RowsSpan(d.tokens, 1, 0, d.rows, 8),
                            RowsSpan(d.parents, 1, 0, d.rows, 4), RowsSpan(d.u, 1, 0, d.rows, 4),
                            RowsSpan(d.u_next, 1, 0, s->seqs, 4), RowsSpan(d.temperature, 1, 0, s->seqs, 4),
                            RowsSpan(s->starts, 1, 0, s->seqs + 1, 4)};
-    for (int i = 0; i < 4; ++i) {
-        for (int j = i + 1; j < 4; ++j)
+    for (int i = 0; i < 5; ++i) {
+        for (int j = i + 1; j < 5; ++j)
             if (Meets(outs[i], outs[j])) refuse("outputs and workspace overlap");
         for (const MemSpan &in : ins)
             if (Meets(outs[i], in)) refuse("an output or the workspace overlaps an input");
@@ -614,33 +832,25 @@ void VerifyLaunch(const kr_drafts *drafts, const kr_seqs *s, const VerifyOut &o,
     p.ld_logits = d.ld_logits;
     p.ld_draft = d.ld_draft;
     p.ld_path = o.ld_path;
-    p.dtype = d.dtype;
-    p.draft_dtype = d.draft_dtype;
     p.vocab = d.vocab;
     p.rows = d.rows;
     p.seqs = s->seqs;
     p.max_new = s->max_new;
     p.width = o.width;
     p.pieces = f.pieces;
-    p.wide = !off(d.logits, 16) && (d.rows <= 1 || d.ld_logits * size % 16 == 0);
-    p.draft_wide = !off(d.draft, 16) && (d.rows <= 1 || d.ld_draft * dsize % 16 == 0);
+    p.end_pieces = f.end_pieces;
     char *base = static_cast<char *>(ws);
     p.parts = reinterpret_cast<RowPart *>(base + f.parts);
-    p.stats = reinterpret_cast<RowPart *>(base + f.stats);
     p.totals = reinterpret_cast<double *>(base + f.totals);
-    p.lefts = reinterpret_cast<LeftPart *>(base + f.lefts);
     p.ends = reinterpret_cast<SeqEnd *>(base + f.ends);
-    if (d.rows > 0 && s->max_new > 0) {
-        hipLaunchKernelGGL(StatsKernel, dim3(unsigned(d.rows) * unsigned(f.pieces)), dim3(256), 0, stream, p);
-        Check(hipGetLastError(), "verify_drafts launch");
-    }
-    hipLaunchKernelGGL(WalkKernel, dim3(unsigned(s->seqs)), dim3(256), 0, stream, p);
-    Check(hipGetLastError(), "verify_drafts launch");
-    if (d.rows > 0 && s->max_new > 0) {
-        hipLaunchKernelGGL(LeftKernel, dim3(unsigned(s->seqs) * unsigned(f.pieces)), dim3(256), 0, stream, p);
-        Check(hipGetLastError(), "verify_drafts launch");
-    }
-    hipLaunchKernelGGL(NextKernel, dim3(unsigned(s->seqs)), dim3(256), 0, stream, p);
+    p.sums = reinterpret_cast<double *>(base + f.sums);
+    p.sums8 = reinterpret_cast<double *>(base + f.sums8);
+    p.refused = reinterpret_cast<int32_t *>(base + f.refused);
+    p.cnt = cnt;
+    const int qt = d.draft != nullptr ? d.draft_dtype : kNone;
+    if (d.dtype == kBF16) VerifyGo<kBF16>(p, qt, stream);
+    else if (d.dtype == kF16) VerifyGo<kF16>(p, qt, stream);
+    else VerifyGo<kF32>(p, qt, stream);
     Check(hipGetLastError(), "verify_drafts launch");
 }
 

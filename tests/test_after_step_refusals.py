@@ -40,9 +40,9 @@ def evict(c=None, s=None, w=None, budget=10, sinks=0, recent=0, keep=FAR):
 
 
 def verify(d=None, s=None, path=FAR, ld_path=5, width=5, lens=FAR + (1 << 20), nxt=FAR + (2 << 20), ws=FAR + (3 << 20),
-           nbytes=1 << 20):
-    return ops._lib().kr_op_verify_drafts(d or drafts(), s or seqs(), path, ld_path, width, lens, nxt, ws, nbytes, None, 0,
-                                          None)
+           nbytes=1 << 20, cnt=FAR + (5 << 20), ncnt=96):
+    return ops._lib().kr_op_verify_drafts(d or drafts(), s or seqs(), path, ld_path, width, lens, nxt, ws, nbytes, cnt,
+                                          ncnt, None)
 
 
 @pytest.mark.parametrize("field,text", BAD_CACHES)
@@ -114,6 +114,9 @@ def test_bad_drafts(field, text):
     (dict(width=0), "path rows"), (dict(ld_path=4), "path rows"), (dict(path=None), "output"), (dict(lens=None), "output"),
     (dict(nxt=None), "output"), (dict(nxt=FAR + 4), "misaligned"), (dict(path=FAR + 1), "misaligned"),
     (dict(ws=None), "workspace"), (dict(nbytes=10), "workspace"), (dict(ws=FAR + 8), "workspace"),
+    (dict(cnt=None), "workspace"), (dict(ncnt=95), "workspace"), (dict(cnt=FAR + (5 << 20) + 2), "workspace"),
+    (dict(cnt=A), "overlap"), (dict(cnt=FAR + (2 << 20)), "overlap"),
+    (dict(cnt=None), "workspace"), (dict(ncnt=95), "workspace"), (dict(cnt=FAR + 2), "workspace"), (dict(cnt=A), "overlap"),
     (dict(path=A), "overlap"), (dict(lens=FAR + 4), "overlap"), (dict(nxt=W), "overlap"), (dict(ws=A), "overlap"),
     (dict(s=seqs(max_new=1025)), "1024"),
 ])
