@@ -303,7 +303,14 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
             x.top = top;
             x.at = min(ax, ay);
         };
-        for (int k = l8; k < p.pieces; k += 8) add(GetPart(parts + k));
+        for (int k = l8; k < p.pieces; k += 32) {
+            RowPart y[4];  // (all on their way before the first is used)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = GetPart(parts + min(k + 8 * i, p.pieces - 1));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + 8 * i < p.pieces) add(y[i]);
+        }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
             RowPart y;
