@@ -12,11 +12,11 @@
 // destination: all of them can move at once. The recent tokens then come down
 // to [end, budget), by a shift, in order.
 //
-// The first launch finds the K-th largest weight by its bits, 11 or 10 at a time
-// from the top (a histogram of those that share the bits found so far), then
+// The first launch finds the K-th largest weight by its bits from the top, then
 // lists holes and movers; the second and third move the rows.
 #include <algorithm>
 
+#include "kr_dma.h"
 #include "kr_paged.h"
 
 namespace kr {
@@ -50,20 +50,22 @@ __device__ __forceinline__ uint32_t KeyOf(float f)
     return f != f ? 0u : (u >> 31) != 0 ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
-
-// Sum of `v` over the threads before this one; `total` over all.
+// Sum of `v` over the threads of the workgroup before this one; `total` over all.
+template <int NT>
 __device__ __forceinline__ int BlockScan(int v, int *part, int &total)
 {
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
     const int incl = WaveScan(v, lane);
+    if constexpr (NT == 64) {
+        total = __shfl(incl, 63, 64);
+        return incl - v;
+    }
     if (lane == 63) part[wave] = incl;
     __syncthreads();
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int i = 0; i < kSelWaves; ++i) {
+    for (int i = 0; i < NT / 64; ++i) {
         const int x = part[i];
         before += i < wave ? x : 0;
         total += x;
@@ -72,129 +74,342 @@ __device__ __forceinline__ int BlockScan(int v, int *part, int &total)
     return before + incl - v;
 }
 
-__global__ void __launch_bounds__(kSelThreads) SelectKernel(EvictParams p)
+// The K-th largest of the keys that `each` goes through, by its bits from the
+// top, and how many of that key are wanted and there.
+struct Threshold {
+    uint32_t key;
+    int want, equal;
+};
+
+// By a histogram of 11, 11 and 10 bits. Weights have few exponents, so that a
+// wave's lanes often add to the same bin, one after the other: many threads have
+// CP copies of it, by the lane.
+template <int NT, int CP, typename F>
+__device__ __forceinline__ Threshold ByHistogram(int K, int *hist, int *part, int *found, F &&each)
 {
-    __shared__ int hist[2048];
-    __shared__ int part[kSelWaves];
-    __shared__ int found[3];
+    constexpr int PER = 2048 / NT;  // bins of a thread
     const int tid = int(threadIdx.x);
-    const int h = int(blockIdx.x) % p.heads, b = int(blockIdx.x) / p.heads, layer = int(blockIdx.y);
-    int32_t *keep = p.keep + ((int64_t(layer) * p.seqs + b) * p.heads + h) * p.budget;
-    int entry;
-    const int len = Evicted(p, b, entry);
-    if (len == 0) {
-        const int n = min(min(max(p.lens[b], 0), p.cap), p.budget);
-        for (int i = tid; i < p.budget; i += kSelThreads) keep[i] = i < n ? i : -1;
-        return;
-    }
-    float *w = p.w + layer * p.w_layer + entry * p.w_entry + h * p.w_head;
-    const int end = p.budget - p.recent, low = len - p.recent;
-    const int K = end - p.sinks;
-    // ---- the K-th largest key of the middle, how many of it are wanted and there
-    uint32_t key = 0;
-    int want = K, equal = 0;
-    if (K > 0) {
-        for (int step = 0; step < 3; ++step) {
-            const int shift = step == 0 ? 21 : step == 1 ? 10 : 0;
-            const int bins = step == 2 ? 1024 : 2048;
-            for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-            __syncthreads();
-            for (int j = p.sinks + tid; j < low; j += kSelThreads) {
-                const uint32_t x = KeyOf(w[j]);
-                const bool in = step == 0 || (step == 1 ? (x >> 21) == (key >> 21) : (x >> 10) == (key >> 10));
-                if (in) atomicAdd(&hist[(x >> shift) & uint32_t(bins - 1)], 1);
-            }
-            __syncthreads();
-            // bins from the top: thread t has the two below 2048 - 2 t
-            const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
-            int total;
-            const int above = BlockScan(hi + lo, part, total);
-            if (above < want && above + hi + lo >= want) {
-                const bool first = above + hi >= want;
-                found[0] = first ? 2047 - 2 * tid : 2046 - 2 * tid;
-                found[1] = want - above - (first ? 0 : hi);
-                found[2] = first ? hi : lo;
-            }
-            __syncthreads();
-            key |= uint32_t(found[0]) << shift;
-            want = found[1];
-            equal = found[2];
-            __syncthreads();
-        }
-    }
-    // of the `equal` tokens with exactly this weight the first `want` stay
-    const bool ranked = want < equal;
-    // ---- movers, in order, to keep[sinks..]; the equal ones before `end` come first
-    int ties = 0, movers = 0;
-    if (ranked) {
-        for (int j0 = p.sinks; j0 < end; j0 += kSelThreads) {
-            int total;
-            const int j = j0 + tid;
-            BlockScan(j < end && KeyOf(w[j]) == key ? 1 : 0, part, total);
-            ties += total;
-        }
-    }
-    const int ties_front = ties;
-    if (K > 0) {
-        for (int j0 = end; j0 < low; j0 += kSelThreads) {
-            const int j = j0 + tid;
-            const uint32_t x = j < low ? KeyOf(w[j]) : 0u;
-            int total;
-            bool wins = j < low && x > key;
-            if (ranked) {
-                const bool tie = j < low && x == key;
-                const int rank = ties + BlockScan(tie ? 1 : 0, part, total);
-                ties += total;
-                wins = wins || (tie && rank < want);
-            } else {
-                wins = wins || (j < low && x == key);
-            }
-            const int at = movers + BlockScan(wins ? 1 : 0, part, total);
-            movers += total;
-            if (wins) keep[p.sinks + at] = j;
-        }
-    }
-    __syncthreads();
-    // ---- the holes, last to first: the one that comes n-th is at sinks + n or
-    // behind it, so what is written over is no longer needed
-    int left = movers;
-    ties = ties_front;
-    for (int j0 = p.sinks + (max(K - 1, 0) / kSelThreads) * kSelThreads; K > 0 && j0 >= p.sinks; j0 -= kSelThreads) {
-        const int j = j0 + tid;
-        const bool in = j < end;
-        const uint32_t x = in ? KeyOf(w[j]) : 0u;
-        int total;
-        bool wins = in && x > key;
-        if (ranked) {
-            const bool tie = in && x == key;
-            const int before = BlockScan(tie ? 1 : 0, part, total);
-            ties -= total;
-            wins = wins || (tie && ties + before < want);
-        } else {
-            wins = wins || (in && x == key);
-        }
-        const bool hole = in && !wins;
-        const int before = BlockScan(hole ? 1 : 0, part, total);
-        left -= total;
-        const int of = hole ? keep[p.sinks + left + before] : j;
+    Threshold t{0, K, 0};
+    for (int step = 0; step < 3; ++step) {
+        const int shift = step == 0 ? 21 : step == 1 ? 10 : 0;
+        const uint32_t mask = step == 2 ? 1023 : 2047;
+        for (int i = tid; i < 2048 * CP; i += NT) hist[i] = 0;
         __syncthreads();
-        if (in) keep[j] = of;
+        each([&](uint32_t x) {
+            const bool in = step == 0 || (step == 1 ? (x >> 21) == (t.key >> 21) : (x >> 10) == (t.key >> 10));
+            if (in) atomicAdd(&hist[((x >> shift) & mask) * CP + (tid & (CP - 1))], 1);
+        });
+        __syncthreads();
+        // bins from the top: thread i has PER of them below 2048 - PER i
+        int mine[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            mine[i] = 0;
+#pragma unroll
+            for (int c = 0; c < CP; ++c) mine[i] += hist[(2047 - PER * tid - i) * CP + c];
+            sum += mine[i];
+        }
+        int total;
+        int above = BlockScan<NT>(sum, part, total);
+        if (above < t.want && above + sum >= t.want) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (above < t.want && above + mine[i] >= t.want) {
+                    found[0] = 2047 - PER * tid - i;
+                    found[1] = t.want - above;
+                    found[2] = mine[i];
+                }
+                above += mine[i];
+            }
+        }
+        __syncthreads();
+        t.key |= uint32_t(found[0]) << shift;
+        t.want = found[1];
+        t.equal = found[2];
+        __syncthreads();
     }
-    for (int i = tid; i < p.sinks; i += kSelThreads) keep[i] = i;
-    for (int i = end + tid; i < p.budget; i += kSelThreads) keep[i] = low + i - end;
-    __syncthreads();
-    // ---- the weights move as the rows will
-    for (int i = p.sinks + tid; i < end; i += kSelThreads) {
-        const int of = keep[i];
-        if (of != i) w[i] = w[of];
-    }
-    __syncthreads();
-    for (int i0 = end; i0 < p.budget; i0 += kSelThreads) {
+    return t;
+}
+
+__device__ __forceinline__ int32_t *KeepOf(const EvictParams &p, int layer, int b, int h)
+{
+    return p.keep + ((int64_t(layer) * p.seqs + b) * p.heads + h) * p.budget;
+}
+
+// Before the rest of a list: a sequence that is left alone.
+__device__ __forceinline__ bool LeftAlone(const EvictParams &p, int b, int len, int32_t *keep, int nt)
+{
+    if (len > 0) return false;
+    const int n = min(min(max(p.lens[b], 0), p.cap), p.budget);
+    for (int i = int(threadIdx.x); i < p.budget; i += nt) keep[i] = i < n ? i : -1;
+    return true;
+}
+
+// The rest of a list, and the recent tokens' weights: a shift, in order.
+template <int NT>
+__device__ __forceinline__ void Recent(const EvictParams &p, int len, int32_t *keep, float *w)
+{
+    const int tid = int(threadIdx.x);
+    const int end = p.budget - p.recent, low = len - p.recent;
+    for (int i = tid; i < p.sinks; i += NT) keep[i] = i;
+    for (int i = end + tid; i < p.budget; i += NT) keep[i] = low + i - end;
+    for (int i0 = end; i0 < p.budget; i0 += NT) {
         const int i = i0 + tid;
         const float x = i < p.budget ? w[low + i - end] : 0.0f;
         __syncthreads();
         if (i < p.budget) w[i] = x;
     }
+}
+
+// A list by NT threads that hold all of the middle: thread t tokens sinks + t +
+// NT i. A wave alone finds the threshold bit by bit with ballots, more of them by
+// histograms. Ranks come from one scan over the items' waves.
+template <int NT, int IT>
+__global__ void __launch_bounds__(NT) SelectKernel(EvictParams p)
+{
+    constexpr int NW = NT / 64, CELLS = IT * NW, CP = NT == 1024 ? 4 : 1;
+    __shared__ int hist[NT == 64 ? 1 : 2048 * CP];
+    __shared__ int part[NW];
+    __shared__ int found[3];
+    __shared__ int cells[2][CELLS];
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const int h = int(blockIdx.x) % p.heads, b = int(blockIdx.x) / p.heads, layer = int(blockIdx.y);
+    int32_t *keep = KeepOf(p, layer, b, h);
+    int entry;
+    const int len = Evicted(p, b, entry);
+    if (LeftAlone(p, b, len, keep, NT)) return;
+    float *w = p.w + layer * p.w_layer + entry * p.w_entry + h * p.w_head;
+    const int end = p.budget - p.recent, low = len - p.recent;
+    const int K = end - p.sinks;
+    if (K > 0) {
+        uint32_t key[IT];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int j = p.sinks + tid + NT * i;
+            key[i] = KeyOf(w[uint32_t(min(j, low - 1))]);
+        }
+        const int items = (low - p.sinks - tid + NT - 1) / NT;
+        const auto in = [&](int i) { return i < items; };
+        Threshold t{0, K, 0};
+        if constexpr (NT == 64) {
+            // the largest key that K of them reach
+            for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < IT; ++i) n += __popcll(__ballot(in(i) && key[i] >= (t.key | bit)));
+                if (n >= K) t.key |= bit;
+            }
+            int above = 0;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                above += __popcll(__ballot(in(i) && key[i] > t.key));
+                t.equal += __popcll(__ballot(in(i) && key[i] == t.key));
+            }
+            t.want = K - above;
+        } else {
+            t = ByHistogram<NT, CP>(K, hist, part, found, [&](auto &&add) {
+#pragma unroll
+                for (int i = 0; i < IT; ++i)
+                    if (in(i)) add(key[i]);
+            });
+        }
+        // how many tokens of an item's wave there are in front, for each of two kinds
+        const uint64_t below = (1ull << lane) - 1;
+        const auto scan = [&](auto &&kind, int kinds) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                for (int k = 0; k < kinds; ++k) {
+                    const int n = __popcll(__ballot(kind(i, k)));
+                    if (lane == 0) cells[k][i * NW + wave] = n;
+                }
+            __syncthreads();
+            for (int k = 0; k < kinds; ++k) {
+                constexpr int PER = (CELLS + NT - 1) / NT;
+                int mine[PER], sum = 0, total;
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    mine[c] = tid * PER + c < CELLS ? cells[k][tid * PER + c] : 0;
+                    sum += mine[c];
+                }
+                int at = BlockScan<NT>(sum, part, total);
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    if (tid * PER + c < CELLS) cells[k][tid * PER + c] = at;
+                    at += mine[c];
+                }
+            }
+            __syncthreads();
+        };
+        uint32_t wins = 0;  // bit i
+        static_assert(IT <= 32, "a bit an item");
+        if (t.want < t.equal) {  // of the equal ones the first `want` stay
+            scan([&](int i, int) { return in(i) && key[i] == t.key; }, 1);
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const bool tie = in(i) && key[i] == t.key;
+                const int rank = cells[0][i * NW + wave] + __popcll(__ballot(tie) & below);
+                if (in(i) && (key[i] > t.key || (tie && rank < t.want))) wins |= 1u << i;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                if (in(i) && key[i] >= t.key) wins |= 1u << i;
+        }
+        const auto won = [&](int i) { return ((wins >> i) & 1) != 0; };
+        const auto kind = [&](int i, int k) {
+            const int j = p.sinks + tid + NT * i;
+            return k == 0 ? won(i) && j >= end : !won(i) && j < end;
+        };
+        scan(kind, 2);
+        // the movers, in order, to keep[sinks..]; then to the holes, which are as many
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const bool mover = kind(i, 0);
+            const uint64_t all = __ballot(mover);
+            if (mover) keep[uint32_t(p.sinks + cells[0][i * NW + wave] + __popcll(all & below))] = p.sinks + tid + NT * i;
+        }
+        __syncthreads();
+        int of[IT];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const bool hole = kind(i, 1);
+            const uint64_t all = __ballot(hole);
+            of[i] = hole ? keep[uint32_t(p.sinks + cells[1][i * NW + wave] + __popcll(all & below))] : -1;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int j = p.sinks + tid + NT * i;
+            if (j >= end) continue;
+            keep[uint32_t(j)] = of[i] >= 0 ? of[i] : j;
+            if (of[i] >= 0) w[uint32_t(j)] = w[uint32_t(of[i])];  // (nobody's hole)
+        }
+        __syncthreads();
+    }
+    Recent<NT>(p, len, keep, w);
+}
+
+// Longer middles: tiles of 1024 x IT tokens, read again for each step.
+template <int IT>
+__global__ void __launch_bounds__(1024) SelectLongKernel(EvictParams p)
+{
+    constexpr int NT = 1024, NW = NT / 64, TILE = NT * IT, CP = 4;
+    __shared__ int hist[2048 * CP];
+    __shared__ int part[NW];
+    __shared__ int found[3];
+    __shared__ int cells[IT * NW];
+    static_assert(IT * NW <= NT, "a cell a thread");
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const int h = int(blockIdx.x) % p.heads, b = int(blockIdx.x) / p.heads, layer = int(blockIdx.y);
+    int32_t *keep = KeepOf(p, layer, b, h);
+    int entry;
+    const int len = Evicted(p, b, entry);
+    if (LeftAlone(p, b, len, keep, NT)) return;
+    float *w = p.w + layer * p.w_layer + entry * p.w_entry + h * p.w_head;
+    const int end = p.budget - p.recent, low = len - p.recent;
+    const int K = end - p.sinks;
+    if (K > 0) {
+        uint32_t key[IT];
+        const auto load = [&](int j0, int last) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i) key[i] = KeyOf(w[uint32_t(min(j0 + tid + NT * i, last - 1))]);
+        };
+        const Threshold t = ByHistogram<NT, CP>(K, hist, part, found, [&](auto &&add) {
+            for (int j0 = p.sinks; j0 < low; j0 += TILE) {
+                load(j0, low);
+#pragma unroll
+                for (int i = 0; i < IT; ++i)
+                    if (j0 + tid + NT * i < low) add(key[i]);
+            }
+        });
+        const uint64_t below = (1ull << lane) - 1;
+        // how many of a tile's tokens of a kind are in front of each item's wave; returns how many there are
+        const auto scan = [&](auto &&kind) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int n = __popcll(__ballot(kind(i)));
+                if (lane == 0) cells[i * NW + wave] = n;
+            }
+            __syncthreads();
+            int total;
+            const int at = BlockScan<NT>(tid < IT * NW ? cells[tid] : 0, part, total);
+            if (tid < IT * NW) cells[tid] = at;
+            __syncthreads();
+            return total;
+        };
+        // which of a tile's tokens stay, as bits; `ties`: equal ones in front of the tile, of which the first `want` stay
+        const bool ranked = t.want < t.equal;
+        const auto winners = [&](int j0, int last, int ties, int &here) {
+            uint32_t wins = 0;
+            here = 0;
+            if (ranked) here = scan([&](int i) { return j0 + tid + NT * i < last && key[i] == t.key; });
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const bool in = j0 + tid + NT * i < last, tie = in && key[i] == t.key;
+                const uint64_t all = __ballot(tie);
+                const bool stays = tie && (!ranked || ties + cells[i * NW + wave] + __popcll(all & below) < t.want);
+                if (stays || (in && key[i] > t.key)) wins |= 1u << i;
+            }
+            if (ranked) __syncthreads();
+            return wins;
+        };
+        // ---- movers, in order, to keep[sinks..]; the equal ones before `end` come first
+        int ties = 0, movers = 0, here;
+        if (ranked)
+            for (int j0 = p.sinks; j0 < end; j0 += TILE) {
+                load(j0, end);
+                winners(j0, end, ties, here);
+                ties += here;
+            }
+        const int ties_front = ties;
+        for (int j0 = end; j0 < low; j0 += TILE) {
+            load(j0, low);
+            const uint32_t wins = winners(j0, low, ties, here);
+            ties += here;
+            const int all = scan([&](int i) { return ((wins >> i) & 1) != 0; });
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const bool mover = ((wins >> i) & 1) != 0;
+                const uint64_t of = __ballot(mover);
+                if (mover)
+                    keep[p.sinks + movers + cells[i * NW + wave] + __popcll(of & below)] = j0 + tid + NT * i;
+            }
+            movers += all;
+            __syncthreads();
+        }
+        // ---- the holes, last tile to first: the one that comes n-th is at sinks +
+        // n or behind it, so what is written over is no longer needed
+        int left = movers;
+        ties = ties_front;
+        for (int j0 = p.sinks + (K - 1) / TILE * TILE; j0 >= p.sinks; j0 -= TILE) {
+            load(j0, end);
+            if (ranked) ties -= scan([&](int i) { return j0 + tid + NT * i < end && key[i] == t.key; });
+            if (ranked) __syncthreads();
+            const uint32_t wins = winners(j0, end, ties, here);
+            const auto hole = [&](int i) { return j0 + tid + NT * i < end && ((wins >> i) & 1) == 0; };
+            left -= scan(hole);
+            int of[IT];
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const bool is = hole(i);
+                const uint64_t all = __ballot(is);
+                of[i] = is ? keep[p.sinks + left + cells[i * NW + wave] + __popcll(all & below)] : j0 + tid + NT * i;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                if (j0 + tid + NT * i < end) keep[j0 + tid + NT * i] = of[i];
+        }
+        __syncthreads();
+        // ---- the weights move as the rows will
+        for (int i = p.sinks + tid; i < end; i += NT) {
+            const int of = keep[i];
+            if (of != i) w[i] = w[of];
+        }
+        __syncthreads();
+    }
+    Recent<NT>(p, len, keep, w);
 }
 
 // Element offset of column `col` of the row at position pos; -1: not there.
@@ -206,82 +421,121 @@ __device__ __forceinline__ int64_t RowAt(const EvictParams &p, const int32_t *ta
     return id * p.page_stride + int64_t(pos - pg * p.div.size) * p.token_stride + col;
 }
 
-constexpr int kMoveRows = 4;  // rows of a thread
+constexpr int kMoveRows = 4;       // rows of a thread
+constexpr int kMoveGroups = 2048;  // workgroups: eight on each of 256 CUs
 
-// Rows to the holes: a workgroup has kMoveRows x 256 / LPR places of one
-// sequence and head in one layer, K and V.
+// The sequences that lose tokens, 64 at a time: body(b, unit) for this
+// workgroup's share of the `per` units of each of them. (Most of a batch that is
+// trimmed often has nothing to lose; a workgroup for each of its units would
+// cost 1 ns a wave to start.)
+template <typename F>
+__device__ __forceinline__ void EachUnit(const EvictParams &p, int64_t per, F &&body)
+{
+    const int lane = int(threadIdx.x) & 63;
+    int64_t u = blockIdx.x;
+    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+        int entry;
+        const uint64_t some = __ballot(b0 + lane < p.seqs && Evicted(p, min(b0 + lane, p.seqs - 1), entry) > 0);
+        const int64_t units = per * __popcll(some);
+        for (; u < units; u += gridDim.x) {
+            const int nth = int(u / per);
+            uint64_t rest = some;
+            for (int i = 0; i < nth; ++i) rest &= rest - 1;
+            body(Uni(b0 + __builtin_ctzll(rest)), u - nth * per);
+        }
+        u -= units;
+    }
+}
+
+// Rows of K and V of a sequence and head in one layer that move together: four
+// a thread, LPR lanes a row. All loads go out before the first store.
+template <int LPR>
+struct MoveRows {
+    static constexpr int RPS = 256 / LPR, ROWS = kMoveRows * RPS;
+    uint4 x[kMoveRows][2];
+    int64_t to[kMoveRows];
+    // place i0 + n gets the row of token of(place); -1: stays
+    template <typename F>
+    __device__ __forceinline__ void Load(const EvictParams &p, int b, int layer, int h, int i0, F &&of)
+    {
+        const int32_t *table = p.table + b * p.ld_table;
+        const int64_t col = h * p.head_stride + (int(threadIdx.x) % LPR) * 8;
+        const uint16_t *k = p.k + layer * p.layer_stride, *v = p.v + layer * p.layer_stride;
+        int64_t from[kMoveRows];
+#pragma unroll
+        for (int n = 0; n < kMoveRows; ++n) {
+            const int i = i0 + n * RPS + int(threadIdx.x) / LPR;
+            const int j = of(i);
+            from[n] = j >= 0 ? RowAt(p, table, j, col) : -1;
+            to[n] = from[n] >= 0 ? RowAt(p, table, i, col) : -1;
+        }
+#pragma unroll
+        for (int n = 0; n < kMoveRows; ++n)
+            if (to[n] >= 0) {
+                x[n][0] = *reinterpret_cast<const uint4 *>(k + from[n]);
+                x[n][1] = *reinterpret_cast<const uint4 *>(v + from[n]);
+            }
+        asm volatile("" ::: "memory");  // (a row's store would join its load)
+    }
+    __device__ __forceinline__ void Store(const EvictParams &p, int layer) const
+    {
+        uint16_t *k = p.k + layer * p.layer_stride, *v = p.v + layer * p.layer_stride;
+#pragma unroll
+        for (int n = 0; n < kMoveRows; ++n)
+            if (to[n] >= 0) {
+                *reinterpret_cast<uint4 *>(k + to[n]) = x[n][0];
+                *reinterpret_cast<uint4 *>(v + to[n]) = x[n][1];
+            }
+    }
+};
+
+// Rows to the holes: a unit is a slice of the places of one sequence and head in one layer.
 template <int LPR>
 __global__ void __launch_bounds__(256) MoveKernel(EvictParams p, int slices)
 {
-    constexpr int RPS = 256 / LPR;
-    const int slice = int(blockIdx.x) % slices, bh = int(blockIdx.x) / slices;
-    const int h = bh % p.heads, b = bh / p.heads, layer = int(blockIdx.y);
-    int entry;
-    if (Evicted(p, b, entry) == 0) return;
-    const int32_t *keep = p.keep + ((int64_t(layer) * p.seqs + b) * p.heads + h) * p.budget;
-    const int32_t *table = p.table + b * p.ld_table;
-    const int end = p.budget - p.recent;
-    const int64_t col = h * p.head_stride + (int(threadIdx.x) % LPR) * 8;
-    uint16_t *k = p.k + layer * p.layer_stride, *v = p.v + layer * p.layer_stride;
-    uint4 x[kMoveRows][2];
-    int64_t to[kMoveRows];
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) {
-        const int i = p.sinks + (slice * kMoveRows + u) * RPS + int(threadIdx.x) / LPR;
-        const int of = i < end ? keep[i] : i;
-        const int64_t src = of != i ? RowAt(p, table, of, col) : -1;
-        to[u] = src >= 0 ? RowAt(p, table, i, col) : -1;
-        if (to[u] >= 0) {
-            x[u][0] = *reinterpret_cast<const uint4 *>(k + src);
-            x[u][1] = *reinterpret_cast<const uint4 *>(v + src);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u)
-        if (to[u] >= 0) {
-            *reinterpret_cast<uint4 *>(k + to[u]) = x[u][0];
-            *reinterpret_cast<uint4 *>(v + to[u]) = x[u][1];
-        }
+    EachUnit(p, int64_t(slices) * p.heads * p.layers, [&](int b, int64_t unit) {
+        const int slice = Uni(int(unit % slices)), lh = Uni(int(unit / slices));
+        const int h = lh % p.heads, layer = lh / p.heads;
+        const int32_t *keep = KeepOf(p, layer, b, h);
+        const int end = p.budget - p.recent;
+        MoveRows<LPR> r;
+        r.Load(p, b, layer, h, p.sinks + slice * MoveRows<LPR>::ROWS, [&](int i) {
+            const int j = i < end ? keep[i] : i;
+            return j != i ? j : -1;
+        });
+        r.Store(p, layer);
+    });
 }
 
-// The recent rows' shift: a workgroup has a sequence and head in one layer, K
-// and V. Sweep by sweep: a later row's old place is behind all new ones so far.
+// The recent rows' shift. Where their new places are none of the old ones, a
+// unit is a slice as above. Otherwise it is all of a sequence and head in one
+// layer, slice by slice, each read before any of it is written: a slice's old
+// places are behind all new ones so far.
 template <int LPR>
-__global__ void __launch_bounds__(256) ShiftKernel(EvictParams p)
+__global__ void __launch_bounds__(256) ShiftKernel(EvictParams p, int slices)
 {
-    constexpr int RPS = 256 / LPR;
-    const int h = int(blockIdx.x) % p.heads, b = int(blockIdx.x) / p.heads, layer = int(blockIdx.y);
-    int entry;
-    const int len = Evicted(p, b, entry);
-    if (len == 0) return;
-    const int32_t *table = p.table + b * p.ld_table;
-    const int end = p.budget - p.recent;
-    const int64_t col = h * p.head_stride + (int(threadIdx.x) % LPR) * 8;
-    uint16_t *k = p.k + layer * p.layer_stride, *v = p.v + layer * p.layer_stride;
-    for (int i0 = end; i0 < p.budget; i0 += kMoveRows * RPS) {
-        uint4 x[kMoveRows][2];
-        int64_t to[kMoveRows];
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u) {
-            const int i = i0 + u * RPS + int(threadIdx.x) / LPR;
-            const int64_t src = i < p.budget ? RowAt(p, table, len - p.budget + i, col) : -1;
-            to[u] = src >= 0 ? RowAt(p, table, i, col) : -1;
-            x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
-            if (to[u] >= 0) {
-                x[u][0] = *reinterpret_cast<const uint4 *>(k + src);
-                x[u][1] = *reinterpret_cast<const uint4 *>(v + src);
+    constexpr int ROWS = MoveRows<LPR>::ROWS;
+    EachUnit(p, int64_t(slices) * p.heads * p.layers, [&](int b, int64_t unit) {
+        // (slice by slice: only the first of an overlapping shift has work)
+        const int slice = Uni(int(unit / (p.heads * p.layers))), lh = Uni(int(unit % (p.heads * p.layers)));
+        const int h = lh % p.heads, layer = lh / p.heads;
+        const int by = min(p.lens[b], p.cap) - p.budget;
+        const auto of = [&](int i) { return i < p.budget ? i + by : -1; };
+        const int i0 = p.budget - p.recent;
+        MoveRows<LPR> r;
+        if (by >= p.recent) {
+            r.Load(p, b, layer, h, i0 + slice * ROWS, of);
+            r.Store(p, layer);
+        } else if (slice == 0) {
+            for (int n = 0; n < slices; ++n) {
+                r.Load(p, b, layer, h, i0 + n * ROWS, of);
+                __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers
+                __syncthreads();
+                r.Store(p, layer);
+                __syncthreads();
             }
         }
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u)
-            if (to[u] >= 0) {
-                *reinterpret_cast<uint4 *>(k + to[u]) = x[u][0];
-                *reinterpret_cast<uint4 *>(v + to[u]) = x[u][1];
-            }
-        __syncthreads();
-    }
+    });
 }
 
 }  // namespace
@@ -335,21 +589,26 @@ void EvictLaunch(const kr_cache *cache, const kr_seqs *s, const kr_weights *weig
     const MemSpan ks{c.k, all}, vs{c.v, all};
     if (Meets(list, ws) || Meets(list, ks) || Meets(list, vs) || Meets(ws, ks) || Meets(ws, vs))
         refuse("keep, the weights and the cache overlap");
-    const int lpr = c.head_dim / 8, per = kMoveRows * (256 / lpr);
-    const int slices = (budget - recent - sinks + per - 1) / per;
-    if (units * std::max(slices, 1) >= (kMaxGrid >> 2)) refuse("too many sequences");
-    hipLaunchKernelGGL(SelectKernel, dim3(unsigned(units), unsigned(c.layers)), dim3(kSelThreads), 0, stream, p);
+    if (units >= (kMaxGrid >> 2)) refuse("too many sequences");
+    // the middle of the longest sequence that there is room for
+    const int64_t middle = std::min<int64_t>(cap, w.width) - sinks - recent;
+    const dim3 lists(unsigned(units), unsigned(c.layers));
+    const auto select = [&](auto kern, int nt) { hipLaunchKernelGGL(kern, lists, dim3(unsigned(nt)), 0, stream, p); };
+    if (middle <= 256) select(SelectKernel<64, 4>, 64);
+    else if (middle <= 1024) select(SelectKernel<256, 4>, 256);
+    else if (middle <= 4096) select(SelectKernel<256, 16>, 256);
+    else if (middle <= 16384) select(SelectKernel<1024, 16>, 1024);
+    else if (middle <= 32768) select(SelectKernel<1024, 32>, 1024);
+    else select(SelectLongKernel<16>, 1024);
     Check(hipGetLastError(), "cache_evict launch");
-    if (slices > 0) {
-        const dim3 grid(unsigned(units) * unsigned(slices), unsigned(c.layers));
-        if (lpr == 8) hipLaunchKernelGGL((MoveKernel<8>), grid, dim3(256), 0, stream, p, slices);
-        else hipLaunchKernelGGL((MoveKernel<16>), grid, dim3(256), 0, stream, p, slices);
-    }
-    if (recent > 0) {
-        const dim3 grid(unsigned(units), unsigned(c.layers));
-        if (lpr == 8) hipLaunchKernelGGL((ShiftKernel<8>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((ShiftKernel<16>), grid, dim3(256), 0, stream, p);
-    }
+    const int lpr = c.head_dim / 8, per = kMoveRows * (256 / lpr);
+    const auto move = [&](auto kern, int places) {
+        const int slices = (places + per - 1) / per;
+        const dim3 grid(unsigned(std::min<int64_t>(units * c.layers * slices, kMoveGroups)));
+        if (slices > 0) hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p, slices);
+    };
+    lpr == 8 ? move(MoveKernel<8>, budget - recent - sinks) : move(MoveKernel<16>, budget - recent - sinks);
+    lpr == 8 ? move(ShiftKernel<8>, recent) : move(ShiftKernel<16>, recent);
     Check(hipGetLastError(), "cache_evict launch");
 }
 
