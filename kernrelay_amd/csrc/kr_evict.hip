@@ -290,11 +290,13 @@ __global__ void __launch_bounds__(NT) SelectKernel(EvictParams p)
     Recent<NT>(p, len, keep, w);
 }
 
-// Longer middles: tiles of 1024 x IT tokens, read again for each step.
-template <int IT>
-__global__ void __launch_bounds__(1024) SelectLongKernel(EvictParams p)
+// Longer middles: tiles of 8192 tokens, read again for each step; two workgroups
+// a CU. (288 middles of 31483: 70 us; in registers, 32 tokens a thread and one
+// workgroup a CU, 66, but tiles of 16384 99.)
+__global__ void __attribute__((amdgpu_flat_work_group_size(1024, 1024), amdgpu_waves_per_eu(8)))
+SelectLongKernel(EvictParams p)
 {
-    constexpr int NT = 1024, NW = NT / 64, TILE = NT * IT, CP = 4;
+    constexpr int NT = 1024, IT = 8, NW = NT / 64, TILE = NT * IT, CP = 4;
     __shared__ int hist[2048 * CP];
     __shared__ int part[NW];
     __shared__ int found[3];
@@ -421,8 +423,9 @@ __device__ __forceinline__ int64_t RowAt(const EvictParams &p, const int32_t *ta
     return id * p.page_stride + int64_t(pos - pg * p.div.size) * p.token_stride + col;
 }
 
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMoveRows = 4;       // rows of a thread
-constexpr int kMoveGroups = 2048;  // workgroups: eight on each of 256 CUs
+constexpr int kMoveGroups = 4096;  // workgroups: 16 for each of 256 CUs
 
 // The sequences that lose tokens, 64 at a time: body(b, unit) for this
 // workgroup's share of the `per` units of each of them. (Most of a batch that is
@@ -448,11 +451,12 @@ __device__ __forceinline__ void EachUnit(const EvictParams &p, int64_t per, F &&
 }
 
 // Rows of K and V of a sequence and head in one layer that move together: four
-// a thread, LPR lanes a row. All loads go out before the first store.
+// a thread, LPR lanes a row. All loads go out before the first store, and the
+// stores do not stay in the L2, which the reads need.
 template <int LPR>
 struct MoveRows {
     static constexpr int RPS = 256 / LPR, ROWS = kMoveRows * RPS;
-    uint4 x[kMoveRows][2];
+    U32x4 x[kMoveRows][2];
     int64_t to[kMoveRows];
     // place i0 + n gets the row of token of(place); -1: stays
     template <typename F>
@@ -472,8 +476,8 @@ struct MoveRows {
 #pragma unroll
         for (int n = 0; n < kMoveRows; ++n)
             if (to[n] >= 0) {
-                x[n][0] = *reinterpret_cast<const uint4 *>(k + from[n]);
-                x[n][1] = *reinterpret_cast<const uint4 *>(v + from[n]);
+                x[n][0] = *reinterpret_cast<const U32x4 *>(k + from[n]);
+                x[n][1] = *reinterpret_cast<const U32x4 *>(v + from[n]);
             }
         asm volatile("" ::: "memory");  // (a row's store would join its load)
     }
@@ -483,8 +487,8 @@ struct MoveRows {
 #pragma unroll
         for (int n = 0; n < kMoveRows; ++n)
             if (to[n] >= 0) {
-                *reinterpret_cast<uint4 *>(k + to[n]) = x[n][0];
-                *reinterpret_cast<uint4 *>(v + to[n]) = x[n][1];
+                __builtin_nontemporal_store(x[n][0], reinterpret_cast<U32x4 *>(k + to[n]));
+                __builtin_nontemporal_store(x[n][1], reinterpret_cast<U32x4 *>(v + to[n]));
             }
     }
 };
@@ -598,8 +602,7 @@ void EvictLaunch(const kr_cache *cache, const kr_seqs *s, const kr_weights *weig
     else if (middle <= 1024) select(SelectKernel<256, 4>, 256);
     else if (middle <= 4096) select(SelectKernel<256, 16>, 256);
     else if (middle <= 16384) select(SelectKernel<1024, 16>, 1024);
-    else if (middle <= 32768) select(SelectKernel<1024, 32>, 1024);
-    else select(SelectLongKernel<16>, 1024);
+    else select(SelectLongKernel, 1024);
     Check(hipGetLastError(), "cache_evict launch");
     const int lpr = c.head_dim / 8, per = kMoveRows * (256 / lpr);
     const auto move = [&](auto kern, int places) {
