@@ -405,6 +405,185 @@ WeighKernel(WeighParams p)
     }
 }
 
+// ------------------------------------------------------- at most 32 rows a head
+// A wave has a run of 32-key blocks, key head by key head. Keys go HBM -> LDS by
+// the DMA, whole rows side by side (a lane for each 16 bytes of a row: loads
+// straight to the product's registers, 32 rows at a time, reached 3.7 TB/s of
+// 197 MB, these 5), a ring of kStepStages blocks for each wave, and nobody
+// waits for another wave. The old weights come the same way, so that the loop
+// holds no load that the compiler would wait for. Up to kStepRun blocks of a key
+// head make a run, whose page ids are read at its start.
+constexpr int kStepStages = 2;
+constexpr int kStepRun = 16;       // blocks
+constexpr int kStepGroups = 512;   // workgroups of four waves: two on each of 256 CUs
+
+template <int DT, int D, bool PLAIN>
+__global__ void __launch_bounds__(256) StepKernel(WeighParams p)
+{
+    constexpr int NS = kStepStages;
+    constexpr int DCH = D / 8;       // 16-byte chunks per row
+    constexpr int RPD = 64 / DCH;    // rows per 1 KB DMA block
+    constexpr int NDMA = 32 / RPD;   // DMA blocks of a stage
+    constexpr int VM = NDMA + 1;     // DMA instructions of a stage
+    __shared__ __attribute__((aligned(1024))) uint16_t ring[4][NS][32 * D];
+    __shared__ __attribute__((aligned(256))) float wring[4][NS][64];
+    __shared__ int64_t offs[4][32];
+    __shared__ int32_t tab[4][kStepRun * 32];
+    const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
+    const int hf = lane >> 5, l32 = lane & 31;
+    const auto blocks_of = [&](const WeighSeq &s) { return (s.cols + 31) / 32; };
+    int total = 0;
+    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+        int u = b0 + lane < p.seqs ? p.HKV * blocks_of(LoadSeq(p, b0 + lane)) : 0;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
+        total += Uni(u);
+    }
+    const int waves = 4 * int(gridDim.x), share = (total + waves - 1) / waves;
+    int x = (4 * int(blockIdx.x) + wave) * share;
+    const int x_end = min(x + share, total);
+    if (x >= x_end) return;
+    int b = 0, base = 0;
+    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+        const int u = b0 + lane < p.seqs ? p.HKV * blocks_of(LoadSeq(p, b0 + lane)) : 0;
+        const int incl = WaveScan(u, lane) + base;
+        const uint64_t above = __ballot(incl > x);
+        const int at = above != 0 ? __builtin_ctzll(above) : 63;
+        base = Uni(__shfl(incl - (above != 0 ? u : 0), at, 64));
+        if (above != 0) {
+            b = b0 + at;
+            break;
+        }
+    }
+    WeighSeq sq = LoadSeq(p, b);
+    const bool causal = PLAIN || p.tree == nullptr || p.path != nullptr;
+    const int kaddr = l32 * D + KSlot<D>(l32, hf) * 8;  // step dc: XOR 16 dc
+    while (x < x_end) {
+        while (x >= base + p.HKV * blocks_of(sq)) {
+            base += p.HKV * blocks_of(sq);
+            sq = LoadSeq(p, ++b);
+        }
+        // ---- a run: blocks t0 .. t0 + ns - 1 of key head h
+        const int per = blocks_of(sq);
+        const int h = Uni((x - base) / per), t0 = x - base - h * per;
+        const int ns = Uni(min(min(per - t0, x_end - x), kStepRun));
+        const int pg0 = Uni(PageOf(p.div, t0 * 32));
+        const int npg = Uni(PageOf(p.div, min((t0 + ns) * 32, sq.total) - 1)) - pg0 + 1;
+        for (int i = lane; i < npg; i += 64) tab[wave][i] = p.table[b * p.ld_table + pg0 + i];
+        // rows: lane l has row l % 32, registers v row 8 (v / 4) + 4 hf + v % 4
+        const int R = (sq.n - sq.skip) * p.G;
+        const int i32 = sq.skip + PageOf(p.group, min(l32, R - 1));  // new token of row l % 32
+        const int g = min(l32, R - 1) - (i32 - sq.skip) * p.G;
+        int tok = i32;
+        if (!PLAIN && p.path != nullptr) tok = p.path[b * p.ld_path + i32];
+        const bool live = l32 < R && tok >= 0 && tok < sq.rows;
+        const int64_t row = sq.first + (live ? tok : 0);
+        uint4 qf[D / 16];
+        {
+            const uint16_t *q = p.q + row * p.ldq + int64_t(h * p.G + g) * D + hf * 8;
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) qf[dc] = *reinterpret_cast<const uint4 *>(q + dc * 16);
+        }
+        const float lse = live ? p.lse[row * p.ld_lse + h * p.G + g] : -INFINITY;
+        const uint32_t counts = uint32_t(__ballot(lse != -INFINITY));  // rows that count
+        float nl[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) nl[v] = __shfl(lse == -INFINITY ? -INFINITY : lse * -kLog2E, 8 * (v >> 2) + 4 * hf + (v & 3), 64);
+        // (used here: see the attention's kernel)
+#pragma unroll
+        for (int dc = 0; dc < D / 16; ++dc) {
+            typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+            U32x4 v = __builtin_bit_cast(U32x4, qf[dc]);
+            asm volatile("" : "+v"(v));
+            qf[dc] = __builtin_bit_cast(uint4, v);
+        }
+        const uint16_t *kh = p.k + h * p.head_stride;
+        float *wh = p.w + int64_t(sq.entry) * p.w_entry + int64_t(h) * p.w_head;
+        KR_WAIT_VM(0);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        uint32_t there[NS];  // keys that are there: of the stage worked on and those in flight
+        const auto fetch = [&](int st) -> uint32_t {
+            const int pos = (t0 + st) * 32 + l32;
+            const int pg = PageOf(p.div, min(pos, sq.total - 1));
+            const int id = tab[wave][pg - pg0];
+            const bool ok = pos < sq.total && uint32_t(id) < uint32_t(p.pages);
+            const int64_t off = int64_t(uint64_t(uint32_t(id)) * p.page_stride +
+                                        uint64_t(uint32_t(pos - pg * p.div.size)) * p.token_stride);
+            offs[wave][l32] = ok ? off : 0;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const uint32_t dst = LdsAddr(&ring[wave][st % NS][0]);
+#pragma unroll
+            for (int j = 0; j < NDMA; ++j) {
+                const int r = j * RPD + lane / DCH;
+                DmaLoad16(kh + offs[wave][r] + KSlot<D>(r, lane % DCH) * 8, dst + uint32_t(j) * 1024u);
+            }
+            DmaTouch4(wh + min(pos, sq.cols - 1), LdsAddr(&wring[wave][st % NS][0]));
+            return uint32_t(__ballot(ok));
+        };
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) there[i] = i < ns ? fetch(i) : 0u;
+        for (int st = 0; st < ns; ++st) {
+            if (st + NS - 1 < ns) {
+                there[NS - 1] = fetch(st + NS - 1);
+                KR_WAIT_VM((NS - 1) * VM);
+            } else {
+                KR_WAIT_VM(0);  // (the last stages of a run)
+            }
+            const uint16_t *K = &ring[wave][st % NS][0];
+            const int j0 = (t0 + st) * 32, nj = j0 - sq.len;  // the first key, and as a new token
+            f32x16 s;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc)
+                s = Mfma<DT>(qf[dc], *reinterpret_cast<const uint4 *>(K + (kaddr ^ (dc * 16))), s);
+            const bool ok = ((there[0] >> l32) & 1) != 0;
+            // do all rows count, and see every key? (Those past the last repeat it with weight 0.)
+            const bool whole = there[0] == ~0u && nj + 32 <= (causal ? sq.skip + 1 : 0) && counts == (~0u >> (32 - min(R, 32)));
+            float sum = 0.0f;
+#pragma unroll
+            for (int v4 = 0; v4 < 4; ++v4) {
+                if (8 * v4 >= R) break;
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * v4 + i], p.scale_log2, nl[4 * v4 + i]));
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * v4 + 4 * hf + i;
+                        bool sees = ok && ((counts >> r) & 1) != 0;
+                        if (nj + 32 > (causal ? sq.skip + 1 : 0)) {
+                            const int at = sq.skip + PageOf(p.group, min(r, R - 1)), k = nj + l32;
+                            if (causal) {
+                                sees = sees && k <= at;
+                            } else if (sees && k >= 0) {
+                                const uint64_t w = (k >> 6) < p.tree_words
+                                                       ? p.tree[int64_t(sq.first + at) * p.ld_tree + (k >> 6)]
+                                                       : 0ull;
+                                sees = ((w >> (k & 63)) & 1) != 0;
+                            }
+                        }
+                        e[i] = sees ? e[i] : 0.0f;
+                    }
+                }
+                sum += (e[0] + e[1]) + (e[2] + e[3]);
+            }
+            sum += __shfl_xor(sum, 32, 64);
+            const int key = j0 + l32;
+            const float old = wring[wave][st % NS][lane];
+            if (hf == 0 && key < sq.cols) wh[key] = (key < sq.len && p.decay != 0.0f ? p.decay * old : 0.0f) + sum;
+#pragma unroll
+            for (int i = 0; i + 1 < NS; ++i) there[i] = there[i + 1];
+        }
+        x += ns;
+    }
+}
+
 // Tiles that came in pieces: workgroup i has the one that begins in part i and
 // ends in a later one, slot 1 of that part and slot 0 of the next.
 __global__ void __launch_bounds__(kWeighKeys) WeighJoinKernel(WeighParams p)
@@ -524,8 +703,22 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
         Meets(out, RowsSpan(d.lse, d.rows, p.ld_lse, d.HQ, 4)) || Meets(out, MemSpan{k.p, k.width * 2}) ||
         Meets(out, MemSpan{d.ws, int64_t(need)}))
         refuse("the weights overlap another tensor of the call");
-    const bool one = OneRowTile(tokens, p.G);
-    const dim3 grid(unsigned(one ? std::min<int64_t>(most, kWeighParts) : kWeighParts));
+    if (OneRowTile(tokens, p.G)) {
+        const int64_t blocks = (std::min<int64_t>(cap, w.width) + 31) / 32 * c.heads * s.seqs;
+        const dim3 grid(unsigned(std::min<int64_t>((blocks + 3) / 4, kStepGroups)));
+        const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p); };
+        const bool bf = c.dtype == kBF16;
+        if (s.tree == nullptr && d.path == nullptr) {
+            if (c.head_dim == 64) bf ? go(StepKernel<kBF16, 64, true>) : go(StepKernel<kF16, 64, true>);
+            else bf ? go(StepKernel<kBF16, 128, true>) : go(StepKernel<kF16, 128, true>);
+        } else {
+            if (c.head_dim == 64) bf ? go(StepKernel<kBF16, 64, false>) : go(StepKernel<kF16, 64, false>);
+            else bf ? go(StepKernel<kBF16, 128, false>) : go(StepKernel<kF16, 128, false>);
+        }
+        Check(hipGetLastError(), "attention_paged_weigh launch");
+        return;
+    }
+    const dim3 grid(kWeighParts);
     const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p); };
     const bool bf = c.dtype == kBF16;
     if (s.tree == nullptr && d.path == nullptr) {
@@ -535,7 +728,7 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
         if (c.head_dim == 64) bf ? go(WeighKernel<kBF16, 64, false>) : go(WeighKernel<kF16, 64, false>);
         else bf ? go(WeighKernel<kBF16, 128, false>) : go(WeighKernel<kF16, 128, false>);
     }
-    if (!one) hipLaunchKernelGGL(WeighJoinKernel, grid, dim3(kWeighKeys), 0, stream, p);
+    hipLaunchKernelGGL(WeighJoinKernel, grid, dim3(kWeighKeys), 0, stream, p);
     Check(hipGetLastError(), "attention_paged_weigh launch");
 }
 
