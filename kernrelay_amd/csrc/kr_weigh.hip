@@ -195,6 +195,23 @@ __device__ __forceinline__ int WeighFind(const WeighParams &p, int lane, int x, 
     return 0;
 }
 
+// A wave's own LDS writes before its other lanes' reads of them.
+__device__ __forceinline__ void WaveLdsOrder()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A loaded value is needed here: the wait for it stands no further down.
+__device__ __forceinline__ void Used(uint4 &x)
+{
+    typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+    U32x4 v = __builtin_bit_cast(U32x4, x);
+    asm volatile("" : "+v"(v));
+    x = __builtin_bit_cast(uint4, v);
+}
+
 // A key's sum to its column.
 __device__ __forceinline__ void PutWeight(const WeighParams &p, const WeighSeq &s, int h, int key, float got)
 {
@@ -216,6 +233,7 @@ WeighKernel(WeighParams p)
     constexpr int DPW = 32 / RPD / 4;     // DMA blocks per wave and row tile
     __shared__ __attribute__((aligned(1024))) uint16_t qring[NS][32 * D];
     __shared__ __attribute__((aligned(256))) float lring[4][NS][64];  // a wave's own: lse of the tile's rows, twice
+    __shared__ int64_t rows[4][32];                                  // and where its rows' queries are
     const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
     const int hf = lane >> 5;
     const int total = WeighTotal(p, lane);
@@ -231,6 +249,8 @@ WeighKernel(WeighParams p)
     const int qaddr = (lane & 31) * D + KSlot<D>(lane & 31, hf) * 8;  // step dc: XOR 16 dc
     // 32 packed rows on: so many tokens and query heads
     const int step_tok = 32 / p.G, step_g = 32 - step_tok * p.G;
+    const int64_t step_q = step_tok * p.ldq + step_g * D, step_qw = step_q + p.ldq - p.G * D;
+    const int64_t step_l = step_tok * p.ld_lse + step_g, step_lw = step_l + p.ld_lse - p.G;
     while (x < x_end) {
         while (sq.cols == 0 || x >= base + p.HKV * line.Head()) {
             if (sq.cols > 0) base += p.HKV * line.Head();
@@ -260,8 +280,11 @@ WeighKernel(WeighParams p)
             there |= ok ? 1u << kb : 0u;
             all = all && __ballot(!ok) == 0;
         }
-        // packed row r: its row of the launch and query head of the key head
-        const auto row_of = [&](int r, int &g) {
+        // packed row r of the unit, r = lane % 32 of a tile: where its query and lse
+        // are; from tile to tile the addresses go on by as many tokens and heads
+        int64_t qo = 0, lo = 0;  // elements
+        int g = 0;
+        const auto point = [&](int r) {
             const int i = PageOf(p.group, r);
             g = r - i * p.G;
             int tok = sq.skip + i;
@@ -269,66 +292,59 @@ WeighKernel(WeighParams p)
                 tok = p.path[b * p.ld_path + tok];
                 if (tok < 0 || tok >= sq.rows) tok = 0;  // (counts nothing, see below)
             }
-            return int64_t(sq.first + tok);
+            const int64_t row = sq.first + tok;
+            qo = row * p.ldq + int64_t(h * p.G + g) * D;
+            lo = row * p.ld_lse + h * p.G + g;
         };
-        // this lane's chunks of a row tile's rows, and their lse: from tile to
-        // tile the addresses go on by as many tokens and heads
-        const uint16_t *qp[DPW];
-        const float *lp;
-        int qg[DPW], lg;
-        const auto point = [&](int r0) {
+        const auto fetch = [&](int st, int slot) {
+            const int r0 = (rt_lo + st) * 32;
+            if (!PLAIN || st == 0 || r0 + 32 > R) {
+                point(min(r0 + (lane & 31), R - 1));
+            } else {
+                g += step_g;
+                const bool wrap = g >= p.G;
+                g -= wrap ? p.G : 0;
+                qo += wrap ? step_qw : step_q;
+                lo += wrap ? step_lw : step_l;
+            }
+            if (lane < 32) rows[wave][lane] = qo;
+            WaveLdsOrder();
+            const uint32_t dst = LdsAddr(&qring[slot][0]) + uint32_t(wave * DPW) * 1024u;
 #pragma unroll
             for (int j = 0; j < DPW; ++j) {
                 const int r = (wave * DPW + j) * RPD + lane / DCH;
-                const int64_t row = row_of(min(r0 + r, R - 1), qg[j]);
-                qp[j] = p.q + row * p.ldq + int64_t(h * p.G + qg[j]) * D + KSlot<D>(r, lane % DCH) * 8;
+                DmaLoad16(p.q + rows[wave][r] + KSlot<D>(r, lane % DCH) * 8, dst + uint32_t(j) * 1024u);
             }
-            const int64_t row = row_of(min(r0 + (lane & 31), R - 1), lg);
-            lp = p.lse + row * p.ld_lse + h * p.G + lg;
-        };
-        const auto fetch = [&](int st) {
-            const int r0 = (rt_lo + st) * 32;
-            if (!PLAIN || st == 0 || r0 + 32 > R) {
-                point(r0);
-            } else {
-#pragma unroll
-                for (int j = 0; j < DPW; ++j) {
-                    qg[j] += step_g;
-                    const bool wrap = qg[j] >= p.G;
-                    qg[j] -= wrap ? p.G : 0;
-                    qp[j] += step_tok * p.ldq + step_g * D + (wrap ? p.ldq - p.G * D : 0);
-                }
-                lg += step_g;
-                const bool wrap = lg >= p.G;
-                lg -= wrap ? p.G : 0;
-                lp += step_tok * p.ld_lse + step_g + (wrap ? p.ld_lse - p.G : 0);
-            }
-            const uint32_t dst = LdsAddr(&qring[st % NS][0]) + uint32_t(wave * DPW) * 1024u;
-#pragma unroll
-            for (int j = 0; j < DPW; ++j) DmaLoad16(qp[j], dst + uint32_t(j) * 1024u);
-            DmaTouch4(lp, LdsAddr(&lring[wave][st % NS][0]));
+            DmaTouch4(p.lse + lo, LdsAddr(&lring[wave][slot][0]));
         };
         const int ns = rt_hi - rt_lo;
         __syncthreads();  // (the rings are free)
-        fetch(0);
-        if (ns > 1) fetch(1);
+        fetch(0, 0);
+        if (ns > 1) fetch(1, 1);
         uint4 kf[KB][D / 16];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int dc = 0; dc < D / 16; ++dc) kf[kb][dc] = *reinterpret_cast<const uint4 *>(kr[kb] + dc * 16);
+        // (used here: a load that the compiler still counts in the loop would make
+        // it wait for the DMA there, tile by tile: 205 us for 100 over a prompt's chunk)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) Used(kf[kb][dc]);
         float sum[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) sum[kb] = 0.0f;
         const int nj = j0 - sq.len;  // the first key as a new token
-        for (int st = 0; st < ns; ++st) {
+        static_assert(NS == 3, "slots");
+        for (int st = 0, slot = 0; st < ns; ++st, slot = slot == NS - 1 ? 0 : slot + 1) {
             if (st + 1 < ns) KR_WAIT_VM(DPW + 1);
             else KR_WAIT_VM(0);
             __syncthreads();
-            if (st + 2 < ns) fetch(st + 2);
+            if (st + 2 < ns) fetch(st + 2, slot == 0 ? NS - 1 : slot - 1);
             const int r0 = (rt_lo + st) * 32;
-            const uint16_t *Q = &qring[st % NS][0];
-            const float *ls = &lring[wave][st % NS][0];
+            const uint16_t *Q = &qring[0][0] + slot * (32 * D);
+            const float *ls = &lring[wave][0][0] + slot * 64;
             // rows that see nothing of the wave's keys, or all of them
             const int tok_lo = sq.skip + Uni(PageOf(p.group, r0));
             const int tok_hi = sq.skip + Uni(PageOf(p.group, min(r0 + 31, R - 1)));
@@ -347,7 +363,9 @@ WeighKernel(WeighParams p)
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) s[kb] = Mfma<DT>(qf, kf[kb][dc], s[kb]);
             }
-            // register v: row 8 (v / 4) + 4 hf + v % 4
+            // register v: row 8 (v / 4) + 4 hf + v % 4. The wave in its
+            // exponentials goes first, as in the attention's kernels.
+            __builtin_amdgcn_s_setprio(2);
             if (whole) {
 #pragma unroll
                 for (int v4 = 0; v4 < 4; ++v4) {
@@ -390,6 +408,7 @@ WeighKernel(WeighParams p)
                     }
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
         }
         // ---- the two halves of a key's rows, and where its sum goes
         const bool cut = x > pc.start || x + ns < pc.start + pc.rows;
@@ -489,20 +508,12 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
         float nl[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) nl[v] = __shfl(lse == -INFINITY ? -INFINITY : lse * -kLog2E, 8 * (v >> 2) + 4 * hf + (v & 3), 64);
-        // (used here: see the attention's kernel)
 #pragma unroll
-        for (int dc = 0; dc < D / 16; ++dc) {
-            typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-            U32x4 v = __builtin_bit_cast(U32x4, qf[dc]);
-            asm volatile("" : "+v"(v));
-            qf[dc] = __builtin_bit_cast(uint4, v);
-        }
+        for (int dc = 0; dc < D / 16; ++dc) Used(qf[dc]);
         const uint16_t *kh = p.k + h * p.head_stride;
         float *wh = p.w + int64_t(sq.entry) * p.w_entry + int64_t(h) * p.w_head;
         KR_WAIT_VM(0);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        WaveLdsOrder();
         uint32_t there[NS];  // keys that are there: of the stage worked on and those in flight
         const auto fetch = [&](int st) -> uint32_t {
             const int pos = (t0 + st) * 32 + l32;
@@ -512,9 +523,7 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
             const int64_t off = int64_t(uint64_t(uint32_t(id)) * p.page_stride +
                                         uint64_t(uint32_t(pos - pg * p.div.size)) * p.token_stride);
             offs[wave][l32] = ok ? off : 0;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            WaveLdsOrder();
             const uint32_t dst = LdsAddr(&ring[wave][st % NS][0]);
 #pragma unroll
             for (int j = 0; j < NDMA; ++j) {
