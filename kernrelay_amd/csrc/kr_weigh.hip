@@ -357,11 +357,26 @@ WeighKernel(WeighParams p)
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) s[kb][v] = 0.0f;
+            {
+                // the Q fragment of step dc is read QAH steps ahead of its MFMAs
+                constexpr int NP = D / 16, QAH = 4;
+                uint4 qf[NP];
+                const auto rd = [&](int dc) { qf[dc] = *reinterpret_cast<const uint4 *>(Q + (qaddr ^ (dc * 16))); };
 #pragma unroll
-            for (int dc = 0; dc < D / 16; ++dc) {
-                const uint4 qf = *reinterpret_cast<const uint4 *>(Q + (qaddr ^ (dc * 16)));
+                for (int dc = 0; dc < QAH; ++dc) rd(dc);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[kb] = Mfma<DT>(qf, kf[kb][dc], s[kb]);
+                for (int dc = 0; dc < NP; ++dc) {
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) s[kb] = Mfma<DT>(qf[dc], kf[kb][dc], s[kb]);
+                    if (dc + QAH < NP) rd(dc + QAH);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, QAH, 0);  // 0x100 LDS read, 0x008 MFMA
+#pragma unroll
+                for (int i = 0; i < NP - QAH; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, KB * QAH, 0);
             }
             // register v: row 8 (v / 4) + 4 hf + v % 4. The wave in its
             // exponentials goes first, as in the attention's kernels.
