@@ -15,9 +15,12 @@
 // pieces of 8192 values; the last workgroup of a sequence to arrive walks down
 // its drafts. In the second a workgroup adds up what is left of 2048 values of a
 // sequence's last row, and the last of them to arrive finds the token: its
-// piece, its thread's eight values, its place. Only where several drafts were
-// drawn after one row does the walk need sums over the vocabulary on its way: it
-// is a launch of its own then, a workgroup a sequence.
+// piece, its thread's eight values, its place. Where several drafts were drawn
+// after one row the walk needs sums over the vocabulary on its way, each after a
+// refusal that it cannot foresee: it stops there, and the next launch makes the
+// sums of the sequences that wait for one, by many workgroups each, and goes on
+// (from the top: the steps up to there are a few hundred operations). After
+// kSumRounds such launches a single workgroup makes what sums are left.
 #include <algorithm>
 
 #include "kr_paged.h"
@@ -32,6 +35,10 @@ constexpr int kMostNew = 1024;  // tokens of a sequence
 // Counters of a sequence, the first of them used: arrivals at one line of memory
 // wait for each other (15 ns each, 32 sequences on a line: 90 us for 53).
 constexpr int kCounters = 32;
+// Launches that make sums for sampled trees. One that finds nothing to do costs
+// 2.5 us, one with work 9, a sum by a single workgroup 10 us (32003 tokens) to
+// 45 (152064).
+constexpr int kSumRounds = 3;
 constexpr int kNone = -1;       // the type of draft probabilities that are not there
 
 struct RowPart {
@@ -42,6 +49,8 @@ struct RowPart {
 struct SeqEnd {
     int row;      // where the walk ended: a row of the sequence
     int refused;  // drafts that were refused there
+    int waits;    // the last of them, if the walk waits for the sum after it; else -1
+    int pad;
     RowPart stats;
 };
 struct VerifyParams {
@@ -55,6 +64,7 @@ struct VerifyParams {
     int vocab, rows, seqs, max_new, width, pieces, end_pieces;
     RowPart *parts;         // [rows, pieces]
     double *totals;         // [rows]: of a sequence's end row, the sums after its refusals
+    double *after;          // [rows]: the sum after the refusal of this draft; -1: not known
     int32_t *refused;       // [rows]: the tokens refused there
     SeqEnd *ends;           // [seqs]
     double *sums;           // [seqs, end_pieces]: of what is left at the end row
@@ -273,13 +283,18 @@ struct WalkLds {
     }
 };
 
+// What a walk does where it needs the sum over the vocabulary after a refusal:
+// it never does (one draft a row, or not drawn); it is the first one, and stops;
+// it goes on behind sums that were made meanwhile, and stops at the next one; it
+// makes them.
+enum { kNoSums, kFirst, kResume, kMakes };
+
 // Down the drafts of sequence b, by NT threads that all take the same steps.
-// SUMS: several drafts after one row may have been drawn, so that a refusal's
-// sum over the vocabulary may be needed.
-template <int XT, int QT, int NT, bool SUMS>
+template <int XT, int QT, int NT, int SUMS>
 __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifySeq &sq, double c, const Pow2 &pow2,
                                        const WalkLds &l, double *part)
 {
+    constexpr int QL = QT == kNone ? kF32 : QT;
     const int tid = int(threadIdx.x), lane = tid & 63;
     // ---- drafts: what they follow
     for (int i = tid; i < sq.n; i += NT) {
@@ -288,6 +303,7 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
         l.above[i] = i > 0 && par >= 0 && par < i ? par : -1;
         l.token[i] = tok >= 0 && tok < p.vocab ? int(tok) : -1;
         l.u[i] = p.u[sq.first + i];
+        if (SUMS == kFirst) PutDev(p.after + sq.first + i, -1.0);
     }
     // ---- rows: their pieces put together, eight lanes to a row
     for (int r0 = 0; r0 < sq.n; r0 += NT / 8) {
@@ -331,7 +347,7 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
             const RowPart s = l.stats[par];
             const int64_t row = sq.first + par;
             const float x = Logit(At<XT>(p.logits, row * p.ld_logits + tok));
-            if (QT != kNone) q = float(Chance(At<QT == kNone ? kF32 : QT>(p.draft, row * p.ld_draft + tok)));
+            if (QT != kNone) q = float(Chance(At<QL>(p.draft, row * p.ld_draft + tok)));
             if (s.top != -INFINITY) w = Weight(pow2, x, tok, s.top, s.at, c) / s.sum;
             if (QT == kNone) {
                 // a token that was refused there already has nothing left
@@ -347,7 +363,7 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
     while (len < p.width) {
         refused = 0;
         double rest = 1.0;  // (drafts that were not drawn)
-        int next = -1;
+        int next = -1, gone = -1;
         for (int i0 = (cur + 1) / 64 * 64; i0 < sq.n && next < 0; i0 += 64) {
             uint64_t hit = __ballot(i0 + lane < sq.n && i0 + lane > cur && l.above[min(i0 + lane, sq.n - 1)] == cur);
             while (hit != 0 && next < 0) {
@@ -358,36 +374,47 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
                     ok = double(l.u[i]) * rest < l.prob[i];
                     rest = fmax(rest - l.prob[i], 0.0);
                 } else {
-                    if (SUMS && refused > 0) {
+                    if (SUMS != kNoSums && refused > 0) {
                         // the sum after the last refusal, over the vocabulary
-                        const RowPart s = l.stats[cur];
-                        const int64_t row = sq.first + cur;
-                        const double inv = 1.0 / s.sum;
-                        double sum = 0.0;
-                        for (int v = tid * 8; v < p.vocab; v += NT * 8) {
-                            const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
-                            const Raw8<QT == kNone ? kF32 : QT> q =
-                                Load8<QT == kNone ? kF32 : QT>(p.draft, row * p.ld_draft, v, p.vocab, 0);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                if (s.top == -INFINITY) continue;
-                                double was;
-                                const double w =
-                                    Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, s.top, s.at, c) * inv;
-                                sum += Left(w, Chance(Val<QT == kNone ? kF32 : QT>::Load(q.v[e])), l.totals, refused, was);
-                            }
+                        double sum = SUMS == kFirst ? -1.0 : GetDev(p.after + sq.first + gone);
+                        if (SUMS != kMakes && sum < 0.0) {
+                            for (int k = tid; k + 1 < refused; k += NT) PutDev(p.totals + sq.first + k, l.totals[k]);
+                            if (tid == 0) p.ends[b] = SeqEnd{cur, refused, gone, 0, l.stats[cur]};
+                            return;
                         }
-                        sum = BlockSumD<NT>(sum, part);
+                        if (SUMS == kMakes && sum < 0.0) {
+                            const RowPart s = l.stats[cur];
+                            const int64_t row = sq.first + cur;
+                            const double inv = 1.0 / s.sum;
+                            sum = 0.0;
+                            for (int v = tid * 8; v < p.vocab; v += NT * 8) {
+                                const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
+                                const Raw8<QL> q = Load8<QL>(p.draft, row * p.ld_draft, v, p.vocab, 0);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    if (s.top == -INFINITY) continue;
+                                    double was;
+                                    const double w =
+                                        Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, s.top, s.at, c) * inv;
+                                    sum += Left(w, Chance(Val<QL>::Load(q.v[e])), l.totals, refused, was);
+                                }
+                            }
+                            sum = BlockSumD<NT>(sum, part);
+                        }
                         if (tid == 0) l.totals[refused - 1] = sum;
                         __syncthreads();
                     }
                     double r = l.prob[i];
-                    for (int k = 0; SUMS && k < refused; ++k)
+                    for (int k = 0; SUMS != kNoSums && k < refused; ++k)
                         r = l.totals[k] > 0.0 ? fmax(r - double(l.chance[i]), 0.0) / l.totals[k] : r;
                     ok = double(l.u[i]) * double(l.chance[i]) < r;
                 }
-                if (ok) next = i;
-                else ++refused;
+                if (ok) {
+                    next = i;
+                } else {
+                    ++refused;
+                    gone = i;
+                }
             }
         }
         if (next < 0) break;
@@ -399,11 +426,11 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
     if (tid == 0) {
         p.path[b * p.ld_path] = 0;
         p.path_lens[b] = len;
-        p.ends[b] = SeqEnd{cur, refused, l.stats[cur]};
+        p.ends[b] = SeqEnd{cur, refused, -1, 0, l.stats[cur]};
     }
     for (int i = len + tid; i < p.width; i += NT) p.path[b * p.ld_path + i] = -1;
     if (QT != kNone) {
-        for (int k = tid; SUMS && k + 1 < refused; k += NT) p.totals[sq.first + k] = l.totals[k];
+        for (int k = tid; SUMS != kNoSums && k + 1 < refused; k += NT) PutDev(p.totals + sq.first + k, l.totals[k]);
     } else if (refused > 0 && tid < 64) {  // (all that follow it)
         int at = 0;
         for (int i0 = (cur + 1) / 64 * 64; i0 < sq.n; i0 += 64) {
@@ -425,8 +452,7 @@ __device__ __forceinline__ void NoRows(const VerifyParams &p, int b, int nt)
     }
 }
 
-// Sampled trees: the walk by itself. 1024 threads, as the sums over the
-// vocabulary are made by one workgroup.
+// Sampled trees whose walk still waits: 1024 threads, as the sums are made by one workgroup.
 template <int XT, int QT>
 __global__ void __launch_bounds__(1024) WalkKernel(VerifyParams p)
 {
@@ -435,16 +461,69 @@ __global__ void __launch_bounds__(1024) WalkKernel(VerifyParams p)
     __shared__ double part[16];
     const int b = int(blockIdx.x);
     const VerifySeq sq = LoadSeq(p, b);
-    if (sq.n == 0) return;  // (the next launch says so)
+    if (sq.n == 0 || p.ends[b].waits < 0) return;
     const double c = SlopeOf(p, b);
     pow2.Fill();
     __syncthreads();
-    Walk<XT, QT, 1024, true>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
+    Walk<XT, QT, 1024, kMakes>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
+}
+
+// The sums that walks wait for: a workgroup has a piece of a row, as in the last
+// launch; the last of them goes on with the walk.
+template <int XT, int QT>
+__global__ void __launch_bounds__(256) SumKernel(VerifyParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ Pow2 pow2;
+    __shared__ double part[4];
+    __shared__ int last;
+    const int b = int(blockIdx.x) / p.end_pieces, mine = int(blockIdx.x) - b * p.end_pieces;
+    const int tid = int(threadIdx.x);
+    const VerifySeq sq = LoadSeq(p, b);
+    if (sq.n == 0) return;
+    const SeqEnd end = p.ends[b];
+    if (end.waits < 0) return;
+    const double c = SlopeOf(p, b);
+    pow2.Fill();
+    const int64_t row = sq.first + end.row;
+    const int v = mine * kEndPiece + tid * 8;
+    const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
+    const Raw8<QT> q = Load8<QT>(p.draft, row * p.ld_draft, v, p.vocab, 0);
+    __syncthreads();
+    double sum = 0.0;
+    if (end.stats.top != -INFINITY) {
+        const double inv = 1.0 / end.stats.sum;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            double was;
+            const double w = Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, end.stats.top, end.stats.at, c) * inv;
+            sum += Left(w, Chance(Val<QT>::Load(q.v[e])), p.totals + sq.first, end.refused, was);
+        }
+    }
+    sum = BlockSumD<256>(sum, part);
+    double *sums = p.sums + int64_t(b) * p.end_pieces;
+    if (tid == 0) {
+        PutDev(sums + mine, sum);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
+        last = Arrive(p.cnt + b * kCounters, p.end_pieces);
+    }
+    __syncthreads();
+    if (!last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    sum = 0.0;
+    for (int k = tid; k < p.end_pieces; k += 256) sum += GetDev(sums + k);
+    sum = BlockSumD<256>(sum, part);
+    if (tid == 0) {
+        PutDev(p.after + sq.first + end.waits, sum);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+    __syncthreads();
+    Walk<XT, QT, 256, kResume>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
 }
 
 // ---------------------------------------------------------------- rows
-// WALK: the last workgroup of a sequence walks.
-template <int XT, int QT, bool WALK>
+// The last workgroup of a sequence walks.
+template <int XT, int QT, int SUMS>
 __global__ void __launch_bounds__(256) StatsKernel(VerifyParams p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -522,19 +601,15 @@ __global__ void __launch_bounds__(256) StatsKernel(VerifyParams p)
         }
         sum = BlockSumD<256>(s[0] + s[1], part);
     }
-    if constexpr (!WALK) {
-        if (threadIdx.x == 0) p.parts[int64_t(row) * p.pieces + piece] = RowPart{top, at, sum};
-    } else {
-        if (threadIdx.x == 0) {
-            PutPart(&p.parts[int64_t(row) * p.pieces + piece], RowPart{top, at, sum});
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
-            last = Arrive(p.cnt + b * kCounters, sq.n * p.pieces);
-        }
-        __syncthreads();
-        if (!last) return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        Walk<XT, QT, 256, false>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
+    if (threadIdx.x == 0) {
+        PutPart(&p.parts[int64_t(row) * p.pieces + piece], RowPart{top, at, sum});
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
+        last = Arrive(p.cnt + b * kCounters, sq.n * p.pieces);
     }
+    __syncthreads();
+    if (!last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    Walk<XT, QT, 256, SUMS>(p, b, sq, c, pow2, WalkLds(lds, p.max_new), part);
 }
 
 // ---------------------------------------------------------------- the token
@@ -711,7 +786,7 @@ __global__ void __launch_bounds__(256) NextKernel(VerifyParams p)
 
 struct VerifyShape {
     int pieces, end_pieces;
-    size_t parts, totals, refused, ends, sums, sums8, bytes;
+    size_t parts, totals, after, refused, ends, sums, sums8, bytes;
 };
 
 VerifyShape ShapeOf(const kr_drafts &d, const kr_seqs &s)
@@ -728,6 +803,7 @@ VerifyShape ShapeOf(const kr_drafts &d, const kr_seqs &s)
     };
     f.parts = take(rows * f.pieces * sizeof(RowPart));
     f.totals = take(rows * sizeof(double));
+    f.after = take(rows * sizeof(double));
     f.refused = take(rows * sizeof(int32_t));
     f.ends = take(seqs * sizeof(SeqEnd));
     f.sums = take(seqs * f.end_pieces * sizeof(double));
@@ -742,12 +818,16 @@ void VerifyGo(const VerifyParams &p, hipStream_t stream)
     const dim3 rows(unsigned(p.rows) * unsigned(p.pieces)), ends(unsigned(p.seqs) * unsigned(p.end_pieces));
     const unsigned lds = unsigned(p.max_new) * WalkLds::kBytes;
     if (p.rows > 0 && p.max_new > 0) {
-        if (QT != kNone && p.parents != nullptr) {
-            hipLaunchKernelGGL((StatsKernel<XT, kNone, false>), rows, dim3(256), 0, stream, p);
-            hipLaunchKernelGGL((WalkKernel<XT, QT>), dim3(unsigned(p.seqs)), dim3(1024), lds, stream, p);
-        } else {
-            hipLaunchKernelGGL((StatsKernel<XT, QT, true>), rows, dim3(256), lds, stream, p);
+        if constexpr (QT != kNone) {
+            if (p.parents != nullptr) {
+                hipLaunchKernelGGL((StatsKernel<XT, QT, kFirst>), rows, dim3(256), lds, stream, p);
+                for (int i = 0; i < kSumRounds; ++i)
+                    hipLaunchKernelGGL((SumKernel<XT, QT>), ends, dim3(256), lds, stream, p);
+                hipLaunchKernelGGL((WalkKernel<XT, QT>), dim3(unsigned(p.seqs)), dim3(1024), lds, stream, p);
+            }
         }
+        if (QT == kNone || p.parents == nullptr)
+            hipLaunchKernelGGL((StatsKernel<XT, QT, kNoSums>), rows, dim3(256), lds, stream, p);
     }
     hipLaunchKernelGGL((NextKernel<XT, QT>), ends, dim3(256), 0, stream, p);
 }
@@ -849,6 +929,7 @@ void VerifyLaunch(const kr_drafts *drafts, const kr_seqs *s, const VerifyOut &o,
     char *base = static_cast<char *>(ws);
     p.parts = reinterpret_cast<RowPart *>(base + f.parts);
     p.totals = reinterpret_cast<double *>(base + f.totals);
+    p.after = reinterpret_cast<double *>(base + f.after);
     p.ends = reinterpret_cast<SeqEnd *>(base + f.ends);
     p.sums = reinterpret_cast<double *>(base + f.sums);
     p.sums8 = reinterpret_cast<double *>(base + f.sums8);
