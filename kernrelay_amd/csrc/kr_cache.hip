@@ -54,6 +54,13 @@ RowSpan LayerSpan(const kr_cache &c, const void *base, int layer)
     return s;
 }
 
+bool MeetsSeqs(const MemSpan &out, const kr_seqs &s, int64_t rows)
+{
+    return Meets(out, RowsSpan(s.table, s.seqs, s.ld_table, s.table_pages, 4)) ||
+           Meets(out, RowsSpan(s.lens, 1, 0, s.seqs, 4)) || Meets(out, RowsSpan(s.starts, 1, 0, int64_t(s.seqs) + 1, 4)) ||
+           (s.tree != nullptr && Meets(out, RowsSpan(s.tree, rows, s.ld_tree, s.tree_words, 8)));
+}
+
 kr_cache CheckCache(const kr_cache *c, const char *who)
 {
     if (c == nullptr || c->k == nullptr || c->v == nullptr) Refuse(who, "needs a cache");

@@ -591,8 +591,11 @@ void EvictLaunch(const kr_cache *cache, const kr_seqs *s, const kr_weights *weig
     const MemSpan list{keep, 4 * units * c.layers * budget}, ws = WeightsSpan(w);
     const int64_t all = 2 * ((c.layers - 1) * c.layer_stride + LayerSpan(c, c.k, 0).width);
     const MemSpan ks{c.k, all}, vs{c.v, all};
+    const MemSpan entry = RowsSpan(w.entry, 1, 0, s->seqs, 4);
     if (Meets(list, ws) || Meets(list, ks) || Meets(list, vs) || Meets(ws, ks) || Meets(ws, vs))
         refuse("keep, the weights and the cache overlap");
+    for (const MemSpan &out : {list, ws, ks, vs})
+        if (MeetsSeqs(out, *s, 0) || Meets(out, entry)) refuse("an output overlaps what the handles read");
     if (units >= (kMaxGrid >> 2)) refuse("too many sequences");
     // the middle of the longest sequence that there is room for
     const int64_t middle = std::min<int64_t>(cap, w.width) - sinks - recent;

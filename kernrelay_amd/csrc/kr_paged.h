@@ -120,6 +120,9 @@ inline MemSpan RowsSpan(const void *p, int64_t rows, int64_t ld, int64_t width, 
     return MemSpan{p, rows < 1 ? 0 : ((rows - 1) * ld + width) * size};
 }
 
+// Does an output meet an array that a launch reads through its sequences' handle?
+bool MeetsSeqs(const MemSpan &out, const kr_seqs &s, int64_t rows);
+
 // Throws unless the weights' rows are apart; strides of dimensions of one element become 0.
 kr_weights CheckWeights(const kr_weights *w, const kr_cache &c, const char *who);
 MemSpan WeightsSpan(const kr_weights &w);

@@ -32,9 +32,14 @@ namespace {
 constexpr int kPiece = 8192;    // values of a piece of a row: 32 a thread
 constexpr int kEndPiece = 2048; // of a sequence's last row: 8 a thread
 constexpr int kMostNew = 1024;  // tokens of a sequence
-// Counters of a sequence, the first of them used: arrivals at one line of memory
-// wait for each other (15 ns each, 32 sequences on a line: 90 us for 53).
+// Counters of a sequence, a line of memory: arrivals at one line wait for each
+// other (32 sampled chains of up to 7, all on one line 90 us, on their own 49).
+// The first counts the pieces of its rows, the second those of its end row; the
+// third is 1 from the walk to the end of the call. Where `starts` does not
+// ascend and two sequences claim a row, a walk may not come; the last launch
+// sees that by it, and leaves all of them zero whatever came.
 constexpr int kCounters = 32;
+enum { kRowsDone, kEndDone, kWalked };
 // Launches that make sums for sampled trees. One that finds nothing to do costs
 // 2.5 us, one with work 9, a sum by a single workgroup 10 us (32003 tokens) to
 // 45 (152064).
@@ -449,6 +454,7 @@ __device__ __forceinline__ void NoRows(const VerifyParams &p, int b, int nt)
     if (threadIdx.x == 0) {
         p.path_lens[b] = 0;
         p.next[b] = -1;
+        p.cnt[b * kCounters + kRowsDone] = 0;
     }
 }
 
@@ -461,7 +467,7 @@ __global__ void __launch_bounds__(1024) WalkKernel(VerifyParams p)
     __shared__ double part[16];
     const int b = int(blockIdx.x);
     const VerifySeq sq = LoadSeq(p, b);
-    if (sq.n == 0 || p.ends[b].waits < 0) return;
+    if (sq.n == 0 || p.cnt[b * kCounters + kWalked] == 0 || p.ends[b].waits < 0) return;
     const double c = SlopeOf(p, b);
     pow2.Fill();
     __syncthreads();
@@ -480,7 +486,7 @@ __global__ void __launch_bounds__(256) SumKernel(VerifyParams p)
     const int b = int(blockIdx.x) / p.end_pieces, mine = int(blockIdx.x) - b * p.end_pieces;
     const int tid = int(threadIdx.x);
     const VerifySeq sq = LoadSeq(p, b);
-    if (sq.n == 0) return;
+    if (sq.n == 0 || p.cnt[b * kCounters + kWalked] == 0) return;
     const SeqEnd end = p.ends[b];
     if (end.waits < 0) return;
     const double c = SlopeOf(p, b);
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(256) SumKernel(VerifyParams p)
     if (tid == 0) {
         PutDev(sums + mine, sum);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
-        last = Arrive(p.cnt + b * kCounters, p.end_pieces);
+        last = Arrive(p.cnt + b * kCounters + kEndDone, p.end_pieces);
     }
     __syncthreads();
     if (!last) return;
@@ -604,7 +610,8 @@ __global__ void __launch_bounds__(256) StatsKernel(VerifyParams p)
     if (threadIdx.x == 0) {
         PutPart(&p.parts[int64_t(row) * p.pieces + piece], RowPart{top, at, sum});
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it is written
-        last = Arrive(p.cnt + b * kCounters, sq.n * p.pieces);
+        last = Arrive(p.cnt + b * kCounters + kRowsDone, sq.n * p.pieces);
+        if (last) p.cnt[b * kCounters + kWalked] = 1;
     }
     __syncthreads();
     if (!last) return;
@@ -663,7 +670,7 @@ __global__ void __launch_bounds__(256) NextKernel(VerifyParams p)
     const int b = int(blockIdx.x) / p.end_pieces, mine = int(blockIdx.x) - b * p.end_pieces;
     const int tid = int(threadIdx.x), lane = tid & 63;
     const VerifySeq sq = LoadSeq(p, b);
-    if (sq.n == 0) {
+    if (sq.n == 0 || p.cnt[b * kCounters + kWalked] == 0) {
         if (mine == 0) NoRows(p, b, 256);
         return;
     }
@@ -721,10 +728,11 @@ __global__ void __launch_bounds__(256) NextKernel(VerifyParams p)
         if (tid == 0) PutDev(sums + mine, all);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's sums are written
         __syncthreads();
-        if (tid == 0) last = Arrive(p.cnt + b * kCounters, p.end_pieces);
+        if (tid == 0) last = Arrive(p.cnt + b * kCounters + kEndDone, p.end_pieces);
         __syncthreads();
         if (!last) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        if (tid == 0) p.cnt[b * kCounters + kWalked] = 0;
     }
     const auto total_of = [&] {
         double s = 0.0;

@@ -725,7 +725,10 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     const RowSpan k = LayerSpan(c, c.k, d.layer);
     if (Meets(out, RowsSpan(d.q, d.rows, p.ldq, int64_t(d.HQ) * c.head_dim, 2)) ||
         Meets(out, RowsSpan(d.lse, d.rows, p.ld_lse, d.HQ, 4)) || Meets(out, MemSpan{k.p, k.width * 2}) ||
-        Meets(out, MemSpan{d.ws, int64_t(need)}))
+        Meets(out, MemSpan{d.ws, int64_t(need)}) || MeetsSeqs(out, s, d.rows) ||
+        Meets(out, RowsSpan(w.entry, 1, 0, s.seqs, 4)) ||
+        Meets(out, RowsSpan(d.path, s.seqs, d.ld_path, d.path_width, 4)) ||
+        Meets(out, RowsSpan(d.path_lens, 1, 0, s.seqs, 4)))
         refuse("the weights overlap another tensor of the call");
     if (OneRowTile(tokens, p.G)) {
         const int64_t blocks = (std::min<int64_t>(cap, w.width) + 31) / 32 * c.heads * s.seqs;

@@ -29,14 +29,21 @@ def drafts(**kw):
     return ops.KrDrafts(**f)
 
 
+def far_seqs(**kw):
+    """Arrays away from the cache's and the weights'."""
+    f = dict(table=FAR + (8 << 20), lens=FAR + (9 << 20), starts=FAR + (10 << 20))
+    f.update(kw)
+    return seqs(**f)
+
+
 def weigh(c=None, s=None, w=None, layer=0, q=FAR, ldq=0, lse=FAR + (1 << 20), ld_lse=0, rows=5, HQ=8, scale=0.1, last=0,
           decay=1.0, path=None, ld_path=0, width=0, lens=None):
-    return ops._lib().kr_op_attention_paged_weigh(c or cache(), layer, s or seqs(), q, ldq, lse, ld_lse, rows, HQ, scale,
+    return ops._lib().kr_op_attention_paged_weigh(c or cache(), layer, s or far_seqs(), q, ldq, lse, ld_lse, rows, HQ, scale,
                                                   w or weights(), last, decay, path, ld_path, width, lens, None, 0, None)
 
 
 def evict(c=None, s=None, w=None, budget=10, sinks=0, recent=0, keep=FAR):
-    return ops._lib().kr_op_cache_evict(c or cache(), s or seqs(), w or weights(), budget, sinks, recent, keep, None)
+    return ops._lib().kr_op_cache_evict(c or cache(), s or far_seqs(), w or weights(), budget, sinks, recent, keep, None)
 
 
 def verify(d=None, s=None, path=FAR, ld_path=5, width=5, lens=FAR + (1 << 20), nxt=FAR + (2 << 20), ws=FAR + (3 << 20),
@@ -81,6 +88,10 @@ def test_bad_weights(field, text):
     (dict(decay=-0.5), "decay"), (dict(decay=float("nan")), "decay"), (dict(path=A), "lengths"), (dict(lens=A), "lengths"),
     (dict(path=A, lens=A, width=0), "path rows"), (dict(path=A, lens=A, width=4, ld_path=3), "path rows"),
     (dict(q=W), "overlap"), (dict(lse=W + 4), "overlap"), (dict(w=weights(w=A)), "overlap"),
+    (dict(s=far_seqs(lens=W + 64)), "overlap"), (dict(s=far_seqs(table=W)), "overlap"),
+    (dict(s=far_seqs(starts=W + 4)), "overlap"), (dict(s=far_seqs(tree=W, tree_words=1, ld_tree=1)), "overlap"),
+    (dict(w=weights(entry=W)), "overlap"), (dict(path=W, lens=FAR + (4 << 20), width=4, ld_path=4), "overlap"),
+    (dict(path=FAR + (4 << 20), lens=W, width=4, ld_path=4), "overlap"),
     (dict(s=seqs(table_pages=1 << 27, ld_table=1 << 27)), "too many tokens"),
 ])
 def test_bad_weigh_calls(kw, text):
@@ -92,6 +103,8 @@ def test_bad_weigh_calls(kw, text):
     (dict(sinks=6, recent=5), "fit the budget"), (dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), "fit the budget"),
     (dict(keep=None), "keep"), (dict(keep=FAR + 2), "keep"), (dict(budget=1 << 30), "too large"),
     (dict(keep=W + 64), "overlap"), (dict(keep=A), "overlap"), (dict(w=weights(w=A + 4)), "overlap"),
+    (dict(s=far_seqs(lens=FAR + 8)), "overlap"), (dict(s=far_seqs(table=W)), "overlap"), (dict(s=seqs()), "overlap"),
+    (dict(w=weights(entry=FAR + 4)), "overlap"),
     (dict(s=seqs(table_pages=1 << 27, ld_table=1 << 27)), "too many tokens"),
 ])
 def test_bad_evictions(kw, text):
@@ -136,6 +149,9 @@ def test_lse_is_checked():
     refused(call(lse=FAR + 64), "lse overlaps")
     refused(call(lse=FAR + (1 << 20)), "lse overlaps")
     refused(call(lse=A + 4096), "lse overlaps")
+    s = far_seqs()
+    refused(ops._lib().kr_op_attention_paged_lse(cache(), 0, s, FAR, 0, FAR + (1 << 20), 0, s.lens, 0, 5, 8, 0.1, None, 0,
+                                                 None, 0, None), "lse overlaps")
 
 
 def test_wrappers_refuse_what_the_entries_cannot_see():

@@ -156,6 +156,25 @@ def test_left_alone(gpu):
     x.check(30, 1, 6)
 
 
+def test_lengths_that_are_none(gpu):
+    announce("evict lengths")
+    x = Case(9, [50, 60, 70], width=60)
+    x.lens = [50, 0, 50]
+    table = x.table
+    x.seqs = ops.make_seqs(ints(table), ints([50, -5, 2 ** 31 - 1]), ints([0] * 4), 0)
+    was = [t.clone() for t in (x.k, x.v, x.w)]
+    keep = x.run(30, 1, 6)
+    assert keep[:, 1].eq(-1).all() and bool((keep[:, 2] == torch.arange(30, device="cuda")).all())
+    for layer in range(2):
+        for h in range(2):
+            assert keep[layer, 0, h].tolist() == kept(was[2][layer, x.entry[0], h].tolist(), 50, 30, 1, 6)
+    others = [e for e in range(x.w.shape[1]) if e != x.entry[0]]
+    assert torch.equal(x.w[:, others], was[2][:, others])
+    mine = set(table[0])
+    pages = [p for p in range(x.k.shape[1]) if p not in mine]
+    assert torch.equal(x.k[:, pages], was[0][:, pages]) and torch.equal(x.v[:, pages], was[1][:, pages])
+
+
 def test_no_sequences(gpu):
     x = Case(8, [5])
     seqs = ops.make_seqs(torch.empty(0, 3, dtype=torch.int32, device="cuda"), ints([]), ints([0]), 0)

@@ -247,6 +247,36 @@ def test_nothing_to_verify(gpu):
     assert x.run() == ([], [], [])
 
 
+@pytest.mark.parametrize("draft", [None, F32])
+@pytest.mark.parametrize("tree", [False, True])
+def test_starts_that_do_not_ascend(gpu, draft, tree):
+    """Sequences that claim each other's rows: nothing is read or written outside, what
+    is no walk is none, and the counters serve the next call."""
+    announce("verify starts %s %s" % (draft, tree))
+    x = Case(6, [5, 7, 4, 6], 5000, F32, tree, draft)
+    good = x.run()
+    x.check()
+    n = len(x.news)
+    seqs = ops.make_seqs(torch.zeros(n, 1, dtype=torch.int32, device="cuda"), ints([3] * n), ints([0, 9, 3, 40, -5]), 8)
+    path, lens, nxt = torch.empty(n, 7, dtype=torch.int32, device="cuda"), ints([9] * n), ints([9] * n, torch.int64)
+    nbytes, ncnt = ops.verify_drafts_workspace(seqs, x.x, draft=x.draft)
+    ws, cnt = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda"), torch.zeros(ncnt, dtype=torch.int32, device="cuda")
+
+    def call(s, p):
+        ops.verify_drafts(s, x.x, x.tokens, x.u, x.u_next, p, lens, nxt, ws, cnt, parents=x.parents, draft=x.draft,
+                          temperature=torch.tensor(x.temps, device="cuda"))
+
+    for _ in range(2):
+        call(seqs, path)
+        assert not bool(cnt.any())
+        # (rows 0 to 7 are the first's; the second has none, the third's are the first's in part)
+        assert lens[0] >= 1 and lens[1].item() == 0 and lens[3].item() == 0
+        assert path[1].tolist() == [-1] * 7 and nxt[1].item() == -1 and nxt[3].item() == -1
+        wide = torch.empty(n, x.width, dtype=torch.int32, device="cuda")
+        call(x.handle(), wide)
+        assert (wide.tolist(), lens.tolist(), nxt.tolist()) == good
+
+
 @pytest.mark.parametrize("draft", [None, BF])
 def test_many_sequences(gpu, draft):
     announce("verify many")

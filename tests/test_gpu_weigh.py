@@ -201,9 +201,10 @@ def test_last_and_decay(gpu, last, decay):
     check_weigh(x, 0, w[0], old[0], [0, 1, 2], lse.float(), scale=0.3, last=last, decay=decay)
 
 
+@pytest.mark.parametrize("last", [0, 2])
 @pytest.mark.parametrize("tree", [False, True])
-def test_accepted_paths(gpu, tree):
-    announce("weigh paths %s" % tree)
+def test_accepted_paths(gpu, tree, last):
+    announce("weigh paths %s %d" % (tree, last))
     x = Batch(5, [130, 0, 61, 9], [24, 9, 70, 4], 14, 2, 64, page=8, tree=tree)
     paths = [[0, 2, 5, 23], [0], [0, 1, 64, 69, 70, -3], []]  # (two that name no row count nothing)
     width = 8
@@ -211,8 +212,30 @@ def test_accepted_paths(gpu, tree):
     w = torch.rand(2, 4, 2, 150, device="cuda", generator=x.g)
     old = w.clone()
     path = ints([p + [-1] * (width - len(p)) for p in paths])
-    weigh(x, 1, w, lse.float(), path=path, path_lens=ints([len(p) for p in paths]))
-    check_weigh(x, 1, w[1], old[1], [0, 1, 2, 3], lse.float(), paths=paths)
+    weigh(x, 1, w, lse.float(), path=path, path_lens=ints([len(p) for p in paths]), last=last)
+    check_weigh(x, 1, w[1], old[1], [0, 1, 2, 3], lse.float(), paths=paths, last=last)
+
+
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_narrow_weights_and_odd_batches(gpu, rows):
+    """Columns for some of the tokens only; starts that do not ascend and lengths that are
+    none leave everything inside."""
+    announce("weigh narrow %s" % rows)
+    x = Batch(8, [300, 40, 90], [3, 2, 1] if rows == "few" else [60, 2, 41], 8, 2, 64, page=8)
+    lse, _ = x.lse(0, x.D ** -0.5)
+    pad = torch.full((2, 5, 2, 140), 3.5, device="cuda")
+    w = pad[:, 1:4, :, :129]
+    weigh(x, 0, w, lse.float())
+    check_weigh(x, 0, w[0], torch.full_like(w[0], 3.5), [0, 1, 2], lse.float())
+    pad[:, 1:4, :, :129] = 3.5
+    assert bool((pad == 3.5).all())
+    n = x.q.shape[0]
+    for lens, starts in (([2 ** 31 - 1, -7, 90], [0, 1, 2, n]), ([300, 40, 90], [n, 0, -9, 2 ** 31 - 1]),
+                         ([300, 40, 90], [5, 2, n + 100, 1])):
+        x.seqs = ops.make_seqs(ints(x.table), ints(lens), ints(starts), max(x.news))
+        weigh(x, 0, w, lse.float(), ints([0, 2, 1]))
+        pad[:, 1:4, :, :129] = 3.5
+        assert bool((pad == 3.5).all())
 
 
 def test_what_nobody_sees(gpu):
