@@ -14,6 +14,14 @@
 //
 // The first launch finds the K-th largest weight by its bits from the top, then
 // lists holes and movers; the second and third move the rows.
+//
+// What bounds it, on an MI355X: the moves by HBM, the lists by the steps of their
+// selection, one after the other. Eight sequences of 1500..3000 tokens down to
+// 1000, 28 layers of 4 heads of 128: lists 19 us, holes 79, the 100 recent tokens
+// 24. One of 32000 down to 4000, 36 layers of 8 heads: 71, 99 and (501) 34. Sixteen
+// of 265..530 down to 512, the same heads: 18, 24 and (128) 42. The rows at the
+// holes are scattered, 256 bytes a key and head: 3.9 TB/s of them, where a large
+// copy reaches 4.9.
 #include <algorithm>
 
 #include "kr_dma.h"
@@ -163,7 +171,11 @@ __device__ __forceinline__ void Recent(const EvictParams &p, int len, int32_t *k
 
 // A list by NT threads that hold all of the middle: thread t tokens sinks + t +
 // NT i. A wave alone finds the threshold bit by bit with ballots, more of them by
-// histograms. Ranks come from one scan over the items' waves.
+// histograms. Ranks come from one scan over the items' waves. The choice of NT and
+// IT, measured on all lists of a launch (lists, tokens of the longest middle): 4608
+// of 232: <64, 4> 41.6 us, <256, 4> 45.3; 4608 of 832: <256, 4> 136, <64, 16> 144;
+// 896 of 3832: <256, 16> 48.5, <1024, 4> 67; 576 of 14900: <1024, 16> 72,
+// SelectLongKernel 84.
 template <int NT, int IT>
 __global__ void __launch_bounds__(NT) SelectKernel(EvictParams p)
 {
@@ -292,7 +304,9 @@ __global__ void __launch_bounds__(NT) SelectKernel(EvictParams p)
 
 // Longer middles: tiles of 8192 tokens, read again for each step; two workgroups
 // a CU. (288 middles of 31483: 70 us; in registers, 32 tokens a thread and one
-// workgroup a CU, 66, but tiles of 16384 99.)
+// workgroup a CU, 66, but tiles of 16384 99.) What is read again may have changed
+// where two sequences have the same entry, against the contract: places and tokens
+// in the list are held within it.
 __global__ void __attribute__((amdgpu_flat_work_group_size(1024, 1024), amdgpu_waves_per_eu(8)))
 SelectLongKernel(EvictParams p)
 {
@@ -313,6 +327,7 @@ SelectLongKernel(EvictParams p)
     const int K = end - p.sinks;
     if (K > 0) {
         uint32_t key[IT];
+        // (the next tile's on their way meanwhile: 73 us for 70)
         const auto load = [&](int j0, int last) {
 #pragma unroll
             for (int i = 0; i < IT; ++i) key[i] = KeyOf(w[uint32_t(min(j0 + tid + NT * i, last - 1))]);
@@ -374,8 +389,8 @@ SelectLongKernel(EvictParams p)
             for (int i = 0; i < IT; ++i) {
                 const bool mover = ((wins >> i) & 1) != 0;
                 const uint64_t of = __ballot(mover);
-                if (mover)
-                    keep[p.sinks + movers + cells[i * NW + wave] + __popcll(of & below)] = j0 + tid + NT * i;
+                const int at = p.sinks + movers + cells[i * NW + wave] + __popcll(of & below);
+                if (mover && at < end) keep[at] = j0 + tid + NT * i;
             }
             movers += all;
             __syncthreads();
@@ -396,7 +411,8 @@ SelectLongKernel(EvictParams p)
             for (int i = 0; i < IT; ++i) {
                 const bool is = hole(i);
                 const uint64_t all = __ballot(is);
-                of[i] = is ? keep[p.sinks + left + cells[i * NW + wave] + __popcll(all & below)] : j0 + tid + NT * i;
+                const int at = p.sinks + left + cells[i * NW + wave] + __popcll(all & below);
+                of[i] = is ? min(max(keep[min(max(at, p.sinks), end - 1)], 0), len - 1) : j0 + tid + NT * i;
             }
             __syncthreads();
 #pragma unroll
@@ -424,6 +440,9 @@ __device__ __forceinline__ int64_t RowAt(const EvictParams &p, const int32_t *ta
 }
 
 typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+// MoveKernel on the eight sequences above: 159 us with 4 rows, 2048 workgroups and
+// plain stores; 97 with 2 rows and stores that do not stay in the L2, 86 with 4096
+// workgroups, 79 with 4 rows.
 constexpr int kMoveRows = 4;       // rows of a thread
 constexpr int kMoveGroups = 4096;  // workgroups: 16 for each of 256 CUs
 

@@ -12,6 +12,16 @@
 // keys by 32 rows at a time, the keys in its registers. Lane l's row is l % 32,
 // register v's key 8 (v / 4) + 4 (l / 32) + v % 4; the sums over rows stay in 16
 // registers until the last row, and are then added up across lanes.
+//
+// What bounds it, on an MI355X:
+//   few rows a head (StepKernel): K, once, and the weights, there and back. 64
+//     sequences of 2000..4000 tokens, 28 heads of 128 over 4, a new token each: 203
+//     MB in 45 us, 4.5 TB/s (a large copy: 4.9).
+//   many rows (WeighKernel): the exponentials beside the products. 2048 new
+//     tokens behind 8000, the same heads: 205 us, 0.65 PFLOP/s; the matrix
+//     cores are at work for 29% of the time and the vector units for 63%, 177
+//     instructions a wave and row tile, 32 of them exponentials. The two hardly
+//     overlap: their sum is nearly all of the time.
 #include <algorithm>
 #include <cmath>
 
@@ -97,7 +107,8 @@ __device__ __forceinline__ WeighSeq LoadSeq(const WeighParams &p, int b)
 }
 
 constexpr int kWeighKeys = 256;   // of a workgroup's tile: 64 a wave
-constexpr int kWeighParts = 768;  // workgroups that share the line: three on each of 256 CUs
+constexpr int kWeighParts = 768;  // workgroups that share the line: three on each of 256 CUs (the chunk above,
+                                  // early on: 512 238 us, 768 219, 1024 244)
 constexpr int kWeighStages = 3;   // row tiles in LDS
 
 // Where in the line a workgroup stands: row tiles of the key tiles of all
@@ -159,21 +170,27 @@ __device__ __forceinline__ WeighPiece PieceAt(const WeighParams &p, const WeighL
     return w;
 }
 
-// The line's length.
+// The line's length. Starts that ascend keep it within what the host has checked;
+// what is longer all the same is not worked on.
+constexpr int64_t kWeighLine = (int64_t(1) << 31) - 4096;
 __device__ __forceinline__ int WeighTotal(const WeighParams &p, int lane)
 {
-    int total = 0;
+    int64_t total = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += 64) {
         int u = 0;
         if (b0 + lane < p.seqs) {
             const WeighSeq s = LoadSeq(p, b0 + lane);
             if (s.cols > 0) u = p.HKV * WeighLine(p, s).Head();
         }
+        uint32_t lo = uint32_t(u) & 0xffff, hi = uint32_t(u) >> 16;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
-        total += Uni(u);
+        for (int o = 32; o > 0; o >>= 1) {
+            lo += uint32_t(__shfl_xor(int(lo), o, 64));
+            hi += uint32_t(__shfl_xor(int(hi), o, 64));
+        }
+        total += Uni(int(lo)) + (int64_t(Uni(int(hi))) << 16);
     }
-    return total;
+    return total < kWeighLine ? int(total) : 0;
 }
 
 // The sequence that holds position x of the line, which is inside it; `base`: where it begins.
@@ -326,8 +343,8 @@ WeighKernel(WeighParams p)
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int dc = 0; dc < D / 16; ++dc) kf[kb][dc] = *reinterpret_cast<const uint4 *>(kr[kb] + dc * 16);
-        // (used here: a load that the compiler still counts in the loop would make
-        // it wait for the DMA there, tile by tile: 205 us for 100 over a prompt's chunk)
+        // (used here: a load that is still counted in the loop would have the compiler
+        // wait there for everything in flight, the DMA of the tiles to come included)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -358,7 +375,8 @@ WeighKernel(WeighParams p)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) s[kb][v] = 0.0f;
             {
-                // the Q fragment of step dc is read QAH steps ahead of its MFMAs
+                // the Q fragment of step dc is read QAH steps ahead of its MFMAs (of the
+                // chunk above: 2 207 us, 4 204.7)
                 constexpr int NP = D / 16, QAH = 4;
                 uint4 qf[NP];
                 const auto rd = [&](int dc) { qf[dc] = *reinterpret_cast<const uint4 *>(Q + (qaddr ^ (dc * 16))); };
@@ -379,7 +397,8 @@ WeighKernel(WeighParams p)
                 __builtin_amdgcn_sched_group_barrier(0x008, KB * QAH, 0);
             }
             // register v: row 8 (v / 4) + 4 hf + v % 4. The wave in its
-            // exponentials goes first, as in the attention's kernels.
+            // exponentials goes first, as in the attention's kernels (without: 216 us
+            // for 205).
             __builtin_amdgcn_s_setprio(2);
             if (whole) {
 #pragma unroll
@@ -441,15 +460,15 @@ WeighKernel(WeighParams p)
 
 // ------------------------------------------------------- at most 32 rows a head
 // A wave has a run of 32-key blocks, key head by key head. Keys go HBM -> LDS by
-// the DMA, whole rows side by side (a lane for each 16 bytes of a row: loads
-// straight to the product's registers, 32 rows at a time, reached 3.7 TB/s of
-// 197 MB, these 5), a ring of kStepStages blocks for each wave, and nobody
-// waits for another wave. The old weights come the same way, so that the loop
-// holds no load that the compiler would wait for. Up to kStepRun blocks of a key
-// head make a run, whose page ids are read at its start.
-constexpr int kStepStages = 2;
-constexpr int kStepRun = 16;       // blocks
-constexpr int kStepGroups = 512;   // workgroups of four waves: two on each of 256 CUs
+// the DMA, whole rows side by side, a lane for each 16 bytes of a row, a ring of
+// kStepStages blocks for each wave, and nobody waits for another wave. The old
+// weights come the same way, so that the loop holds no load that the compiler
+// would wait for. Up to kStepRun blocks of a key head make a run, whose page ids
+// are read at its start. (The step above, 203 MB: WeighKernel, whose loads go
+// straight to the product's registers, 32 rows at a time, 53.4 us; this one 45.)
+constexpr int kStepStages = 2;     // (3 46.2 us, 4 47.3)
+constexpr int kStepRun = 16;       // blocks (8 44.7 us, 16 45.0; 16 read the page table half as often)
+constexpr int kStepGroups = 512;   // workgroups of four waves: two on each of 256 CUs (1024 46.3 us, 2048 50.8)
 
 template <int DT, int D, bool PLAIN>
 __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
@@ -631,7 +650,8 @@ __global__ void __launch_bounds__(kWeighKeys) WeighJoinKernel(WeighParams p)
     PutWeight(p, sq, pc.h, key, got);
 }
 
-// Is every tile one row tile, so that none is cut?
+// Is every tile one row tile? Then none is cut, there is nothing to join, and a
+// wave that holds all rows need not share them: StepKernel.
 bool OneRowTile(int64_t tokens, int G) { return tokens * G <= 32; }
 
 }  // namespace
@@ -719,8 +739,10 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     if (d.path != nullptr) tokens = std::min<int64_t>(tokens, d.path_width);
     if (d.last > 0) tokens = std::min<int64_t>(tokens, d.last);
     const int64_t tiles = (std::min<int64_t>(cap, w.width) + kWeighKeys - 1) / kWeighKeys;
-    const int64_t most = tiles * c.heads * s.seqs, row_tiles = (tokens * p.G + 31) / 32;
-    if (most >= (int64_t(1) << 31) / row_tiles) refuse("too many rows and keys for one launch");
+    // (of all sequences together: no more than the rows fill, and one that is not full for each)
+    const int64_t row_tiles = std::min((tokens * p.G + 31) / 32 * s.seqs, int64_t(d.rows) * p.G / 32 + s.seqs);
+    if (tiles * c.heads >= kWeighLine / row_tiles || 8 * tiles * c.heads >= kWeighLine / s.seqs)
+        refuse("too many rows and keys for one launch");
     const MemSpan out = WeightsSpan(w);
     const RowSpan k = LayerSpan(c, c.k, d.layer);
     if (Meets(out, RowsSpan(d.q, d.rows, p.ldq, int64_t(d.HQ) * c.head_dim, 2)) ||

@@ -98,6 +98,22 @@ def test_bad_weigh_calls(kw, text):
     refused(weigh(**kw), text)
 
 
+# weights that hold as many tokens as the page table; their rows times the key tiles, and the blocks alone
+WIDE = dict(w=FAR << 4, layer_stride=1 << 38, entry_stride=1 << 34, head_stride=1 << 30, width=1 << 30)
+
+
+@pytest.mark.parametrize("kw,s", [(dict(rows=5000), dict(max_new=5000)), (dict(rows=1), dict(seqs=20, max_new=1))])
+def test_more_rows_and_keys_than_a_launch_can_count(kw, s):
+    s = far_seqs(table_pages=1 << 26, ld_table=1 << 26, **s)
+    ws = ctypes.c_size_t(0)
+    assert ops._lib().kr_op_attention_paged_weigh_workspace(cache(), s, 8, ctypes.byref(ws)) == 0
+    f = dict(q=FAR, lse=FAR + (1 << 30), HQ=8)
+    f.update(kw)
+    refused(ops._lib().kr_op_attention_paged_weigh(cache(), 0, s, f["q"], 0, f["lse"], 0, f["rows"], 8, 0.1, weights(**WIDE),
+                                                   0, 1.0, None, 0, 0, None, FAR + (2 << 30), ws.value, None),
+            "too many rows and keys")
+
+
 @pytest.mark.parametrize("kw,text", [
     (dict(budget=0), "budget"), (dict(sinks=-1), "fit the budget"), (dict(recent=-1), "fit the budget"),
     (dict(sinks=6, recent=5), "fit the budget"), (dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), "fit the budget"),

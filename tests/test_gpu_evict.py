@@ -175,6 +175,23 @@ def test_lengths_that_are_none(gpu):
     assert torch.equal(x.k[:, pages], was[0][:, pages]) and torch.equal(x.v[:, pages], was[1][:, pages])
 
 
+@pytest.mark.parametrize("n,budget", [(700, 300), (30000, 9000)])
+def test_one_entry_twice(gpu, n, budget):
+    """Against the contract: which tokens stay is open, but lists name tokens of
+    their sequence, and what is around them stays."""
+    announce("evict twice %d" % n)
+    x = Case(5, [n] * 4, layers=2, entries=[1, 1, 1, 1], page=16)
+    x.w.copy_((x.w * 9).floor())
+    others, was = [0, 2, 3, 4, 5], x.w.clone()
+    room = torch.full((2 * 4 * 2 * budget + 4096,), 77, dtype=torch.int32, device="cuda")
+    keep = room[2048:-2048].view(2, 4, 2, budget)
+    ops.cache_evict(x.cache, x.seqs, ops.make_weights(x.w, entry=ints(x.entry)), keep, sinks=3, recent=50)
+    assert bool(room[:2048].eq(77).all()) and bool(room[-2048:].eq(77).all())
+    assert int(keep.min()) >= 0 and int(keep.max()) < n
+    assert bool((keep[..., :3] == ints([0, 1, 2])).all()) and bool((keep[..., -50:] == torch.arange(n - 50, n, device="cuda")).all())
+    assert torch.equal(x.w[:, others], was[:, others])
+
+
 def test_no_sequences(gpu):
     x = Case(8, [5])
     seqs = ops.make_seqs(torch.empty(0, 3, dtype=torch.int32, device="cuda"), ints([]), ints([0]), 0)

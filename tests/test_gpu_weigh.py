@@ -278,6 +278,25 @@ def test_nothing_to_do(gpu):
     assert torch.equal(w, old)
 
 
+def test_starts_that_go_back_and_forth(gpu):
+    """Half of 1024 sequences claim all 2048 rows, a million tokens each: more row
+    tiles of key tiles than a launch counts. Nothing is worked on."""
+    announce("weigh starts")
+    n, page, rows, HQ = 1024, 1024, 2048, 32
+    k = torch.zeros(1, 2, page, 1, 64, device="cuda", dtype=BF)
+    cache = ops.make_cache(k, k.clone())
+    table = torch.full((n, 1024), -1, dtype=torch.int32, device="cuda")
+    seqs = ops.make_seqs(table, ints([page * 1024 - rows] * n), ints([0, rows] * (n // 2) + [0]), rows)
+    w = torch.rand(1, 1, page * 1024, device="cuda")
+    old = w.clone()
+    h = ops.make_weights(w, entry=ints([0] * n))
+    ws = torch.empty(ops.attention_paged_weigh_workspace(cache, seqs, HQ), dtype=torch.uint8, device="cuda")
+    q = torch.zeros(rows, HQ, 64, device="cuda", dtype=BF)
+    ops.attention_paged_weigh(cache, 0, seqs, q, torch.zeros(rows, HQ, device="cuda"), h, ws)
+    torch.cuda.synchronize()
+    assert torch.equal(w, old)
+
+
 @pytest.mark.parametrize("D,HQ,HKV,lens,news", [(128, 28, 4, [5000, 3100], [300, 1]), (64, 14, 2, [20000], [1]),
                                                 (128, 32, 8, [2500], [64]), (64, 4, 4, [0], [1100])])
 def test_long_ones_add_up(gpu, D, HQ, HKV, lens, news):
