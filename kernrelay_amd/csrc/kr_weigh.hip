@@ -238,6 +238,26 @@ __device__ __forceinline__ void PutWeight(const WeighParams &p, const WeighSeq &
     *w = old + got;
 }
 
+// Which of the 64 keys from nj on (as new tokens; negative: cached ones) row i of
+// the sequence's new tokens sees: bit k for key nj + k.
+template <bool PLAIN>
+__device__ __forceinline__ uint64_t RowMask(const WeighParams &p, const WeighSeq &s, int b, int i, int nj, bool causal)
+{
+    if (!PLAIN && p.path != nullptr) {
+        const int at = p.path[b * p.ld_path + i];
+        if (at < 0 || at >= s.rows) return 0;
+    }
+    if (PLAIN || causal) {
+        const int n = i - nj + 1;
+        return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+    }
+    const uint64_t *tree = p.tree + int64_t(s.first + i) * p.ld_tree;
+    const auto word = [&](int w) { return w < 0 ? ~0ull : w < p.tree_words ? tree[w] : 0ull; };
+    const int w = nj >> 6, by = nj & 63;
+    const uint64_t lo = word(w);
+    return by == 0 ? lo : (lo >> by) | (word(w + 1) << (64 - by));
+}
+
 // PLAIN: causal, no path.
 template <int DT, int D, bool PLAIN>
 __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2)))
@@ -251,6 +271,7 @@ WeighKernel(WeighParams p)
     __shared__ __attribute__((aligned(1024))) uint16_t qring[NS][32 * D];
     __shared__ __attribute__((aligned(256))) float lring[4][NS][64];  // a wave's own: lse of the tile's rows, twice
     __shared__ int64_t rows[4][32];                                  // and where its rows' queries are
+    __shared__ __attribute__((aligned(16))) uint2 masks[4][32];      // and which of its keys they see
     const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
     const int hf = lane >> 5;
     const int total = WeighTotal(p, lane);
@@ -369,6 +390,12 @@ WeighKernel(WeighParams p)
             const bool dead = __ballot(ls[lane & 31] == -INFINITY) != 0;
             const bool whole = all && !dead && (PLAIN || p.path == nullptr) && r0 + 32 <= R &&
                                nj + 32 * KB <= (causal ? tok_lo + 1 : 0);
+            if (!whole) {
+                // a row's keys as 64 bits, made by the lane of that row
+                const int rl = lane & 31, i32 = sq.skip + PageOf(p.group, min(r0 + rl, R - 1));
+                const uint64_t m = r0 + rl < R && ls[rl] != -INFINITY ? RowMask<PLAIN>(p, sq, b, i32, nj, causal) : 0;
+                if (lane < 32) masks[wave][lane] = make_uint2(uint32_t(m), uint32_t(m >> 32));
+            }
             f32x16 s[KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -415,32 +442,28 @@ WeighKernel(WeighParams p)
                     }
                 }
             } else {
+                WaveLdsOrder();
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int r = 8 * (v >> 2) + 4 * hf + (v & 3);
-                    const float lse = ls[r];
-                    const int tok = sq.skip + PageOf(p.group, min(r0 + r, R - 1));
-                    bool live = r0 + r < R && lse != -INFINITY;
-                    if (!PLAIN && p.path != nullptr) {
-                        const int at = p.path[b * p.ld_path + tok];
-                        live = live && at >= 0 && at < sq.rows;
-                    }
+                for (int v4 = 0; v4 < 4; ++v4) {
+                    const float4 l4 = *reinterpret_cast<const float4 *>(ls + 8 * v4 + 4 * hf);
+                    const uint4 m01 = *reinterpret_cast<const uint4 *>(&masks[wave][8 * v4 + 4 * hf]);
+                    const uint4 m23 = *reinterpret_cast<const uint4 *>(&masks[wave][8 * v4 + 4 * hf + 2]);
+                    const float nl[4] = {l4.x * -kLog2E, l4.y * -kLog2E, l4.z * -kLog2E, l4.w * -kLog2E};
+                    const uint32_t mm[4][KB] = {{m01.x, m01.y}, {m01.z, m01.w}, {m23.x, m23.y}, {m23.z, m23.w}};
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb) {
-                        const int k = nj + kb * 32 + (lane & 31);  // the key as a new token
-                        bool sees = live && ((there >> kb) & 1) != 0;
-                        if (causal) {
-                            sees = sees && k <= tok;
-                        } else if (sees && k >= 0) {
-                            const uint64_t w = (k >> 6) < p.tree_words
-                                                   ? p.tree[int64_t(sq.first + tok) * p.ld_tree + (k >> 6)]
-                                                   : 0ull;
-                            sees = ((w >> (k & 63)) & 1) != 0;
+                        float e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][4 * v4 + i], p.scale_log2, nl[i]));
+                            e[i] = __uint_as_float(__float_as_uint(e[i]) &
+                                                   uint32_t(__builtin_amdgcn_sbfe(int(mm[i][kb]), uint32_t(lane & 31), 1u)));
                         }
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][v], p.scale_log2, lse * -kLog2E));
-                        sum[kb] += sees ? e : 0.0f;
+                        const float of4 = (e[0] + e[1]) + (e[2] + e[3]);
+                        sum[kb] += ((there >> kb) & 1) != 0 ? of4 : 0.0f;
                     }
                 }
+                WaveLdsOrder();
             }
             __builtin_amdgcn_s_setprio(0);
         }
