@@ -110,6 +110,7 @@ constexpr int kWeighKeys = 256;   // of a workgroup's tile: 64 a wave
 constexpr int kWeighParts = 768;  // workgroups that share the line: three on each of 256 CUs (the chunk above,
                                   // early on: 512 238 us, 768 219, 1024 244)
 constexpr int kWeighStages = 3;   // row tiles in LDS
+constexpr int kWeighMasked = 1;   // quarters that a row tile counts for more where it needs masks
 
 // Where in the line a workgroup stands: row tiles of the key tiles of all
 // sequences, key head by key head. A key tile of new tokens begins with the
@@ -119,6 +120,15 @@ struct WeighLine {
     int rt;           // row tiles of the sequence
     int full, more;   // key tiles of a key head with all row tiles, and the others
     int first, step;  // row tiles that the first of the others leaves out, and each after it more
+    // The others' first `step` row tiles see a part of them, by masks, and count
+    // for more than one: where a tile of so many row tiles ends in the line, and
+    // the row tile that a place in it stands for.
+    __device__ __forceinline__ int Places(int rows) const { return rows + min(rows, step) / 4 * kWeighMasked; }
+    __device__ __forceinline__ int Row(int rows, int place) const
+    {
+        const int m = min(rows, step) / 4;
+        return place < m * (4 + kWeighMasked) ? place * 4 / (4 + kWeighMasked) : place - m * kWeighMasked;
+    }
     __device__ __forceinline__ WeighLine(const WeighParams &p, const WeighSeq &s)
     {
         const int tiles = (s.cols + kWeighKeys - 1) / kWeighKeys;
@@ -131,15 +141,19 @@ struct WeighLine {
     }
     __device__ __forceinline__ int Head() const  // of a key head
     {
-        return full * rt + more * (rt - first) - step * (more * (more - 1) / 2);
+        // (of the others only the last can have fewer than `step`)
+        const int few = more > 0 ? min(rt - first - step * (more - 1), step) / 4 : 0;
+        return full * rt + more * (rt - first) - step * (more * (more - 1) / 2) +
+               (max(more - 1, 0) * (step / 4) + few) * kWeighMasked;
     }
 };
 
 // A piece of a key tile: row tiles r_lo .. r_hi - 1.
 struct WeighPiece {
     int b, h, t;
-    int start, rows;  // of the tile: where in the line it begins, and its row tiles
-    int skip;         // row tiles that it leaves out
+    int start, places;  // of the tile: where in the line it begins, and its places there
+    int skip, rows;     // row tiles that it leaves out, and that it has
+    bool masked;
 };
 
 // Position x of the line, in a sequence that begins at `base` of it.
@@ -154,18 +168,21 @@ __device__ __forceinline__ WeighPiece PieceAt(const WeighParams &p, const WeighL
     if (y < l.full * l.rt) {
         w.t = Uni(y / l.rt);
         w.start = at + w.t * l.rt;
-        w.rows = l.rt;
+        w.places = w.rows = l.rt;
         w.skip = 0;
+        w.masked = false;
     } else {
         w.start = at + l.full * l.rt;
         w.t = l.full;
         w.skip = l.first;
-        while (x >= w.start + (l.rt - w.skip)) {
-            w.start += l.rt - w.skip;
+        while (x >= w.start + l.Places(l.rt - w.skip)) {
+            w.start += l.Places(l.rt - w.skip);
             w.skip += l.step;
             ++w.t;
         }
         w.rows = l.rt - w.skip;
+        w.places = l.Places(w.rows);
+        w.masked = true;
     }
     return w;
 }
@@ -297,8 +314,9 @@ WeighKernel(WeighParams p)
         }
         const WeighPiece pc = PieceAt(p, line, b, base, x);
         const int h = pc.h;
-        const int rt_lo = Uni(pc.skip + x - pc.start);
-        const int rt_hi = Uni(min(pc.skip + pc.rows, rt_lo + (x_end - x)));
+        const int y = x - pc.start, y_end = min(pc.places, x_end - pc.start);
+        const int rt_lo = Uni(pc.skip + (pc.masked ? line.Row(pc.rows, y) : y));
+        const int rt_hi = Uni(pc.skip + (pc.masked ? line.Row(pc.rows, y_end) : y_end));
         const int R = (sq.n - sq.skip) * p.G;
         const int j0 = Uni(pc.t * kWeighKeys + wave * (32 * KB));
         // ---- this wave's keys: lane l holds key l % 32 of each block, chunks of 8, every second one
@@ -357,7 +375,7 @@ WeighKernel(WeighParams p)
         };
         const int ns = rt_hi - rt_lo;
         __syncthreads();  // (the rings are free)
-        fetch(0, 0);
+        if (ns > 0) fetch(0, 0);
         if (ns > 1) fetch(1, 1);
         uint4 kf[KB][D / 16];
 #pragma unroll
@@ -468,7 +486,7 @@ WeighKernel(WeighParams p)
             __builtin_amdgcn_s_setprio(0);
         }
         // ---- the two halves of a key's rows, and where its sum goes
-        const bool cut = x > pc.start || x + ns < pc.start + pc.rows;
+        const bool cut = y > 0 || y_end < pc.places;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             const float got = sum[kb] + __shfl_xor(sum[kb], 32, 64);
@@ -477,7 +495,7 @@ WeighKernel(WeighParams p)
             if (cut) p.parts[(2 * int(blockIdx.x) + (x > pc.start ? 0 : 1)) * kWeighKeys + wave * 32 * KB + kb * 32 + lane] = got;
             else if (key < sq.cols) PutWeight(p, sq, h, key, got);
         }
-        x += ns;
+        x = pc.start + y_end;
     }
 }
 
@@ -663,7 +681,7 @@ __global__ void __launch_bounds__(kWeighKeys) WeighJoinKernel(WeighParams p)
     const int b = WeighFind(p, lane, x1 - 1, base);
     const WeighSeq sq = LoadSeq(p, b);
     const WeighPiece pc = PieceAt(p, WeighLine(p, sq), b, base, x1 - 1);
-    const int end = pc.start + pc.rows;
+    const int end = pc.start + pc.places;
     if (pc.start < x0 || end <= x1) return;
     const int key = pc.t * kWeighKeys + int(threadIdx.x);
     if (key >= sq.cols) return;
@@ -764,7 +782,7 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     const int64_t tiles = (std::min<int64_t>(cap, w.width) + kWeighKeys - 1) / kWeighKeys;
     // (of all sequences together: no more than the rows fill, and one that is not full for each)
     const int64_t row_tiles = std::min((tokens * p.G + 31) / 32 * s.seqs, int64_t(d.rows) * p.G / 32 + s.seqs);
-    if (tiles * c.heads >= kWeighLine / row_tiles || 8 * tiles * c.heads >= kWeighLine / s.seqs)
+    if (tiles * c.heads >= kWeighLine / (row_tiles + row_tiles * kWeighMasked / 4) || 8 * tiles * c.heads >= kWeighLine / s.seqs)
         refuse("too many rows and keys for one launch");
     const MemSpan out = WeightsSpan(w);
     const RowSpan k = LayerSpan(c, c.k, d.layer);
