@@ -275,6 +275,12 @@ __device__ __forceinline__ uint64_t RowMask(const WeighParams &p, const WeighSeq
     return by == 0 ? lo : (lo >> by) | (word(w + 1) << (64 - by));
 }
 
+// e where bit `key` of a row's mask is set, else 0, whatever e is.
+__device__ __forceinline__ float Seen(float e, uint32_t mask, int key)
+{
+    return __uint_as_float(__float_as_uint(e) & uint32_t(__builtin_amdgcn_sbfe(int(mask), uint32_t(key), 1u)));
+}
+
 // PLAIN: causal, no path.
 template <int DT, int D, bool PLAIN>
 __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2)))
@@ -474,8 +480,7 @@ WeighKernel(WeighParams p)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][4 * v4 + i], p.scale_log2, nl[i]));
-                            e[i] = __uint_as_float(__float_as_uint(e[i]) &
-                                                   uint32_t(__builtin_amdgcn_sbfe(int(mm[i][kb]), uint32_t(lane & 31), 1u)));
+                            e[i] = Seen(e[i], mm[i][kb], lane & 31);
                         }
                         const float of4 = (e[0] + e[1]) + (e[2] + e[3]);
                         sum[kb] += ((there >> kb) & 1) != 0 ? of4 : 0.0f;
@@ -522,6 +527,7 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
     __shared__ __attribute__((aligned(1024))) uint16_t ring[4][NS][32 * D];
     __shared__ __attribute__((aligned(256))) float wring[4][NS][64];
     __shared__ int64_t offs[4][32];
+    __shared__ __attribute__((aligned(16))) uint32_t masks[4][32];  // which keys of the block a row sees
     __shared__ int32_t tab[4][kStepRun * 32];
     const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
     const int hf = lane >> 5, l32 = lane & 31;
@@ -628,6 +634,12 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
             const bool ok = ((there[0] >> l32) & 1) != 0;
             // do all rows count, and see every key? (Those past the last repeat it with weight 0.)
             const bool whole = there[0] == ~0u && nj + 32 <= (causal ? sq.skip + 1 : 0) && counts == (~0u >> (32 - min(R, 32)));
+            if (!whole) {
+                WaveLdsOrder();
+                const uint32_t m = ((counts >> l32) & 1) != 0 ? uint32_t(RowMask<PLAIN>(p, sq, b, i32, nj, causal)) : 0u;
+                if (lane < 32) masks[wave][lane] = m;
+                WaveLdsOrder();
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int v4 = 0; v4 < 4; ++v4) {
@@ -637,23 +649,10 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
                 for (int i = 0; i < 4; ++i)
                     e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * v4 + i], p.scale_log2, nl[4 * v4 + i]));
                 if (!whole) {
+                    const uint4 m = *reinterpret_cast<const uint4 *>(&masks[wave][8 * v4 + 4 * hf]);
+                    const uint32_t mm[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 8 * v4 + 4 * hf + i;
-                        bool sees = ok && ((counts >> r) & 1) != 0;
-                        if (nj + 32 > (causal ? sq.skip + 1 : 0)) {
-                            const int at = sq.skip + PageOf(p.group, min(r, R - 1)), k = nj + l32;
-                            if (causal) {
-                                sees = sees && k <= at;
-                            } else if (sees && k >= 0) {
-                                const uint64_t w = (k >> 6) < p.tree_words
-                                                       ? p.tree[int64_t(sq.first + at) * p.ld_tree + (k >> 6)]
-                                                       : 0ull;
-                                sees = ((w >> (k & 63)) & 1) != 0;
-                            }
-                        }
-                        e[i] = sees ? e[i] : 0.0f;
-                    }
+                    for (int i = 0; i < 4; ++i) e[i] = ok ? Seen(e[i], mm[i], l32) : 0.0f;
                 }
                 sum += (e[0] + e[1]) + (e[2] + e[3]);
             }
