@@ -346,13 +346,16 @@ WeighKernel(WeighParams p)
         // are; from tile to tile the addresses go on by as many tokens and heads
         int64_t qo = 0, lo = 0;  // elements
         int g = 0;
+        bool out = false;  // of a path: does an entry of the tiles so far name no row?
         const auto point = [&](int r) {
             const int i = PageOf(p.group, r);
             g = r - i * p.G;
             int tok = sq.skip + i;
             if (!PLAIN && p.path != nullptr) {
                 tok = p.path[b * p.ld_path + tok];
-                if (tok < 0 || tok >= sq.rows) tok = 0;  // (counts nothing, see below)
+                const bool none = tok < 0 || tok >= sq.rows;
+                out = out || __ballot(none) != 0;
+                if (none) tok = 0;  // (counts nothing, see RowMask)
             }
             const int64_t row = sq.first + tok;
             qo = row * p.ldq + int64_t(h * p.G + g) * D;
@@ -412,7 +415,7 @@ WeighKernel(WeighParams p)
             const int tok_hi = sq.skip + Uni(PageOf(p.group, min(r0 + 31, R - 1)));
             if (j0 >= sq.cols || (causal && nj > tok_hi)) continue;
             const bool dead = __ballot(ls[lane & 31] == -INFINITY) != 0;
-            const bool whole = all && !dead && (PLAIN || p.path == nullptr) && r0 + 32 <= R &&
+            const bool whole = all && !dead && (PLAIN || !out) && r0 + 32 <= R &&
                                nj + 32 * KB <= (causal ? tok_lo + 1 : 0);
             if (!whole) {
                 // a row's keys as 64 bits, made by the lane of that row
