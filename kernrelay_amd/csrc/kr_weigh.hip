@@ -8,20 +8,19 @@
 // The attention over the same rows has left lse, so one pass over K is enough
 // and a key's sum belongs to one wave: no atomics.
 //
-// The scores are those of the attention (kr_paged.hip): S^T = K Q^T, a wave 32
-// keys by 32 rows at a time, the keys in its registers. Lane l's row is l % 32,
-// register v's key 8 (v / 4) + 4 (l / 32) + v % 4; the sums over rows stay in 16
-// registers until the last row, and are then added up across lanes.
+// The scores S = Q K^T of a wave, 32 rows by 32 keys at a time: lane l's key is
+// l % 32, register v's row 8 (v / 4) + 4 (l / 32) + v % 4. A key's sum stays in its
+// two lanes until the last row, in fp32; the two are added at the end.
 //
 // What bounds it, on an MI355X:
 //   few rows a head (StepKernel): K, once, and the weights, there and back. 64
 //     sequences of 2000..4000 tokens, 28 heads of 128 over 4, a new token each: 203
-//     MB in 45 us, 4.5 TB/s (a large copy: 4.9).
-//   many rows (WeighKernel): the exponentials beside the products. 2048 new
-//     tokens behind 8000, the same heads: 205 us, 0.65 PFLOP/s; the matrix
-//     cores are at work for 29% of the time and the vector units for 63%, 177
-//     instructions a wave and row tile, 32 of them exponentials. The two hardly
-//     overlap: their sum is nearly all of the time.
+//     MB in 44 us, 4.6 TB/s (a large copy: 4.9).
+//   many rows (WeighKernel): products and vector work, which hardly overlap. 2048
+//     new tokens behind 8000, the same heads: 168 us, 0.79 PFLOP/s; the matrix
+//     cores are at work for 35% of the time, vector instructions for 57%. Without
+//     the products it takes 129 us, without the exponentials 153, without the
+//     rows' DMA 151, without reading the rows from LDS 163.
 #include <algorithm>
 #include <cmath>
 
@@ -110,7 +109,8 @@ constexpr int kWeighKeys = 256;   // of a workgroup's tile: 64 a wave
 constexpr int kWeighParts = 768;  // workgroups that share the line: three on each of 256 CUs (the chunk above,
                                   // early on: 512 238 us, 768 219, 1024 244)
 constexpr int kWeighStages = 3;   // row tiles in LDS
-constexpr int kWeighMasked = 1;   // quarters that a row tile counts for more where it needs masks
+constexpr int kWeighMasked = 1;   // quarters that a row tile counts for more where it needs masks (the chunk: 0 170.9
+                                  // us, 1 167.5, 2 172.8; 512 tokens behind 40000: 190, 178.8, 178.7)
 
 // Where in the line a workgroup stands: row tiles of the key tiles of all
 // sequences, key head by key head. A key tile of new tokens begins with the
@@ -256,7 +256,9 @@ __device__ __forceinline__ void PutWeight(const WeighParams &p, const WeighSeq &
 }
 
 // Which of the 64 keys from nj on (as new tokens; negative: cached ones) row i of
-// the sequence's new tokens sees: bit k for key nj + k.
+// the sequence's new tokens sees: bit k for key nj + k. (Made once a row and tile,
+// by the row's lane; looked up row by row and key by key the chunk above took 197
+// us for 172, and 8 sequences of 1500 with trees of up to 60 drafts 44.7 for 30.7.)
 template <bool PLAIN>
 __device__ __forceinline__ uint64_t RowMask(const WeighParams &p, const WeighSeq &s, int b, int i, int nj, bool causal)
 {
@@ -514,8 +516,9 @@ WeighKernel(WeighParams p)
 // weights come the same way, so that the loop holds no load that the compiler
 // would wait for. Up to kStepRun blocks of a key head make a run, whose page ids
 // are read at its start. (The step above, 203 MB: WeighKernel, whose loads go
-// straight to the product's registers, 32 rows at a time, 53.4 us; this one 45.)
-constexpr int kStepStages = 2;     // (3 46.2 us, 4 47.3)
+// straight to the product's registers, 32 rows at a time, 53.4 us; this one 45,
+// now 44.)
+constexpr int kStepStages = 2;     // (45.0 us; 3 46.2, 4 47.3)
 constexpr int kStepRun = 16;       // blocks (8 44.7 us, 16 45.0; 16 read the page table half as often)
 constexpr int kStepGroups = 512;   // workgroups of four waves: two on each of 256 CUs (1024 46.3 us, 2048 50.8)
 
