@@ -187,47 +187,58 @@ __device__ __forceinline__ WeighPiece PieceAt(const WeighParams &p, const WeighL
     return w;
 }
 
-// The line's length. Starts that ascend keep it within what the host has checked;
-// what is longer all the same is not worked on.
+// All sequences' units one after the other, units(sequence) of each. Up to 64
+// sequences are read once, one a lane, and looked up there.
 constexpr int64_t kWeighLine = (int64_t(1) << 31) - 4096;
-__device__ __forceinline__ int WeighTotal(const WeighParams &p, int lane)
-{
-    int64_t total = 0;
-    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int u = 0;
-        if (b0 + lane < p.seqs) {
-            const WeighSeq s = LoadSeq(p, b0 + lane);
-            if (s.cols > 0) u = p.HKV * WeighLine(p, s).Head();
-        }
-        uint32_t lo = uint32_t(u) & 0xffff, hi = uint32_t(u) >> 16;
+template <typename F>
+struct WeighPlan {
+    const WeighParams &p;
+    const F units;
+    const int lane;
+    WeighSeq mine;
+    int u, total;
+    __device__ __forceinline__ int Units(const WeighSeq &s, int b) const { return b < p.seqs && s.cols > 0 ? units(s) : 0; }
+    // Starts that ascend keep the total within what the host has checked; what is
+    // longer all the same is not worked on.
+    __device__ __forceinline__ WeighPlan(const WeighParams &p_, int lane_, F units_) : p(p_), units(units_), lane(lane_)
+    {
+        int64_t sum = 0;
+        for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+            mine = LoadSeq(p, min(b0 + lane, p.seqs - 1));
+            u = Units(mine, b0 + lane);
+            uint32_t lo = uint32_t(u) & 0xffff, hi = uint32_t(u) >> 16;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            lo += uint32_t(__shfl_xor(int(lo), o, 64));
-            hi += uint32_t(__shfl_xor(int(hi), o, 64));
+            for (int o = 32; o > 0; o >>= 1) {
+                lo += uint32_t(__shfl_xor(int(lo), o, 64));
+                hi += uint32_t(__shfl_xor(int(hi), o, 64));
+            }
+            sum += Uni(int(lo)) + (int64_t(Uni(int(hi))) << 16);
         }
-        total += Uni(int(lo)) + (int64_t(Uni(int(hi))) << 16);
+        total = sum < kWeighLine ? int(sum) : 0;
     }
-    return total < kWeighLine ? int(total) : 0;
-}
-
-// The sequence that holds position x of the line, which is inside it; `base`: where it begins.
-__device__ __forceinline__ int WeighFind(const WeighParams &p, int lane, int x, int &base)
-{
-    base = 0;
-    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int u = 0;
-        if (b0 + lane < p.seqs) {
-            const WeighSeq s = LoadSeq(p, b0 + lane);
-            if (s.cols > 0) u = p.HKV * WeighLine(p, s).Head();
+    // The sequence that holds unit x, which there is; `base`: the first of it.
+    __device__ __forceinline__ int Find(int x, int &base, WeighSeq &s)
+    {
+        base = 0;
+        for (int b0 = 0; b0 < p.seqs; b0 += 64) {
+            if (p.seqs > 64) {
+                mine = LoadSeq(p, min(b0 + lane, p.seqs - 1));
+                u = Units(mine, b0 + lane);
+            }
+            const int incl = WaveScan(u, lane) + base;
+            const uint64_t above = __ballot(incl > x);
+            const int at = above != 0 ? __builtin_ctzll(above) : 63;
+            base = Uni(__shfl(incl - (above != 0 ? u : 0), at, 64));
+            if (above == 0) continue;
+            const auto of = [&](int v) { return Uni(__shfl(v, at, 64)); };
+            s = WeighSeq{of(mine.first), of(mine.rows), of(mine.n), of(mine.skip),
+                         of(mine.len),   of(mine.total), of(mine.cols), of(mine.entry)};
+            return b0 + at;
         }
-        const int incl = WaveScan(u, lane) + base;
-        const uint64_t above = __ballot(incl > x);
-        const int at = above != 0 ? __builtin_ctzll(above) : 63;
-        base = Uni(__shfl(incl - (above != 0 ? u : 0), at, 64));
-        if (above != 0) return b0 + at;
+        s = LoadSeq(p, 0);
+        return 0;
     }
-    return 0;
-}
+};
 
 // A wave's own LDS writes before its other lanes' reads of them.
 __device__ __forceinline__ void WaveLdsOrder()
@@ -299,14 +310,14 @@ WeighKernel(WeighParams p)
     __shared__ __attribute__((aligned(16))) uint2 masks[4][32];      // and which of its keys they see
     const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
     const int hf = lane >> 5;
-    const int total = WeighTotal(p, lane);
-    const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+    WeighPlan plan(p, lane, [&](const WeighSeq &s) { return p.HKV * WeighLine(p, s).Head(); });
+    const int share = (plan.total + int(gridDim.x) - 1) / int(gridDim.x);
     int x = int(blockIdx.x) * share;
-    const int x_end = min(x + share, total);
+    const int x_end = min(x + share, plan.total);
     if (x >= x_end) return;
     int base;
-    int b = WeighFind(p, lane, x, base);
-    WeighSeq sq = LoadSeq(p, b);
+    WeighSeq sq;
+    int b = plan.Find(x, base, sq);
     WeighLine line(p, sq);
     const bool causal = PLAIN || p.tree == nullptr || p.path != nullptr;
     const int qaddr = (lane & 31) * D + KSlot<D>(lane & 31, hf) * 8;  // step dc: XOR 16 dc
@@ -538,30 +549,14 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
     const int lane = int(threadIdx.x) & 63, wave = Uni(int(threadIdx.x) >> 6);
     const int hf = lane >> 5, l32 = lane & 31;
     const auto blocks_of = [&](const WeighSeq &s) { return (s.cols + 31) / 32; };
-    int total = 0;
-    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        int u = b0 + lane < p.seqs ? p.HKV * blocks_of(LoadSeq(p, b0 + lane)) : 0;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
-        total += Uni(u);
-    }
-    const int waves = 4 * int(gridDim.x), share = (total + waves - 1) / waves;
+    WeighPlan plan(p, lane, [&](const WeighSeq &s) { return p.HKV * blocks_of(s); });
+    const int waves = 4 * int(gridDim.x), share = (plan.total + waves - 1) / waves;
     int x = (4 * int(blockIdx.x) + wave) * share;
-    const int x_end = min(x + share, total);
+    const int x_end = min(x + share, plan.total);
     if (x >= x_end) return;
-    int b = 0, base = 0;
-    for (int b0 = 0; b0 < p.seqs; b0 += 64) {
-        const int u = b0 + lane < p.seqs ? p.HKV * blocks_of(LoadSeq(p, b0 + lane)) : 0;
-        const int incl = WaveScan(u, lane) + base;
-        const uint64_t above = __ballot(incl > x);
-        const int at = above != 0 ? __builtin_ctzll(above) : 63;
-        base = Uni(__shfl(incl - (above != 0 ? u : 0), at, 64));
-        if (above != 0) {
-            b = b0 + at;
-            break;
-        }
-    }
-    WeighSeq sq = LoadSeq(p, b);
+    int base;
+    WeighSeq sq;
+    int b = plan.Find(x, base, sq);
     const bool causal = PLAIN || p.tree == nullptr || p.path != nullptr;
     const int kaddr = l32 * D + KSlot<D>(l32, hf) * 8;  // step dc: XOR 16 dc
     while (x < x_end) {
@@ -678,13 +673,13 @@ __global__ void __launch_bounds__(256) StepKernel(WeighParams p)
 __global__ void __launch_bounds__(kWeighKeys) WeighJoinKernel(WeighParams p)
 {
     const int lane = int(threadIdx.x) & 63;
-    const int total = WeighTotal(p, lane);
-    const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+    WeighPlan plan(p, lane, [&](const WeighSeq &s) { return p.HKV * WeighLine(p, s).Head(); });
+    const int share = (plan.total + int(gridDim.x) - 1) / int(gridDim.x);
     const int x0 = int(blockIdx.x) * share, x1 = x0 + share;
-    if (x1 >= total) return;
+    if (x1 >= plan.total) return;
     int base;
-    const int b = WeighFind(p, lane, x1 - 1, base);
-    const WeighSeq sq = LoadSeq(p, b);
+    WeighSeq sq;
+    const int b = plan.Find(x1 - 1, base, sq);
     const WeighPiece pc = PieceAt(p, WeighLine(p, sq), b, base, x1 - 1);
     const int end = pc.start + pc.places;
     if (pc.start < x0 || end <= x1) return;
