@@ -216,6 +216,25 @@ def test_accepted_paths(gpu, tree, last):
     check_weigh(x, 1, w[1], old[1], [0, 1, 2, 3], lse.float(), paths=paths, last=last)
 
 
+@pytest.mark.parametrize("form", ["causal", "tree", "path"])
+@pytest.mark.parametrize("HQ,HKV", [(8, 1), (2, 1)])
+def test_more_sequences_than_a_wave_has_lanes(gpu, form, HQ, HKV):
+    """130 of them, in the form for many rows and the one for few."""
+    announce("weigh 130 %s %d" % (form, HQ))
+    rng = random.Random(130)
+    lens, news = [rng.randint(0, 90) for _ in range(130)], [rng.choice((0, 1, 5, 13)) for _ in range(130)]
+    x = Batch(130, lens, news, HQ, HKV, 64, page=8, layers=1, tree=form != "causal")
+    lse, _ = x.lse(0, x.D ** -0.5)
+    entry = list(range(130))[::-1]
+    w = torch.rand(130, HKV, 105, device="cuda", generator=x.g)
+    old, kw, paths = w.clone(), {}, None
+    if form == "path":
+        paths = [sorted(rng.sample(range(n), rng.randint(0, n))) for n in news]
+        kw = dict(path=ints([p + [-1] * (13 - len(p)) for p in paths]), path_lens=ints([len(p) for p in paths]))
+    weigh(x, 0, w, lse.float(), ints(entry), **kw)
+    check_weigh(x, 0, w, old, entry, lse.float(), paths=paths)
+
+
 @pytest.mark.parametrize("rows", ["few", "many"])
 def test_narrow_weights_and_odd_batches(gpu, rows):
     """Columns for some of the tokens only; starts that do not ascend and lengths that are
