@@ -22,11 +22,12 @@
 // (from the top: the steps up to there are a few hundred operations). After
 // kSumRounds such launches a single workgroup makes what sums are left.
 //
-// What bounds it, on an MI355X: the 64-bit exponentials of 16-bit logits (32
-// chains of up to 7 over 152064 tokens, 27 million values, 55 MB: the first launch
-// 34 us, 27 without the exponentials, 11 for the bytes at a copy's rate); HBM,
-// nearly, with 32-bit ones (16 trees of up to 24, 173 MB in 50 us); the launches
-// and the last workgroups' own steps for one sequence of 5 rows (12 us and 10).
+// What bounds it, on an MI355X: for many rows the first launch's vector work, the
+// 64-bit exponentials with their conversions and sums. 16 trees of up to 24 over
+// 151936 tokens, 43 million values, take 61 us with bf16 logits (87 MB) and with
+// fp32 ones (173), 50 of them here; 32 chains of up to 7, 27 million, 34 (27 without
+// the exponentials, 11 for the bytes at a copy's rate). For one sequence of 5 rows
+// the launches and the last workgroups' own steps (12 us and 10).
 #include <algorithm>
 
 #include "kr_paged.h"
@@ -36,7 +37,8 @@ namespace kr {
 namespace {
 
 constexpr int kPiece = 8192;    // values of a piece of a row: 32 a thread (of the chains above: pieces of 4096
-                                // 41 us for 33; 512 threads 38 for 34, 1024 57)
+                                // 41 us for 33; 512 threads 38 for 34, 1024 57; of 16384 the whole call 53.6
+                                // for 51.2, the trees 59.7 for 61.4)
 constexpr int kEndPiece = 2048; // of a sequence's last row: 8 a thread
 constexpr int kMostNew = 1024;  // tokens of a sequence
 // Counters of a sequence, a line of memory: arrivals at one line wait for each
