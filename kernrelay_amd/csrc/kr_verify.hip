@@ -297,11 +297,7 @@ struct WalkLds {
     }
 };
 
-// What a walk does where it needs the sum over the vocabulary after a refusal:
-// it never does (one draft a row, or not drawn); it is the first one, and stops;
-// it goes on behind sums that were made meanwhile, and stops at the next one; it
-// makes them.
-enum { kNoSums, kFirst, kResume, kMakes };
+#include "kr_walk.inc"
 
 // Down the drafts of sequence b, by NT threads that all take the same steps.
 template <int XT, int QT, int NT, int SUMS>
@@ -373,69 +369,35 @@ __device__ __forceinline__ void Walk(const VerifyParams &p, int b, const VerifyS
         l.chance[i] = q;
     }
     __syncthreads();
-    int cur = 0, len = 1, refused = 0;
-    while (len < p.width) {
-        refused = 0;
-        double rest = 1.0;  // (drafts that were not drawn)
-        int next = -1, gone = -1;
-        for (int i0 = (cur + 1) / 64 * 64; i0 < sq.n && next < 0; i0 += 64) {
-            uint64_t hit = __ballot(i0 + lane < sq.n && i0 + lane > cur && l.above[min(i0 + lane, sq.n - 1)] == cur);
-            while (hit != 0 && next < 0) {
-                const int i = Uni(i0 + __builtin_ctzll(hit));
-                hit &= hit - 1;
-                bool ok;
-                if (QT == kNone) {
-                    ok = double(l.u[i]) * rest < l.prob[i];
-                    rest = fmax(rest - l.prob[i], 0.0);
-                } else {
-                    if (SUMS != kNoSums && refused > 0) {
-                        // the sum after the last refusal, over the vocabulary
-                        double sum = SUMS == kFirst ? -1.0 : GetDev(p.after + sq.first + gone);
-                        if (SUMS != kMakes && sum < 0.0) {
-                            for (int k = tid; k + 1 < refused; k += NT) PutDev(p.totals + sq.first + k, l.totals[k]);
-                            if (tid == 0) p.ends[b] = SeqEnd{cur, refused, gone, 0, l.stats[cur]};
-                            return;
-                        }
-                        if (SUMS == kMakes && sum < 0.0) {
-                            const RowPart s = l.stats[cur];
-                            const int64_t row = sq.first + cur;
-                            const double inv = 1.0 / s.sum;
-                            sum = 0.0;
-                            for (int v = tid * 8; v < p.vocab; v += NT * 8) {
-                                const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
-                                const Raw8<QL> q = Load8<QL>(p.draft, row * p.ld_draft, v, p.vocab, 0);
+    const auto known = [&](int gone) { return GetDev(p.after + sq.first + gone); };
+    const auto make = [&](int cur, int refused) {
+        double sum = 0.0;
+        if constexpr (SUMS == kMakes) {
+            const RowPart s = l.stats[cur];
+            const int64_t row = sq.first + cur;
+            const double inv = 1.0 / s.sum;
+            for (int v = tid * 8; v < p.vocab; v += NT * 8) {
+                const Raw8<XT> x = Load8<XT>(p.logits, row * p.ld_logits, v, p.vocab, Val<XT>::kLow);
+                const Raw8<QL> q = Load8<QL>(p.draft, row * p.ld_draft, v, p.vocab, 0);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    if (s.top == -INFINITY) continue;
-                                    double was;
-                                    const double w =
-                                        Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, s.top, s.at, c) * inv;
-                                    sum += Left(w, Chance(Val<QL>::Load(q.v[e])), l.totals, refused, was);
-                                }
-                            }
-                            sum = BlockSumD<NT>(sum, part);
-                        }
-                        if (tid == 0) l.totals[refused - 1] = sum;
-                        __syncthreads();
-                    }
-                    double r = l.prob[i];
-                    for (int k = 0; SUMS != kNoSums && k < refused; ++k)
-                        r = l.totals[k] > 0.0 ? fmax(r - double(l.chance[i]), 0.0) / l.totals[k] : r;
-                    ok = double(l.u[i]) * double(l.chance[i]) < r;
-                }
-                if (ok) {
-                    next = i;
-                } else {
-                    ++refused;
-                    gone = i;
+                for (int e = 0; e < 8; ++e) {
+                    if (s.top == -INFINITY) continue;
+                    double was;
+                    const double w = Weight(pow2, Logit(Val<XT>::Load(x.v[e])), v + e, s.top, s.at, c) * inv;
+                    sum += Left(w, Chance(Val<QL>::Load(q.v[e])), l.totals, refused, was);
                 }
             }
+            sum = BlockSumD<NT>(sum, part);
         }
-        if (next < 0) break;
-        if (tid == 0) p.path[b * p.ld_path + len] = next;
-        refused = 0;
-        cur = next;
-        ++len;
+        return sum;
+    };
+    const WalkEnd at = WalkDown<QT != kNone, SUMS>(l, sq.n, p.width, known, make,
+                                                  [&](int len, int i) { p.path[b * p.ld_path + len] = i; });
+    const int cur = at.cur, len = at.len, refused = at.refused;
+    if (at.waits >= 0) {
+        for (int k = tid; k + 1 < refused; k += NT) PutDev(p.totals + sq.first + k, l.totals[k]);
+        if (tid == 0) p.ends[b] = SeqEnd{cur, refused, at.waits, 0, l.stats[cur]};
+        return;
     }
     if (tid == 0) {
         p.path[b * p.ld_path] = 0;
