@@ -306,9 +306,11 @@ class PagedCache:
         tokens the first `sinks`, the last `recent` and those with the largest
         weights stay (ops.cache_evict, of every layer and head by itself); the
         pages behind them are free again. weights: a handle (ops.make_weights)
-        whose entries are these sequences', in this order. Positions of later
-        tokens go on as if nothing had gone. Batches of the sequences are out of
-        date afterwards. Returns keep [layers, seqs, heads, budget]."""
+        whose entries are these sequences', in this order: every one that loses
+        tokens must have one of its own (the entry vector is read back for that, so
+        the call waits for the stream). Positions of later tokens go on as if
+        nothing had gone. Batches of the sequences are out of date afterwards.
+        Returns keep [layers, seqs, heads, budget]."""
         import torch
         self._current()
         seqs = list(seqs)
@@ -324,6 +326,11 @@ class PagedCache:
             raise ValueError("the weights must have an entry for each sequence")
         if any(n > budget and n > weights.width for n in tokens):
             raise ValueError("a sequence has more tokens than the weights have columns")
+        if weights.seqs is not None and any(n > budget for n in tokens):
+            # (the vector is on the device, where a sequence without weights is left alone)
+            entry = [e for e, n in zip(weights.keep[1].tolist(), tokens) if n > budget]
+            if len(set(entry)) != len(entry) or any(not 0 <= e < weights.entries for e in entry):
+                raise ValueError("each sequence that loses tokens must have an entry of its own in the weights")
         # (all that can be refused is, before the tables change)
         src, dst = self.tables.own({s: budget for s, n in zip(seqs, tokens) if n > budget})
         ops.cache_copy_pages(self.handle, src, dst)

@@ -158,3 +158,23 @@ def test_not_while_a_graph_is_captured(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(ValueError, match="captured"):
         cache.evict([a], weights(), 10)
+
+
+@pytest.mark.parametrize("entry,ok", [
+    ([2, 0, 1], True), ([2, 0, -1], True), ([2, 0, 2], True),  # (the last has too few tokens to lose any)
+    ([4, 0, 1], False), ([0, -1, 1], False), ([3, 3, 1], False),
+])
+def test_sequences_that_lose_tokens_have_weights_of_their_own(monkeypatch, entry, ok):
+    """The device leaves a sequence without weights alone, and two of one entry move
+    its weights twice: the tables would say otherwise."""
+    calls, cache, ids = make(monkeypatch, [30, 20, 7])
+    w = weights(seqs=3, keep=(None, torch.tensor(entry, dtype=torch.int32)))
+    pages = [cache.tables.pages_of(s) for s in ids]
+    if ok:
+        cache.evict(ids, w, 10)
+        assert [cache.tables.tokens(s) for s in ids] == [10, 10, 7]
+        return
+    with pytest.raises(ValueError, match="entry of its own"):
+        cache.evict(ids, w, 10)
+    assert calls.made == [] and [cache.tables.tokens(s) for s in ids] == [30, 20, 7]
+    assert [cache.tables.pages_of(s) for s in ids] == pages
