@@ -201,7 +201,8 @@ class PagedCache:
 
     def _state(self, seq):
         """What a batch's rows of a sequence depend on."""
-        return self._last.get(seq), self.tables.tokens(seq), self.tables.pages_of(seq)
+        # (the position too: an eviction can bring back the tokens and pages of before)
+        return self._last.get(seq), self.tables.tokens(seq), self.tables.position(seq), self.tables.pages_of(seq)
 
     def _current(self):
         """Before the tables change: the calls that follow must reach the pages,

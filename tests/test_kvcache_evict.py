@@ -178,3 +178,18 @@ def test_sequences_that_lose_tokens_have_weights_of_their_own(monkeypatch, entry
         cache.evict(ids, w, 10)
     assert calls.made == [] and [cache.tables.tokens(s) for s in ids] == [30, 20, 7]
     assert [cache.tables.pages_of(s) for s in ids] == pages
+
+
+def test_a_batch_that_was_kept_before_an_eviction_is_out_of_date_too(monkeypatch):
+    """As many tokens on the same pages as when it was made: accept refuses it all the
+    same, before any row moves."""
+    calls, cache, (a, b) = make(monkeypatch, [9, 7])
+    seqs, _, _ = cache.batch({a: 2, b: 3})
+    cache.commit({a: 2})
+    cache.evict([a], weights(), 9)
+    assert cache.tables.tokens(a) == 9
+    calls.made.clear()
+    for path in ([], [0], [1]):
+        with pytest.raises(ValueError, match="out of date"):
+            cache.accept(seqs, {a: path, b: [0, 1]})
+    assert calls.made == [] and (cache.tables.tokens(a), cache.tables.tokens(b)) == (9, 7)
