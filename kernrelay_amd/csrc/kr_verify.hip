@@ -838,6 +838,8 @@ kr_drafts CheckDrafts(const kr_drafts *d, const kr_seqs *s)
     const int64_t pieces = (int64_t(d->vocab) + kPiece - 1) / kPiece;
     const int64_t end_pieces = (int64_t(d->vocab) + kEndPiece - 1) / kEndPiece;
     if (pieces * d->rows >= kMaxGrid || end_pieces * s->seqs >= kMaxGrid) refuse("too many rows for one launch");
+    // (kMaxGrid is for workgroups of 256 threads, WalkKernel's have 1024)
+    if (d->draft != nullptr && d->parents != nullptr && s->seqs >= (kMaxGrid >> 2)) refuse("too many sequences");
     return *d;
 }
 

@@ -240,3 +240,17 @@ def test_verify_wrapper():
         ops.verify_drafts(s, **{**good, "logits": torch.zeros(7, 50).double()})
     with pytest.raises(RuntimeError, match="device tensors"):
         ops.verify_drafts(s, **good)
+
+
+@pytest.mark.parametrize("n,tree,ok", [(1 << 21, True, False), (1 << 22, True, False), ((1 << 21) - 1, True, True),
+                                       (1 << 22, False, True)])
+def test_sampled_trees_of_more_sequences_than_a_launch_can_count(n, tree, ok):
+    """The walk of sampled trees takes 1024 threads a sequence, of which the runtime
+    counts 2^32 and the launches here 2^31."""
+    d = drafts(draft=A + 4096, ld_draft=100, draft_dtype=ops.KR_BF16, parents=W + 16384 if tree else None)
+    s = far_seqs(seqs=n, ld_table=4)
+    # (what may be launched ends at the workspace)
+    refused(verify(d, s, nbytes=0, ncnt=0), "workspace is too small" if ok else "too many sequences")
+    b, c = ctypes.c_size_t(0), ctypes.c_int(0)
+    rc = ops._lib().kr_op_verify_drafts_workspace(d, s, b, c)
+    assert rc == 0 if ok else rc != 0
