@@ -784,15 +784,19 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     const int64_t row_tiles = std::min((tokens * p.G + 31) / 32 * s.seqs, int64_t(d.rows) * p.G / 32 + s.seqs);
     if (tiles * c.heads >= kWeighLine / (row_tiles + row_tiles * kWeighMasked / 4) || 8 * tiles * c.heads >= kWeighLine / s.seqs)
         refuse("too many rows and keys for one launch");
-    const MemSpan out = WeightsSpan(w);
     const RowSpan k = LayerSpan(c, c.k, d.layer);
-    if (Meets(out, RowsSpan(d.q, d.rows, p.ldq, int64_t(d.HQ) * c.head_dim, 2)) ||
-        Meets(out, RowsSpan(d.lse, d.rows, p.ld_lse, d.HQ, 4)) || Meets(out, MemSpan{k.p, k.width * 2}) ||
-        Meets(out, MemSpan{d.ws, int64_t(need)}) || MeetsSeqs(out, s, d.rows) ||
-        Meets(out, RowsSpan(w.entry, 1, 0, s.seqs, 4)) ||
-        Meets(out, RowsSpan(d.path, s.seqs, d.ld_path, d.path_width, 4)) ||
-        Meets(out, RowsSpan(d.path_lens, 1, 0, s.seqs, 4)))
-        refuse("the weights overlap another tensor of the call");
+    const MemSpan weights_span = WeightsSpan(w), ws{d.ws, int64_t(need)};
+    const MemSpan ins[] = {RowsSpan(d.q, d.rows, p.ldq, int64_t(d.HQ) * c.head_dim, 2),
+                           RowsSpan(d.lse, d.rows, p.ld_lse, d.HQ, 4), MemSpan{k.p, k.width * 2},
+                           RowsSpan(w.entry, 1, 0, s.seqs, 4), RowsSpan(d.path, s.seqs, d.ld_path, d.path_width, 4),
+                           RowsSpan(d.path_lens, 1, 0, s.seqs, 4)};
+    if (Meets(weights_span, ws)) refuse("the weights and the workspace overlap");
+    for (const MemSpan &in : ins) {
+        if (Meets(weights_span, in)) refuse("the weights overlap another tensor of the call");
+        if (Meets(ws, in)) refuse("the workspace overlaps another tensor of the call");
+    }
+    if (MeetsSeqs(weights_span, s, d.rows) || MeetsSeqs(ws, s, d.rows))
+        refuse("the weights or the workspace overlap the sequences' arrays");
     if (OneRowTile(tokens, p.G)) {
         const int64_t blocks = (std::min<int64_t>(cap, w.width) + 31) / 32 * c.heads * s.seqs;
         const dim3 grid(unsigned(std::min<int64_t>((blocks + 3) / 4, kStepGroups)));

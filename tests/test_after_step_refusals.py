@@ -254,3 +254,24 @@ def test_sampled_trees_of_more_sequences_than_a_launch_can_count(n, tree, ok):
     b, c = ctypes.c_size_t(0), ctypes.c_int(0)
     rc = ops._lib().kr_op_verify_drafts_workspace(d, s, b, c)
     assert rc == 0 if ok else rc != 0
+
+
+WS = FAR + (64 << 20)  # more than 32 packed rows: the workspace is written
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=WS), dict(lse=WS + (1 << 20)), dict(c=cache(k=WS, v=A)), dict(s=dict(table=WS + 64)), dict(s=dict(lens=WS + 64)),
+    dict(s=dict(starts=WS + 64)), dict(s=dict(tree=WS, tree_words=1, ld_tree=1)), dict(w=weights(entry=WS + 64)),
+    dict(w=weights(w=WS + 64)), dict(path=WS + 64, lens=FAR, width=40, ld_path=40),
+    dict(path=FAR, lens=WS + 64, width=40, ld_path=40),
+])
+def test_weigh_workspaces_on_what_the_call_reads(kw):
+    kw = dict(kw)
+    s = far_seqs(max_new=40, **kw.pop("s", {}))
+    b = ctypes.c_size_t(0)
+    c = kw.pop("c", cache())
+    assert ops._lib().kr_op_attention_paged_weigh_workspace(c, s, 8, b) == 0 and (1 << 20) < b.value < (4 << 20)
+    f = dict(q=FAR + (16 << 20), lse=FAR + (32 << 20), w=weights(), path=None, lens=None, width=0, ld_path=0)
+    f.update(kw)
+    refused(ops._lib().kr_op_attention_paged_weigh(c, 0, s, f["q"], 0, f["lse"], 0, 120, 8, 0.1, f["w"], 0, 1.0, f["path"],
+                                                   f["ld_path"], f["width"], f["lens"], WS, b.value, None), "overlap")
