@@ -357,7 +357,7 @@ int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs,
  * none), fp32 [rows, HQ], ld_lse = 0 for packed rows: what
  * kr_op_attention_paged_weigh takes. The same results and workspace; lse
  * overlaps no other tensor of the call (refused for q, out and the layer). */
-int kr_op_attention_paged_lse(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
+ * overlaps no other tensor of the call (refused for all that it passes). */
                               void *out, int64_t ldo, float *lse, int64_t ld_lse, int rows, int HQ, float scale,
                               void *ws, size_t ws_bytes, int32_t *counters, int n_counters, void *stream);
 

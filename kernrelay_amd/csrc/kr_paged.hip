@@ -1125,7 +1125,8 @@ void PagedAttnLaunch(const PagedAttnDesc &d, hipStream_t stream)
         const RowSpan k = LayerSpan(c, c.k, d.layer), v = LayerSpan(c, c.v, d.layer);
         if (Meets(lse, RowsSpan(d.q, d.rows, p.ldq, width, 2)) || Meets(lse, RowsSpan(d.out, d.rows, p.ldo, width, 2)) ||
             Meets(lse, MemSpan{k.p, k.width * 2}) || Meets(lse, MemSpan{v.p, v.width * 2}) ||
-            Meets(lse, MemSpan{p.ws, int64_t(f.ws_bytes)}) || MeetsSeqs(lse, s, d.rows))
+            Meets(lse, MemSpan{p.ws, int64_t(f.ws_bytes)}) || Meets(lse, MemSpan{p.cnt, int64_t(f.counters) * 4}) ||
+            MeetsSeqs(lse, s, d.rows))
             refuse("lse overlaps another tensor of the call");
     }
     void *args[] = {&p};

@@ -275,3 +275,14 @@ def test_weigh_workspaces_on_what_the_call_reads(kw):
     f.update(kw)
     refused(ops._lib().kr_op_attention_paged_weigh(c, 0, s, f["q"], 0, f["lse"], 0, 120, 8, 0.1, f["w"], 0, 1.0, f["path"],
                                                    f["ld_path"], f["width"], f["lens"], WS, b.value, None), "overlap")
+
+
+def test_lse_on_the_counters():
+    """(which the last piece of a row leaves zero)"""
+    s = far_seqs(seqs=256, max_new=1, ld_table=64, table_pages=64)  # (units enough for tickets)
+    b, n = ctypes.c_size_t(0), ctypes.c_int(0)
+    assert ops._lib().kr_op_attention_paged_workspace(cache(), s, 8, b, n) == 0 and n.value > 0 and b.value > 0
+    cnt = FAR + (64 << 20)
+    for lse in (cnt - 4, cnt + 4 * n.value - 4):
+        refused(ops._lib().kr_op_attention_paged_lse(cache(), 0, s, FAR, 0, FAR + (16 << 20), 0, lse, 0, 256, 8, 0.1,
+                                                     FAR + (1 << 30), b.value, cnt, n.value, None), "lse overlaps")
