@@ -356,8 +356,8 @@ int kr_op_attention_paged(const kr_cache *cache, int layer, const kr_seqs *seqs,
  * exp(scale q.k) over the keys that the row sees (-infinity where it sees
  * none), fp32 [rows, HQ], ld_lse = 0 for packed rows: what
  * kr_op_attention_paged_weigh takes. The same results and workspace; lse
- * overlaps no other tensor of the call (refused for q, out and the layer). */
  * overlaps no other tensor of the call (refused for all that it passes). */
+int kr_op_attention_paged_lse(const kr_cache *cache, int layer, const kr_seqs *seqs, const void *q, int64_t ldq,
                               void *out, int64_t ldo, float *lse, int64_t ld_lse, int rows, int HQ, float scale,
                               void *ws, size_t ws_bytes, int32_t *counters, int n_counters, void *stream);
 
