@@ -71,7 +71,7 @@ struct WeighParams {
     int64_t ldq, ld_lse, ld_table, ld_tree, ld_path;
     int64_t head_stride, w_entry, w_head;
     uint32_t page_stride, token_stride;
-    int cap, pages, table_pages, seqs, rows, max_new, tree_words, HQ, HKV, G;
+    int cap, pages, seqs, rows, max_new, tree_words, HQ, HKV, G;
     int entries, width, path_width, last;
     float scale_log2, decay;
     PageDiv div, group;  // by page_size, by G
@@ -758,7 +758,6 @@ void WeighLaunch(const WeighDesc &d, hipStream_t stream)
     p.token_stride = uint32_t(c.token_stride);
     p.cap = int(cap);
     p.pages = c.pages;
-    p.table_pages = s.table_pages;
     p.seqs = s.seqs;
     p.rows = d.rows;
     p.max_new = s.max_new;
