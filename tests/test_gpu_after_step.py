@@ -213,3 +213,31 @@ def test_forks_keep_their_tokens(gpu):
     for h in range(2):
         assert torch.equal(now[:, :, h], was[:, keep[0, 0, h].long(), h])
     assert not set(cache.tables.pages_of(a)) & set(cache.tables.pages_of(b))
+
+
+def test_entries_are_read_before_tokens_go(gpu):
+    """A sequence that would lose tokens without weights of its own is refused, and all
+    stays; with them it is trimmed."""
+    announce("evict entries")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    cache = kvcache.PagedCache(1, 30, 8, 2, 64)
+    ids = [cache.tables.add() for _ in range(2)]
+    news = dict(zip(ids, (50, 30)))
+    cache.batch(news)
+    cache.commit(news)
+    cache.k.copy_(torch.randn(cache.k.shape, device="cuda", generator=gen))
+    w = torch.rand(1, 3, 2, 60, device="cuda", generator=gen)
+    was, old = cache.k.clone(), w.clone()
+    entry = torch.zeros(2, dtype=torch.int32, device="cuda")
+    weights = ops.make_weights(w, entry=entry)
+    for bad in ([0, 3], [-1, 0], [1, 1]):
+        entry.copy_(torch.tensor(bad, dtype=torch.int32))
+        with pytest.raises(ValueError, match="entry of its own"):
+            cache.evict(ids, weights, 20, recent=4)
+    assert torch.equal(cache.k, was) and torch.equal(w, old) and [cache.tables.tokens(s) for s in ids] == [50, 30]
+    entry.copy_(torch.tensor([2, -1], dtype=torch.int32))
+    keep = cache.evict(ids, weights, 40, recent=4)  # (the second has too few tokens to lose any)
+    assert [cache.tables.tokens(s) for s in ids] == [40, 30]
+    for h in range(2):
+        assert keep[0, 0, h].tolist() == kept(old[0, 2, h].tolist(), 50, 40, 0, 4)
+        assert keep[0, 1, h].tolist() == list(range(30)) + [-1] * 10

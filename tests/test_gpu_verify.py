@@ -323,3 +323,23 @@ def test_captured_and_two_at_once(gpu):
         assert tuple(t.tolist() for t in outs[0][:3]) == want
         x.temps = [1.0] * 3
         x.check()
+
+
+def test_sums_at_several_rows(gpu):
+    """Sampled trees whose walks refuse drafts at one row, accept a later one there and
+    refuse again further down: the sums of both rows, made and known ones."""
+    announce("verify sums at several rows")
+    n, V = 85, 9001
+    x = Case(11, [n] * 24, V, F32, True, F32, temps=(1.0, 0.8), peak=1.5)
+    x.par = [[(i - 1) // 4 if i else -1 for i in range(n)] for _ in x.news]
+    x.parents = ints([p for s in x.par for p in s])
+    above = ints([b * n + max(p, 0) for b, s in enumerate(x.par) for p in s], torch.int64)
+    # half of it the target's own opinion, half another's
+    t = torch.tensor(x.temps, device="cuda").repeat_interleave(n)[:, None]
+    other = torch.randn(x.x.shape, device="cuda", generator=x.g) * 1.5
+    x.draft.copy_((torch.softmax(x.x / t, 1) + torch.softmax(other, 1)) / 2)
+    x.tokens = (x.draft[above] / -torch.rand(x.x.shape, device="cuda", generator=x.g).clamp(min=1e-30).log()).argmax(1)
+    x.check()
+    paths, _, _ = x.run()
+    later = [sum((c - 1) % 4 > 0 for c in p if c > 0) for p in paths]  # rows where another child than the first was accepted
+    assert max(later) >= 2 and sum(k >= 2 for k in later) >= 3, later
