@@ -461,8 +461,8 @@ typedef struct kr_drafts {
  * rows of the sequence from 0 on, then -1 (kr_op_cache_compact takes it; a
  * walk ends after `width` rows, with the p of the last one); path_lens
  * [seqs]; next [seqs]: -1 where a row has no logit above -infinity, or the
- * sequence no rows. max_new <= 1024; of kr_seqs starts and max_new are looked
- * at. ws: caller-owned device memory of at least the sizes that
+ * sequence no rows. max_new <= 1024; with draft and parents fewer than 2^21
+ * sequences; of kr_seqs starts and max_new are looked at. ws: caller-owned device memory of at least the sizes that
  * kr_op_verify_drafts_workspace reports (functions of host fields alone);
  * counters zero before the first call and left zero; calls sharing them must
  * be ordered. */

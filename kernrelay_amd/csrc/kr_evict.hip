@@ -15,13 +15,16 @@
 // The first launch finds the K-th largest weight by its bits from the top, then
 // lists holes and movers; the second and third move the rows.
 //
-// What bounds it, on an MI355X: the moves by HBM, the lists by the steps of their
-// selection, one after the other. Eight sequences of 1500..3000 tokens down to
-// 1000, 28 layers of 4 heads of 128: lists 19 us, holes 79, the 100 recent tokens
-// 24. One of 32000 down to 4000, 36 layers of 8 heads: 71, 99 and (501) 34. Sixteen
-// of 265..530 down to 512, the same heads: 18, 24 and (128) 42. The rows at the
-// holes are scattered, 256 bytes a key and head: 3.9 TB/s of them, where a large
-// copy reaches 4.9.
+// What bounds it, on an MI355X, on states that were not trimmed before: the moves
+// by HBM, the lists by the steps of their selection, one after the other. Eight
+// sequences of 1500..3000 tokens down to 1000, 28 layers of 4 heads of 128: lists
+// 17 us, holes 131, the 100 recent tokens 25. One of 32000 down to 4000, 36 layers
+// of 8 heads: 60, 213 and (501) 33. Sixteen of 265..530 down to 512, the same
+// heads: 18, 25 (16 MB; the rest is the reading of every place's list entry) and
+// (128) 44. The rows at the holes are scattered, 256 bytes a key and head: 4.0 and
+// 4.3 TB/s of them, where a large copy reaches 4.9. A sequence that was trimmed and
+// is trimmed again with the weights that the first time left behind moves half of
+// these rows and less.
 #include <algorithm>
 
 #include "kr_dma.h"
@@ -440,9 +443,12 @@ __device__ __forceinline__ int64_t RowAt(const EvictParams &p, const int32_t *ta
 }
 
 typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-// MoveKernel on the eight sequences above: 159 us with 4 rows, 2048 workgroups and
-// plain stores; 97 with 2 rows and stores that do not stay in the L2, 86 with 4096
-// workgroups, 79 with 4 rows.
+// All of the call, trims / the eight sequences / the long one above, on states that
+// were not trimmed before: 91 / 175 / 303 us; 2 rows 98 / 180 / 306, 8 rows 89 / 176
+// / 309; 2048 workgroups 92 / 188 / 319, 8192 92 / 169 / 298; stores that stay in
+// the L2 90 / 162 / 282. The same states trimmed again and again, where few rows
+// move: 83 / 67 / 126; 8 rows 83 / 66 / 131; 8192 workgroups 85 / 67 / 126; stores
+// that stay 85 / 70 / 133. (Chosen by the second, where all of it was timed then.)
 constexpr int kMoveRows = 4;       // rows of a thread
 constexpr int kMoveGroups = 4096;  // workgroups: 16 for each of 256 CUs
 
@@ -533,7 +539,9 @@ __global__ void __launch_bounds__(256) MoveKernel(EvictParams p, int slices)
 // The recent rows' shift. Where their new places are none of the old ones, a
 // unit is a slice as above. Otherwise it is all of a sequence and head in one
 // layer, slice by slice, each read before any of it is written: a slice's old
-// places are behind all new ones so far.
+// places are behind all new ones so far. What that costs, 6000 recent tokens of one
+// sequence that come down by 10: 48 lists of 64 values a row 103 us, 1.4 TB/s from
+// 48 workgroups; 288 of 128 a row 475 us, 3.7 TB/s.
 template <int LPR>
 __global__ void __launch_bounds__(256) ShiftKernel(EvictParams p, int slices)
 {
@@ -616,7 +624,10 @@ void EvictLaunch(const kr_cache *cache, const kr_seqs *s, const kr_weights *weig
     for (const MemSpan &out : {list, ws, ks, vs})
         if (MeetsSeqs(out, *s, 0) || Meets(out, entry)) refuse("an output overlaps what the handles read");
     if (units >= (kMaxGrid >> 2)) refuse("too many sequences");
-    // the middle of the longest sequence that there is room for
+    // the middle of the longest sequence that there is room for: lengths are on the
+    // device, so that wide tables and weights choose kernels for longer sequences than
+    // there are. (The calls at kMoveRows with room for 8192 tokens: trims 193 us for
+    // 91, one of 700 tokens 29 for 24; the eight with room for 16384, 218 for 175.)
     const int64_t middle = std::min<int64_t>(cap, w.width) - sinks - recent;
     const dim3 lists(unsigned(units), unsigned(c.layers));
     const auto select = [&](auto kern, int nt) { hipLaunchKernelGGL(kern, lists, dim3(unsigned(nt)), 0, stream, p); };

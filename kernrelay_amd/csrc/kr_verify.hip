@@ -22,12 +22,16 @@
 // (from the top: the steps up to there are a few hundred operations). After
 // kSumRounds such launches a single workgroup makes what sums are left.
 //
-// What bounds it, on an MI355X: for many rows the first launch's vector work, the
-// 64-bit exponentials with their conversions and sums. 16 trees of up to 24 over
-// 151936 tokens, 43 million values, take 61 us with bf16 logits (87 MB) and with
-// fp32 ones (173), 50 of them here; 32 chains of up to 7, 27 million, 34 (27 without
-// the exponentials, 11 for the bytes at a copy's rate). For one sequence of 5 rows
-// the launches and the last workgroups' own steps (12 us and 10).
+// What bounds it, on an MI355X: for many rows the first launch, and there no one
+// thing: the start of its waves (about 1 ns each), the loads behind it and the
+// 64-bit exponentials overlap little. 32 chains of up to 7 over 152064 tokens (bf16,
+// 176 rows, 13 thousand waves): 35 us of 49; without the exponentials 26, without
+// their sums too 26, without the maximum 24, without the loads as well, so that the
+// waves start, find their sequence, arrive and the last of them walks, 16. The bytes
+// alone are 11 at a copy's rate. 16 trees of up to 24 over 151936 (fp32, 301 rows,
+// 23 thousand waves): 49 us of 61, 42, 42, 41 and 22; the bytes 37. (All of the call
+// with bf16 logits, half the bytes: 65.) For one sequence of 5 rows the launches and
+// the last workgroups' own steps (12 us and 10; the first without its logits 7.5).
 #include <algorithm>
 
 #include "kr_paged.h"
