@@ -462,10 +462,10 @@ typedef struct kr_drafts {
  * walk ends after `width` rows, with the p of the last one); path_lens
  * [seqs]; next [seqs]: -1 where a row has no logit above -infinity, or the
  * sequence no rows. max_new <= 1024; with draft and parents fewer than 2^21
- * sequences; of kr_seqs starts and max_new are looked at. ws: caller-owned device memory of at least the sizes that
- * kr_op_verify_drafts_workspace reports (functions of host fields alone);
- * counters zero before the first call and left zero; calls sharing them must
- * be ordered. */
+ * sequences; of kr_seqs starts and max_new are looked at. ws: caller-owned
+ * device memory of at least the sizes that kr_op_verify_drafts_workspace
+ * reports (functions of host fields alone); counters zero before the first
+ * call and left zero; calls sharing them must be ordered. */
 int kr_op_verify_drafts_workspace(const kr_drafts *drafts, const kr_seqs *seqs, size_t *ws_bytes, int *counters);
 int kr_op_verify_drafts(const kr_drafts *drafts, const kr_seqs *seqs, int32_t *path, int64_t ld_path, int width,
                         int32_t *path_lens, int64_t *next, void *ws, size_t ws_bytes, int32_t *counters,
