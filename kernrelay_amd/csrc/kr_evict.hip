@@ -448,7 +448,7 @@ typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
 // / 309; 2048 workgroups 92 / 188 / 319, 8192 92 / 169 / 298; stores that stay in
 // the L2 90 / 162 / 282. The same states trimmed again and again, where few rows
 // move: 83 / 67 / 126; 8 rows 83 / 66 / 131; 8192 workgroups 85 / 67 / 126; stores
-// that stay 85 / 70 / 133. (Chosen by the second, where all of it was timed then.)
+// that stay 85 / 70 / 133. (Chosen on the latter, the only ones timed at first.)
 constexpr int kMoveRows = 4;       // rows of a thread
 constexpr int kMoveGroups = 4096;  // workgroups: 16 for each of 256 CUs
 
